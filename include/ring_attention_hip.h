@@ -360,6 +360,48 @@ int ra_bwd_call(const ra_rows* before, int32_t n_before, const ra_bwd_step_param
                 void* dk, void* dv, int64_t dkv_stride_b, int64_t dkv_stride_h, int64_t dkv_stride_l,
                 void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Terms of a whole call that take arguments of their own (the reference has neither): a learned relative position bias by
+ * buckets, with its gradient, and dropout of the attention weights.  At least one of them; they combine with every term of
+ * ra_bias but a dense block.
+ *  - table: [n_buckets, H] of table_dtype (RA_DTYPE_*), strides in elements, added to the scaled scores:
+ *    table[bucket(kv_pos - q_pos), h].  A side has n_buckets buckets of distances (two_sided: n_buckets / 2), 2 to RA_MAX_SIDE
+ *    of them; bucket b holds the distances from starts[b] up to the next start, the last one all beyond.  starts (HOST memory,
+ *    read during the call) begins with 0 and does not decrease.  Keys behind the query's position: two_sided, the buckets from
+ *    n_buckets / 2 on; else bucket 0.
+ *  - drop > 0: the weight of (query i, key j) of head b * H + h is left out where its 16 random bits are below `drop` (<= 65535), and the
+ *    others are divided by 1 - drop / 65536; the logsumexp is that of all weights.  The bits: Philox 4x32, seven rounds, key = the
+ *    seed's low and high word, counter = (j / 2, i / 4, b * H + h, 0); word i % 4, its low half for even j, its high half for odd.
+ *    i and j count from the start of the arrays.  The seed is `seed`, or, with seed_at, the device word that it points at when the
+ *    kernels run: forward and backward have to meet the same.
+ *  - operands: the type of q, k, v and dout, RA_DTYPE_BF16 or RA_DTYPE_F16; the output is of that type or fp32.
+ *  - rest (optional): what the rounded output lacks of its value, of the operands' type and with the output's strides.  ra_fwd_terms writes it, and
+ *    with it ra_bwd_terms takes rowsum(out * dout) as if the output had not been rounded.  NULL with an fp32 output. */
+#define RA_MAX_SIDE 64
+typedef struct ra_terms {
+  const void* table; /* NULL: no relative bias */
+  int64_t table_stride_bucket, table_stride_head;
+  int32_t table_dtype, n_buckets, two_sided, operands;
+  uint32_t drop; /* 0: no dropout */
+  const int32_t* starts;
+  const uint64_t* seed_at;
+  uint64_t seed;
+  void* rest;
+} ra_terms;
+
+/* ra_fwd_call / ra_bwd_call with such terms; segment ids of any length.  d_table (NULL: not wanted) receives the table's gradient,
+ * [n_buckets, H] contiguous, of table_dtype; its workspace is always part of ra_bwd_terms_workspace().  A query without a key has no
+ * part in any gradient (its dq is 0).  RA_ERR_TOO_LARGE: B * H * Lq of 2^30 or more in the backward. */
+int64_t ra_fwd_terms_workspace(const ra_fwd_step_params* p, const ra_terms* t);
+int ra_fwd_terms(const ra_rows* before, int32_t n_before, const ra_fwd_step_params* p, const ra_terms* t, void* out, int32_t out_dtype,
+                 int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, float* lse, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+int64_t ra_bwd_terms_workspace(const ra_bwd_step_params* p, const ra_terms* t);
+int ra_bwd_terms(const ra_rows* before, int32_t n_before, const ra_bwd_step_params* p, const ra_terms* t, const void* out,
+                 int32_t out_dtype, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l,
+                 int32_t grad_dtype, void* dq, int64_t dq_stride_b, int64_t dq_stride_h, int64_t dq_stride_l,
+                 void* dk, void* dv, int64_t dkv_stride_b, int64_t dkv_stride_h, int64_t dkv_stride_l, void* d_table,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Host-only, pure: 1 if every score of the (query shard, key/value shard) pair is masked
  * by the positional terms of `bias` (CAUSAL / WINDOW), so that the whole ring step is an
  * identity on the carry and may be skipped; 0 otherwise.  The reference runs such steps and

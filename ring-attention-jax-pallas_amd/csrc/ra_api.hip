@@ -68,7 +68,8 @@ int check_dims(int B, int H, int Lq, int Lk, int D, bool any_dim = false) {
   return RA_OK;
 }
 
-int check_bias(const ra_bias& b, int Lq, int Lk) {
+// any_length: the kernels test every tile of ids that do not fit their list
+int check_bias(const ra_bias& b, int Lq, int Lk, bool any_length = false) {
   const int known = RA_BIAS_CAUSAL | RA_BIAS_WINDOW | RA_BIAS_SEGMENT | RA_BIAS_PREFIX | RA_BIAS_ALIBI |
                     RA_BIAS_DENSE;
   if (b.flags & ~known) return fail(RA_ERR_BIAS, "unknown bias flag bits 0x%x", b.flags & ~known);
@@ -78,7 +79,7 @@ int check_bias(const ra_bias& b, int Lq, int Lk) {
     return fail(RA_ERR_BIAS, "causal attention does not support a prefix mask");
   if ((b.flags & RA_BIAS_SEGMENT) && (!b.q_segment_ids || !b.kv_segment_ids))
     return fail(RA_ERR_NULL, "segment bias needs q_segment_ids and kv_segment_ids");
-  if ((b.flags & RA_BIAS_SEGMENT) && (Lq > kMaxSegLen || Lk > kMaxSegLen))
+  if ((b.flags & RA_BIAS_SEGMENT) && !any_length && (Lq > kMaxSegLen || Lk > kMaxSegLen))
     return fail(RA_ERR_SHAPE, "segment bias supports shards of at most %d tokens", kMaxSegLen);
   if ((b.flags & RA_BIAS_PREFIX) && (!b.q_prefix || !b.kv_prefix))
     return fail(RA_ERR_NULL, "prefix bias needs q_prefix and kv_prefix");
@@ -767,7 +768,8 @@ bool step_on_pair(const ra_bias& bias, int B, int H, int Lq, int Lk, int D, bool
   if (wgs <= kPairSlots / 2) return true;
   return wgs <= kPairSlots ? !even : total < 56 * (int64_t)live;
 }
-PairPlan plan_fwd_pair(const ra_fwd_step_params& p) {
+// always: the kernels of ra_pair_kernels.h whatever the size (those of ra_terms.hip have no others)
+PairPlan plan_fwd_pair(const ra_fwd_step_params& p, bool always = false) {
   const int rows = (p.Lq + kPairRowsHost - 1) / kPairRowsHost;
   const int64_t heads = (int64_t)p.B * p.H, wgs = heads * rows;
   int64_t total;
@@ -778,7 +780,7 @@ PairPlan plan_fwd_pair(const ra_fwd_step_params& p) {
   // uneven rows that fill the chip less than one and a quarter times: 8 heads of 10240, 0.275 | 0.250)
   const bool even = even_rows(total, most, rows), quarter_more = wgs <= kPairSlots * 5 / 4;
   const bool nearly_one = wgs <= (even ? kPairSlots * 3 / 2 : kPairSlots * 5 / 4);
-  if (!nearly_one && long_stretches(p.bias, p.D, wgs, total, rows, (p.bias.flags & RA_BIAS_ALIBI) ? 192 : 56)) r.pair = false;
+  if (!always && !nearly_one && long_stretches(p.bias, p.D, wgs, total, rows, (p.bias.flags & RA_BIAS_ALIBI) ? 192 : 56)) r.pair = false;
   // Even rows that need up to a quarter more places than there are leave most of the chip empty in their second round: halved if they
   // are long enough for the halves' partial results.  fwd_step_kernel (D = 128) or fwd_pair_kernel unshared | in two shares, us, unmasked: 9 heads
   // of 8192, D=128 429 | 369, D=64 232 | 215, D=96 339 | 303; 18 of 4096 232 | 202, 123 | 119, 180 | 171; 5 of 16384, D=128 826 | 717; not 36 of 2048
@@ -801,9 +803,9 @@ struct TileCount {
 // dQ, likewise (dq_kernel | dq_pair_kernel): 65 tiles (32 heads of 8192) 0.70 | 0.66 ms, 66 (window 4096 of 65536, H=8) 1.36 |
 // 1.33, 129 (16 of 16384) 1.31 | 1.30, 128 (16 of 8192 x 8192) 0.64 | 0.66, 257 (32 of 32768) 10.1 | 10.4; ALiBi, 129: 1.41 | 1.32.
 // beside: dK and dV run in the same launch, if that is what comes out (plan_bwd_pair).
-PairPlan plan_dq_pair(const ra_bwd_step_params& p, const TileCount& c, bool beside) {
+PairPlan plan_dq_pair(const ra_bwd_step_params& p, const TileCount& c, bool beside, bool always) {
   PairPlan r{true, 1, std::max(c.most, 1), kHeadGroup};
-  if (long_stretches(p.bias, p.D, c.heads * c.rows, c.total, c.rows, 160)) r.pair = false;
+  if (!always && long_stretches(p.bias, p.D, c.heads * c.rows, c.total, c.rows, 160)) r.pair = false;
   else plan_split(r, c.heads, c.rows, c.total, c.most, kMinChunk, 4 * c.heads * p.Lq * p.D, p.bias, beside);
   if (one_by_one(p.bias, c.total, c.most, c.rows)) r.group = 1;
   return r;
@@ -819,13 +821,13 @@ PairPlan plan_dq_pair(const ra_bwd_step_params& p, const TileCount& c, bool besi
 // 18 of 4096 337 | 272; even rows too, but for long ones that all have a place: unmasked 18 heads of 4096 574 | 486, 9 of 8192 1089 | 958, with ALiBi 1206 |
 // 990, 10 of 8192 1112 | 1045, 16 of 4096 435 | 416, window 4096 of 8192, 8 heads 392 | 358; 8 of 8192 796 | 805, 4 of 16384 1560 | 1620.
 // Fewer slabs are shared (12 heads of 2048: 0.056 | 0.050).  beside: as for dQ.
-PairPlan plan_dkdv_pair(const ra_bwd_step_params& p, const TileCount& c, bool beside) {
+PairPlan plan_dkdv_pair(const ra_bwd_step_params& p, const TileCount& c, bool beside, bool always) {
   PairPlan r{true, 1, std::max(c.most, 1), kHeadGroup};
   const int64_t wgs = c.heads * c.rows;
   const bool one_round = wgs > kPairSlots / 2 && wgs <= kPairSlots * 5 / 4;
   int tiles = one_round ? (c.even ? 112 : 0) : (p.bias.flags & RA_BIAS_ALIBI) ? 448 : c.even ? 112 : 192;
   if (one_round && beside) tiles = c.even && wgs <= kPairSlots ? 224 : kWholeRow;
-  if (long_stretches(p.bias, p.D, one_round ? kPairSlots + 1 : wgs, c.total, c.rows, tiles)) r.pair = false;
+  if (!always && long_stretches(p.bias, p.D, one_round ? kPairSlots + 1 : wgs, c.total, c.rows, tiles)) r.pair = false;
   else if (c.heads * p.Lq + 31 >= (int64_t)1 << 30) r.pair = false;  // one 32-bit byte offset reaches both statistics of a tile's 32 rows
   else plan_split(r, c.heads, c.rows, c.total, c.most, 2 * kMinChunk, 8 * c.heads * p.Lk * p.D, p.bias, beside);
   if (one_by_one(p.bias, c.total, c.most, c.rows)) r.group = 1;
@@ -843,7 +845,7 @@ struct BwdPlan {
 // H=24 441 | 370.  Past eight rounds (at D <= 64 of 768 workgroups: documents of 2000 in 48128, causal, B=2, H=4, 7.8 of them, a pass
 // 1409 | 1296) the last one is a few per cent, and the one launch draws more power
 // without a pause (documents of 1200 + ALiBi, 29696, 24 heads: a pass 3.86 | 4.00 ms).
-BwdPlan plan_bwd_pair(const ra_bwd_step_params& p) {
+BwdPlan plan_bwd_pair(const ra_bwd_step_params& p, bool always = false) {
   const int64_t heads = (int64_t)p.B * p.H;
   TileCount q{heads, (p.Lq + kPairRowsHost - 1) / kPairRowsHost, 0, 0, false}, k{heads, (p.Lk + kPairRowsHost - 1) / kPairRowsHost, 0, 0, false};
   count_key_tiles(p.bias, p.Lq, p.Lk, q.total, q.most);
@@ -857,16 +859,17 @@ BwdPlan plan_bwd_pair(const ra_bwd_step_params& p) {
   }
   q.even = even_rows(q.total, q.most, q.rows);
   k.even = even_rows(k.total, k.most, k.rows);
-  const BwdPlan r{plan_dq_pair(p, q, true), plan_dkdv_pair(p, k, true), true};
+  const BwdPlan r{plan_dq_pair(p, q, true, always), plan_dkdv_pair(p, k, true, always), true};
   const int64_t wgs = heads * (q.rows * r.dq.n_split + k.rows * r.dkdv.n_split);
-  if (r.dq.pair && r.dkdv.pair && wgs <= (p.D <= 64 ? 12 : 8) * kPairSlots) return r;
-  return {plan_dq_pair(p, q, false), plan_dkdv_pair(p, k, false), false};
+  if (always || (r.dq.pair && r.dkdv.pair && wgs <= (p.D <= 64 ? 12 : 8) * kPairSlots)) return r;
+  return {plan_dq_pair(p, q, false, false), plan_dkdv_pair(p, k, false, false), false};
 }
 // The workspace of ra_bwd_pair: the rows' statistics, then the shares of dQ and of dK and dV.
 struct BwdSpace {
-  int64_t delta, stat, dq_part, dq_n, dkdv_part, dkdv_n, total;  // byte offsets (16-byte aligned) and the size
+  int64_t delta, stat, dq_part, dq_n, dkdv_part, dkdv_n, grad_part, total;  // byte offsets (16-byte aligned) and the size
 };
-BwdSpace bwd_space(const ra_bwd_step_params& p, const PairPlan& dq, const PairPlan& dkdv) {
+// table: a relative bias's gradient is taken
+BwdSpace bwd_space(const ra_bwd_step_params& p, const PairPlan& dq, const PairPlan& dkdv, bool table = false) {
   BwdSpace s;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -882,6 +885,7 @@ BwdSpace bwd_space(const ra_bwd_step_params& p, const PairPlan& dq, const PairPl
   s.dq_n = take(dq.n_split > 1 ? 4 * heads * tiles(p.Lq) : 0);
   s.dkdv_part = take(dkdv.n_split > 1 ? 8 * dkdv.n_split * k_rows * p.D : 0);
   s.dkdv_n = take(dkdv.n_split > 1 ? 4 * heads * tiles(p.Lk) : 0);
+  s.grad_part = take(table ? 4 * ra::kGradRow * heads * tiles(p.Lq) * dq.n_split : 0);
   s.total = at;
   return s;
 }
@@ -894,11 +898,11 @@ int64_t fwd_part_bytes(const ra_fwd_step_params& p, int n_split) {
 
 extern "C" {
 
-int ra_version(void) { return 1009; }
+int ra_version(void) { return 1010; }
 
-static int64_t fwd_pair_workspace(const ra_fwd_step_params* p, bool any_dim) {
+static int64_t fwd_pair_workspace(const ra_fwd_step_params* p, bool any_dim, bool always = false) {
   if (!p || check_dims(p->B, p->H, p->Lq, p->Lk, p->D, any_dim)) return 0;
-  const int n = plan_fwd_pair(*p).n_split;
+  const int n = plan_fwd_pair(*p, always).n_split;
   return n > 1 ? fwd_part_bytes(*p, n) : 0;
 }
 
@@ -909,8 +913,72 @@ static int check_whole_call(const char* what, int D, const ra_bias& bias) {
     return fail(RA_ERR_HEAD_DIM, "%s: head dim %d with a dense block (64 or 128)", what, D);
   return RA_OK;
 }
-static int check_fwd_step(const ra_fwd_step_params* p, bool any_dim);
-static int check_bwd_step(const ra_bwd_step_params* p, bool any_dim);
+static int check_fwd_step(const ra_fwd_step_params* p, bool any_dim, bool any_length = false);
+static int check_bwd_step(const ra_bwd_step_params* p, bool any_dim, bool any_length = false);
+
+static int check_terms(const ra_terms& t, const ra_bias& bias, int out_dtype) {
+  if (!t.table && !t.drop) return fail(RA_ERR_NULL, "ra_terms: neither a relative bias nor dropout");
+  if (bias.flags & RA_BIAS_DENSE) return fail(RA_ERR_BIAS, "a relative bias or dropout does not combine with a dense block");
+  if (t.operands != RA_DTYPE_BF16 && t.operands != RA_DTYPE_F16) return fail(RA_ERR_DTYPE, "ra_terms: unknown operand type %d", t.operands);
+  if (out_dtype != t.operands && out_dtype != RA_DTYPE_F32)
+    return fail(RA_ERR_DTYPE, "ra_terms: an output of type %d of operands of type %d", out_dtype, t.operands);
+  if (t.rest && (out_dtype == RA_DTYPE_F32 || !aligned16(t.rest)))
+    return fail(RA_ERR_ALIGN, "ra_terms: rest goes with a rounded output and must be 16-byte aligned");
+  if (t.drop > 65535) return fail(RA_ERR_BIAS, "dropout: drop = %u is above 65535", t.drop);
+  if (t.drop && reinterpret_cast<uintptr_t>(t.seed_at) % 8) return fail(RA_ERR_ALIGN, "dropout: seed_at is not 8-byte aligned");
+  if (!t.table) return RA_OK;
+  if (t.table_dtype != RA_DTYPE_BF16 && t.table_dtype != RA_DTYPE_F32 && t.table_dtype != RA_DTYPE_F16)
+    return fail(RA_ERR_DTYPE, "relative bias: unknown table dtype %d", t.table_dtype);
+  if (reinterpret_cast<uintptr_t>(t.table) % (t.table_dtype == RA_DTYPE_F32 ? 4 : 2))
+    return fail(RA_ERR_ALIGN, "relative bias: the table is not aligned to its elements");
+  const int side = t.two_sided ? t.n_buckets / 2 : t.n_buckets;
+  if (side < 2 || side > RA_MAX_SIDE || (t.two_sided && t.n_buckets % 2))
+    return fail(RA_ERR_BIAS, "relative bias: a side has 2 to %d buckets (n_buckets = %d)", RA_MAX_SIDE, t.n_buckets);
+  if (!t.starts) return fail(RA_ERR_NULL, "relative bias: starts is NULL");
+  if (t.starts[0] != 0) return fail(RA_ERR_BIAS, "relative bias: the first bucket starts at 0");
+  for (int i = 1; i < side; ++i)
+    if (t.starts[i] < t.starts[i - 1] || t.starts[i] >= (1 << 30)) return fail(RA_ERR_BIAS, "relative bias: starts must not decrease and lie below 2^30");
+  if (t.starts[side - 1] < 1) return fail(RA_ERR_BIAS, "relative bias: the last bucket starts at 1 or beyond");
+  return RA_OK;
+}
+
+// Which end of the distances holds more than half of the pairs (TermArgs::derive), by the positions of every 128th row.
+static int larger_end(const ra_terms& t, const ra_bias& bias, int Lq, int Lk) {
+  const int64_t far = t.starts[(t.two_sided ? t.n_buckets / 2 : t.n_buckets) - 1], ahead = t.two_sided ? far : 0;
+  auto keys = [&](int64_t n) { return std::min<int64_t>(std::max<int64_t>(n, 0), Lk); };
+  int64_t past = 0, future = 0, all = 0;
+  for (int64_t i = 0; i < Lq; i += kPairRowsHost) {
+    const int64_t at = bias.q_offset + std::min<int64_t>(i + kPairRowsHost / 2, Lq - 1) - bias.kv_offset;  // the middle row's position among the keys'
+    past += keys(at - far + 1);
+    future += (bias.flags & RA_BIAS_CAUSAL) ? 0 : keys(Lk - (at + ahead));
+    all += (bias.flags & RA_BIAS_CAUSAL) ? keys(at + 1) : Lk;
+  }
+  return 2 * past > all ? -1 : 2 * future > all ? 1 : 0;
+}
+
+static ra::TermArgs to_terms(const ra_terms& t, const ra_bias& bias, int Lq, int Lk) {
+  static_assert(ra::kMaxSide == RA_MAX_SIDE, "buckets of a side");
+  ra::TermArgs r;
+  memset(&r, 0, sizeof(r));
+  if (t.table) {
+    r.table = t.table;
+    r.table_sb = t.table_stride_bucket;
+    r.table_sh = t.table_stride_head;
+    r.table_dtype = t.table_dtype;
+    r.two_sided = t.two_sided != 0;
+    r.side = r.two_sided ? t.n_buckets / 2 : t.n_buckets;
+    memcpy(r.start, t.starts, sizeof(int) * r.side);
+    r.derive = larger_end(t, bias, Lq, Lk);
+  }
+  r.half = t.operands == RA_DTYPE_F16;
+  r.rest = t.rest;
+  r.drop = t.drop;
+  r.keep = 1.0f - (float)t.drop / 65536.0f;  // (exact)
+  r.inv_keep = 1.0f / r.keep;
+  r.seed_at = (const unsigned long long*)t.seed_at;
+  r.seed = t.seed;
+  return r;
+}
 
 // The conversions that go before a call, which has been checked by then: nothing is launched for one that is refused.
 struct Before {
@@ -920,18 +988,20 @@ struct Before {
 };
 
 static int fwd_pair(const Before& before, const ra_fwd_step_params* p, bool any_dim, void* out, int32_t out_dtype, int64_t out_stride_b,
-                    int64_t out_stride_h, int64_t out_stride_l, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+                    int64_t out_stride_h, int64_t out_stride_l, float* lse, void* workspace, int64_t workspace_bytes, void* stream,
+                    const ra_terms* terms = nullptr) {
   if (!p) return fail(RA_ERR_NULL, "params is NULL");
   ra_fwd_step_params c = *p;
   c.o = c.m = c.l = reinterpret_cast<float*>(uintptr_t(16));  // not used: there is no carry
-  int rc = check_fwd_step(&c, any_dim);
+  int rc = check_fwd_step(&c, any_dim, terms != nullptr);
   if (rc || (rc = check_whole_call("ra_fwd_whole", c.D, c.bias))) return rc;
+  if (terms && (rc = check_terms(*terms, c.bias, out_dtype))) return rc;
   if (!lse) return fail(RA_ERR_NULL, "ra_fwd_pair: lse is NULL");
   const RingResult r{out, nullptr, lse, out_dtype, 0, out_stride_b, out_stride_h, out_stride_l};
-  if ((rc = check_ring_result("ra_fwd_pair", r))) return rc;
-  const PairPlan plan = plan_fwd_pair(*p);
+  if ((rc = check_ring_result("ra_fwd_pair", r, terms != nullptr))) return rc;
+  const PairPlan plan = plan_fwd_pair(*p, terms != nullptr);
   if (!plan.pair) return (rc = before.launch(stream)) ? rc : fwd_passes(p, std::vector<int>{0, 1}, 1, stream, &r);
-  ra::PairFwdArgs a;
+  ra::PairFwdTermArgs a;
   memset(&a, 0, sizeof(a));
   a.q = to_arg(p->q);
   a.k = to_arg(p->k);
@@ -961,7 +1031,12 @@ static int fwd_pair(const Before& before, const ra_fwd_step_params* p, bool any_
     a.part_n = (int*)(a.part_s + rows * 4);
   }
   if ((rc = before.launch(stream))) return rc;
-  hipError_t e = ra::launch_fwd_pair(a, p->D, kernel_mode(p->bias.flags), (hipStream_t)stream);
+  if (terms) {
+    a.out_f32 = out_dtype;  // (any of them)
+    a.t = to_terms(*terms, p->bias, p->Lq, p->Lk);
+  }
+  hipError_t e = terms ? ra::launch_fwd_terms(a, p->D, (hipStream_t)stream)
+                       : ra::launch_fwd_pair(a, p->D, kernel_mode(p->bias.flags), (hipStream_t)stream);
   return e == hipSuccess ? RA_OK : hip_fail(e, "ra_fwd_pair launch");
 }
 
@@ -992,7 +1067,7 @@ int ra_step_is_skippable(const ra_bias* bias, int32_t Lq, int32_t Lk) {
   return 0;
 }
 
-static int check_fwd_step(const ra_fwd_step_params* p, bool any_dim) {
+static int check_fwd_step(const ra_fwd_step_params* p, bool any_dim, bool any_length) {
   if (!p) return fail(RA_ERR_NULL, "params is NULL");
   int rc = check_dims(p->B, p->H, p->Lq, p->Lk, p->D, any_dim);
   if (rc) return rc;
@@ -1003,10 +1078,10 @@ static int check_fwd_step(const ra_fwd_step_params* p, bool any_dim) {
   if (!aligned16(p->o)) return fail(RA_ERR_ALIGN, "o is not 16-byte aligned");
   if (!(p->sm_scale > 0.f) || p->sm_scale > 3.0e38f)
     return fail(RA_ERR_SHAPE, "sm_scale must be a positive finite number");
-  return check_bias(p->bias, p->Lq, p->Lk);
+  return check_bias(p->bias, p->Lq, p->Lk, any_length);
 }
 
-static int check_bwd_step(const ra_bwd_step_params* p, bool any_dim) {
+static int check_bwd_step(const ra_bwd_step_params* p, bool any_dim, bool any_length) {
   if (!p) return fail(RA_ERR_NULL, "params is NULL");
   int rc = check_dims(p->B, p->H, p->Lq, p->Lk, p->D, any_dim);
   if (rc) return rc;
@@ -1020,7 +1095,7 @@ static int check_bwd_step(const ra_bwd_step_params* p, bool any_dim) {
     return fail(RA_ERR_ALIGN, "gradient accumulators must be 16-byte aligned");
   if (!(p->sm_scale > 0.f) || p->sm_scale > 3.0e38f)
     return fail(RA_ERR_SHAPE, "sm_scale must be a positive finite number");
-  return check_bias(p->bias, p->Lq, p->Lk);
+  return check_bias(p->bias, p->Lq, p->Lk, any_length);
 }
 
 int ra_fwd_step_check(const ra_fwd_step_params* p) { return check_fwd_step(p, false); }
@@ -1249,36 +1324,43 @@ static int convert_args(const ra_rows* items, int32_t n_items, ra::ConvertArgs& 
   return RA_OK;
 }
 
-static int64_t bwd_pair_workspace(const ra_bwd_step_params* p, bool any_dim) {
+static int64_t bwd_pair_workspace(const ra_bwd_step_params* p, bool any_dim, const ra_terms* terms = nullptr) {
   if (!p || check_dims(p->B, p->H, p->Lq, p->Lk, p->D, any_dim)) return 0;
-  const BwdPlan plan = plan_bwd_pair(*p);
-  return bwd_space(*p, plan.dq, plan.dkdv).total;
+  const BwdPlan plan = plan_bwd_pair(*p, terms != nullptr);
+  return bwd_space(*p, plan.dq, plan.dkdv, terms && terms->table).total;
 }
 
 static int bwd_pair(const Before& before, const ra_bwd_step_params* p, bool any_dim, int grad_dtype, const void* out, int32_t out_dtype, int64_t out_stride_b,
                 int64_t out_stride_h, int64_t out_stride_l, void* dq, int64_t dq_stride_b, int64_t dq_stride_h,
                 int64_t dq_stride_l, void* dk, void* dv, int64_t dkv_stride_b, int64_t dkv_stride_h,
-                int64_t dkv_stride_l, void* workspace, int64_t workspace_bytes, void* stream) {
+                int64_t dkv_stride_l, void* workspace, int64_t workspace_bytes, void* stream, const ra_terms* terms = nullptr, void* d_table = nullptr) {
   if (!p) return fail(RA_ERR_NULL, "params is NULL");
   ra_bwd_step_params c = *p;
   c.delta = c.dq = c.dk = c.dv = reinterpret_cast<float*>(uintptr_t(16));  // not used: no accumulators
-  int rc = check_bwd_step(&c, any_dim);
+  int rc = check_bwd_step(&c, any_dim, terms != nullptr);
   if (rc || (rc = check_whole_call("ra_bwd_whole", c.D, c.bias))) return rc;
+  if (terms && (rc = check_terms(*terms, c.bias, out_dtype))) return rc;
+  if (d_table && !(terms && terms->table)) return fail(RA_ERR_NULL, "ra_bwd_terms: a gradient of no table");
+  if (d_table && reinterpret_cast<uintptr_t>(d_table) % (terms->table_dtype == RA_DTYPE_F32 ? 4 : 2))
+    return fail(RA_ERR_ALIGN, "ra_bwd_terms: d_table is not aligned to its elements");
   const bool via_bf16 = grad_dtype & RA_DTYPE_VIA_BF16;
   grad_dtype &= ~RA_DTYPE_VIA_BF16;
   const RingResult rq{dq, nullptr, nullptr, grad_dtype, 0, dq_stride_b, dq_stride_h, dq_stride_l, via_bf16};
   const RingResult rk{dk, dv, nullptr, grad_dtype, 0, dkv_stride_b, dkv_stride_h, dkv_stride_l, via_bf16};
   if ((rc = check_ring_result("ra_bwd_pair", rq, true)) || (rc = check_ring_result("ra_bwd_pair", rk, true))) return rc;
   if (!dv) return fail(RA_ERR_NULL, "ra_bwd_pair: dv is NULL");
-  const BwdPlan plan = plan_bwd_pair(*p);
+  const BwdPlan plan = plan_bwd_pair(*p, terms != nullptr);
   const PairPlan &plan_q = plan.dq, &plan_k = plan.dkdv;
-  if (!plan_k.pair && narrow(c.D)) return fail(RA_ERR_TOO_LARGE, "ra_bwd_whole: too many rows");
-  const BwdSpace sp = bwd_space(*p, plan_q, plan_k);
+  if (!plan_k.pair && (narrow(c.D) || terms)) return fail(RA_ERR_TOO_LARGE, "ra_bwd_whole: too many rows");
+  const int64_t tiles_q = (c.Lq + kPairRowsHost - 1) / kPairRowsHost, tiles_k = (c.Lk + kPairRowsHost - 1) / kPairRowsHost;
+  if (terms && (int64_t)c.B * c.H * (tiles_q * plan_q.n_split + tiles_k * plan_k.n_split) > 0x7fffffffll)
+    return fail(RA_ERR_TOO_LARGE, "ra_bwd_terms: too many workgroups for one launch");
+  const BwdSpace sp = bwd_space(*p, plan_q, plan_k, terms && terms->table);
   if (!workspace || !aligned16(workspace)) return fail(RA_ERR_ALIGN, "ra_bwd_pair: the workspace must be 16-byte aligned");
   if (workspace_bytes < sp.total) return fail(RA_ERR_SHAPE, "ra_bwd_pair: the workspace is smaller than ra_bwd_pair_workspace()");
   if (!out || !aligned16(out) || (out_stride_b % 8) || (out_stride_h % 8) || (out_stride_l % 8))
     return fail(RA_ERR_ALIGN, "ra_bwd_pair: out must be 16-byte aligned with strides that are multiples of 8");
-  if (out_dtype != RA_DTYPE_BF16 && out_dtype != RA_DTYPE_F32) return fail(RA_ERR_DTYPE, "unknown out_dtype %d", out_dtype);
+  if (!terms && out_dtype != RA_DTYPE_BF16 && out_dtype != RA_DTYPE_F32) return fail(RA_ERR_DTYPE, "unknown out_dtype %d", out_dtype);
   char* const ws = (char*)workspace;
   c.delta = (float*)(ws + sp.delta);
   ra::PairBwdArgs a;
@@ -1298,19 +1380,28 @@ static int bwd_pair(const Before& before, const ra_bwd_step_params* p, bool any_
   st.dout_d = c.D;
   st.dout_vec = 1;
   st.lse = c.lse;
+  ra::TermArgs extra;
+  if (terms) extra = to_terms(*terms, c.bias, c.Lq, c.Lk);
+  const int operand_dtype = terms ? terms->operands : RA_DTYPE_BF16;
+  if (operand_dtype == RA_DTYPE_F16) {  // (a power of two would leave fp16's range where it does not leave bf16's)
+    a.a.scale_p2 = 1.0f;
+    a.a.scale_res = a.a.scale2;
+  }
+  st.keep = terms ? extra.keep : 1.0f;
+  st.rest = terms ? extra.rest : nullptr;
   st.inv_res = 1.0f / a.a.scale_res;
   st.stat = (float*)(ws + sp.stat);
   st.delta = (float*)(ws + sp.delta);
   st.B = c.B;
   st.H = c.H;
   st.L = c.Lq;
-  int dout_dtype = RA_DTYPE_BF16;
+  int dout_dtype = operand_dtype;
   // A conversion that makes dO, row after row, is left to the statistics, which read it anyway.
   ra::ConvertArgs conv;
   const bool made = before.n == 1 && before.items && before.items[0].dst == c.dout.ptr;
   if (made && (rc = convert_args(before.items, 1, conv))) return rc;
   const ra::ConvertItem& it = conv.item[0];
-  if (made && it.dst_dtype == RA_DTYPE_BF16 && it.dst_d == c.D && it.B == c.B && it.L == c.Lq && it.H == c.H && it.dst_sh == c.D &&
+  if (made && it.dst_dtype == operand_dtype && it.dst_d == c.D && it.B == c.B && it.L == c.Lq && it.H == c.H && it.dst_sh == c.D &&
       it.dst_sl == (int64_t)c.H * c.D && it.dst_sb == (int64_t)c.Lq * c.H * c.D && c.dout.stride_h == it.dst_sh && c.dout.stride_l == it.dst_sl &&
       c.dout.stride_b == it.dst_sb) {
     st.dout = it.src;
@@ -1324,7 +1415,8 @@ static int bwd_pair(const Before& before, const ra_bwd_step_params* p, bool any_
   } else if ((rc = before.launch(stream))) {
     return rc;
   }
-  hipError_t e = ra::launch_pair_stat(st, out_dtype == RA_DTYPE_F32, dout_dtype, c.D, (hipStream_t)stream);
+  hipError_t e = terms ? ra::launch_terms_stat(st, extra.half, out_dtype == RA_DTYPE_F32, dout_dtype, c.D, (hipStream_t)stream)
+                       : ra::launch_pair_stat(st, out_dtype == RA_DTYPE_F32, dout_dtype, c.D, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "ra_bwd_pair launch");
   const std::vector<int> one{0, 1};
   const int mode = kernel_mode(c.bias.flags);
@@ -1345,6 +1437,14 @@ static int bwd_pair(const Before& before, const ra_bwd_step_params* p, bool any_
     return x;
   };
   const ra::PairBwdArgs dkdv = share(plan_k, sp.dkdv_part, sp.dkdv_n, rk), dq_args = share(plan_q, sp.dq_part, sp.dq_n, rq);
+  if (terms) {
+    if (d_table) {
+      extra.grad = d_table;
+      extra.grad_part = (float*)(ws + sp.grad_part);
+    }
+    e = ra::launch_bwd_terms(dkdv, dq_args, extra, c.D, (hipStream_t)stream);
+    return e == hipSuccess ? RA_OK : hip_fail(e, "ra_bwd_terms launch");
+  }
   auto on_pair = [&](const ra::PairBwdArgs* kv, const ra::PairBwdArgs* q) -> int {
     hipError_t err = ra::launch_bwd_pair(kv, q, c.D, mode, (hipStream_t)stream);
     return err == hipSuccess ? RA_OK : hip_fail(err, "ra_bwd_pair launch");
@@ -1407,6 +1507,25 @@ int ra_bwd_call(const ra_rows* before, int32_t n_before, const ra_bwd_step_param
                 int64_t dkv_stride_l, void* workspace, int64_t workspace_bytes, void* stream) {
   return bwd_pair({before, n_before}, p, true, grad_dtype, out, out_dtype, out_stride_b, out_stride_h, out_stride_l, dq, dq_stride_b, dq_stride_h,
                   dq_stride_l, dk, dv, dkv_stride_b, dkv_stride_h, dkv_stride_l, workspace, workspace_bytes, stream);
+}
+
+int64_t ra_fwd_terms_workspace(const ra_fwd_step_params* p, const ra_terms* t) { return t ? fwd_pair_workspace(p, true, true) : 0; }
+int64_t ra_bwd_terms_workspace(const ra_bwd_step_params* p, const ra_terms* t) { return t ? bwd_pair_workspace(p, true, t) : 0; }
+
+int ra_fwd_terms(const ra_rows* before, int32_t n_before, const ra_fwd_step_params* p, const ra_terms* t, void* out, int32_t out_dtype,
+                 int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, float* lse, void* workspace, int64_t workspace_bytes,
+                 void* stream) {
+  if (!t) return fail(RA_ERR_NULL, "terms is NULL");
+  return fwd_pair({before, n_before}, p, true, out, out_dtype, out_stride_b, out_stride_h, out_stride_l, lse, workspace, workspace_bytes, stream, t);
+}
+
+int ra_bwd_terms(const ra_rows* before, int32_t n_before, const ra_bwd_step_params* p, const ra_terms* t, const void* out, int32_t out_dtype,
+                 int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, int32_t grad_dtype, void* dq, int64_t dq_stride_b,
+                 int64_t dq_stride_h, int64_t dq_stride_l, void* dk, void* dv, int64_t dkv_stride_b, int64_t dkv_stride_h,
+                 int64_t dkv_stride_l, void* d_table, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!t) return fail(RA_ERR_NULL, "terms is NULL");
+  return bwd_pair({before, n_before}, p, true, grad_dtype, out, out_dtype, out_stride_b, out_stride_h, out_stride_l, dq, dq_stride_b, dq_stride_h,
+                  dq_stride_l, dk, dv, dkv_stride_b, dkv_stride_h, dkv_stride_l, workspace, workspace_bytes, stream, t, d_table);
 }
 
 int ra_bwd_finalize_passes(const float* acc, void* out, int64_t out_stride_pass, int64_t out_stride_b,

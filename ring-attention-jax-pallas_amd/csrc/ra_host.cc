@@ -33,6 +33,10 @@ struct Library {
   decltype(&ra_bwd_call) bwd_call;
   decltype(&ra_bwd_whole_workspace) bwd_workspace;
   decltype(&ra_convert) convert;
+  decltype(&ra_fwd_terms) fwd_terms;
+  decltype(&ra_bwd_terms) bwd_terms;
+  decltype(&ra_fwd_terms_workspace) fwd_terms_workspace;
+  decltype(&ra_bwd_terms_workspace) bwd_terms_workspace;
   PyObject* check;  // _lib.check: raises what the code says
 } g_lib;
 
@@ -94,25 +98,25 @@ void convert(Tensor* const* t, const at::ScalarType* to, int n, int64_t d) {
   if (!rows.empty()) check("ra_convert", g_lib.convert(rows.data(), (int)rows.size(), stream(device)));
 }
 
-// bf16 [b, l, h, d] as the kernels take it: unit inner stride, aligned rows that do not overlap, within the ABI's row stride.
+// bf16 (or fp16) [b, l, h, d] as the kernels take it: unit inner stride, aligned rows that do not overlap, within the ABI's row stride.
 Tensor ready(const Tensor& t) {
   const bool ok = t.stride(3) == 1 && !((t.stride(0) | t.stride(1) | t.stride(2)) & 7) && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) &&
                   t.size(3) <= t.stride(1) && t.stride(1) <= (int64_t)1 << 27;
   return ok ? t : t.contiguous();
 }
 
-bool is_operand(const Tensor& t, int64_t d) { return t.scalar_type() == at::kBFloat16 && t.size(3) == d; }
+bool is_operand(const Tensor& t, int64_t d, at::ScalarType type = at::kBFloat16) { return t.scalar_type() == type && t.size(3) == d; }
 
 // Tensors as the kernels of head dim d take them, in place.
-void operands(Tensor* const* t, int n, int64_t d) {
+void operands(Tensor* const* t, int n, int64_t d, at::ScalarType type = at::kBFloat16) {
   Tensor* todo[kMostArrays];
-  const at::ScalarType bf16[kMostArrays] = {at::kBFloat16, at::kBFloat16, at::kBFloat16, at::kBFloat16};
+  const at::ScalarType types[kMostArrays] = {type, type, type, type};
   int m = 0;
   for (int i = 0; i < n; ++i) {
-    if (is_operand(*t[i], d)) *t[i] = ready(*t[i]);
+    if (is_operand(*t[i], d, type)) *t[i] = ready(*t[i]);
     else todo[m++] = t[i];
   }
-  if (m) convert(todo, bf16, m, d);
+  if (m) convert(todo, types, m, d);
 }
 
 ra_tensor view(const Tensor& t) { return ra_tensor{t.data_ptr(), t.stride(0), t.stride(2), t.stride(1)}; }
@@ -127,11 +131,32 @@ struct Plan : torch::CustomClassHolder {
   at::Device device = at::kCPU;
   std::vector<Tensor> arrays;
 };
+// A call's relative bias and dropout; the tensors that `t` points into are the caller's.
+struct Terms {
+  ra_terms t;
+  int32_t starts[RA_MAX_SIDE];
+  int64_t q_offset, kv_offset;
+  void point_at(const Tensor& table, const Tensor& seed, const Tensor& rest) {
+    t.rest = rest.defined() ? rest.data_ptr() : nullptr;
+    t.starts = starts;
+    t.table = table.defined() ? table.data_ptr() : nullptr;
+    t.seed_at = seed.defined() ? (const uint64_t*)seed.data_ptr() : nullptr;
+  }
+  ra_bias bias_of(const Plan& p) const {
+    ra_bias b = p.bias;
+    b.q_offset = q_offset;
+    b.kv_offset = kv_offset;
+    return b;
+  }
+};
 struct Call : torch::CustomClassHolder {
   c10::intrusive_ptr<Plan> plan;
   float scale;
   int64_t dim;
   at::ScalarType given[3];
+  at::ScalarType type = at::kBFloat16;  // of the operands: fp16 arrays stay what they are under terms
+  bool with_terms = false;
+  Terms terms;
 };
 
 // q, k and v of a call: three tensors, or one buffer that holds the three converted ones.
@@ -151,21 +176,28 @@ Tensor workspace(int64_t bytes, const at::Device& device) { return bytes ? empty
 void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Output and logsumexp [1, b, h, l] of operands as the kernels take them, or as the `rows` before the call make them.
-variable_list run_forward(const Plan& p, float scale, const variable_list& kept, const ra_rows* rows, int n_rows, at::ScalarType out_dtype) {
+variable_list run_forward(const Plan& p, float scale, const variable_list& kept, const ra_rows* rows, int n_rows, at::ScalarType out_dtype,
+                          const Terms* terms = nullptr) {
   Tensor out = empty({p.B, p.Lq, p.H, p.D}, out_dtype, p.device), lse = empty({1, p.B, p.H, p.Lq}, at::kFloat, p.device);
-  const Tensor ws = workspace(p.fwd_bytes, p.device);
   ra_tensor x[3];
   operand_views(p, kept, x);
   const ra_fwd_step_params a{(int32_t)p.B, (int32_t)p.H, (int32_t)p.Lq, (int32_t)p.Lk, (int32_t)p.D, scale, x[0], x[1], x[2],
-                             nullptr, nullptr, nullptr, p.bias};
+                             nullptr, nullptr, nullptr, terms ? terms->bias_of(p) : p.bias};
+  const int64_t bytes = terms ? g_lib.fwd_terms_workspace(&a, &terms->t) : p.fwd_bytes;
+  const Tensor ws = workspace(bytes, p.device);
+  if (terms) {
+    check("ra_fwd_terms", g_lib.fwd_terms(rows, n_rows, &a, &terms->t, out.data_ptr(), row_dtype(out_dtype), p.Lq * p.H * p.D, p.D, p.H * p.D,
+                                          (float*)lse.data_ptr(), pointer(ws), bytes, stream(p.device)));
+    return {out, lse};
+  }
   check("ra_fwd_call", g_lib.fwd_call(rows, n_rows, &a, out.data_ptr(), row_dtype(out_dtype), p.Lq * p.H * p.D, p.D, p.H * p.D,
-                                      (float*)lse.data_ptr(), pointer(ws), p.fwd_bytes, stream(p.device)));
+                                      (float*)lse.data_ptr(), pointer(ws), bytes, stream(p.device)));
   return {out, lse};
 }
 
 // dq, dk and dv, of bf16 precision whatever their dtype.  dout: as the kernels take it, or as `rows` makes it.
 variable_list run_backward(Plan& p, float scale, const variable_list& kept, const Tensor& out, const Tensor& lse, const ra_rows* rows, int n_rows,
-                           const Tensor& dout, at::ScalarType dtype) {
+                           const Tensor& dout, at::ScalarType dtype, const Terms* terms = nullptr, const Tensor& d_table = {}) {
   Tensor dq, dk, dv;
   if (kept.size() == 3) {
     // laid out as the operands; dk and dv have the same strides, which the library stores them with
@@ -185,11 +217,20 @@ variable_list run_backward(Plan& p, float scale, const variable_list& kept, cons
   operand_views(p, kept, x);
   const float* l = (const float*)lse.data_ptr();
   const ra_bwd_step_params a{(int32_t)p.B, (int32_t)p.H, (int32_t)p.Lq, (int32_t)p.Lk, (int32_t)p.D, scale, x[0], x[1], x[2],
-                             view(dout), l, nullptr, nullptr, nullptr, nullptr, p.bias};
+                             view(dout), l, nullptr, nullptr, nullptr, nullptr, terms ? terms->bias_of(p) : p.bias};
+  const ra_tensor o = view(out), gq = view(dq), gk = view(dk);
+  if (terms) {
+    const int64_t bytes = g_lib.bwd_terms_workspace(&a, &terms->t);
+    const Tensor ws = workspace(bytes, p.device);
+    check("ra_bwd_terms", g_lib.bwd_terms(rows, n_rows, &a, &terms->t, o.ptr, row_dtype(out.scalar_type()), o.stride_b, o.stride_h, o.stride_l,
+                                          row_dtype(dtype) | (terms->t.operands == RA_DTYPE_BF16 ? RA_DTYPE_VIA_BF16 : 0), dq.data_ptr(), gq.stride_b, gq.stride_h,
+                                          gq.stride_l, dk.data_ptr(), dv.data_ptr(), gk.stride_b, gk.stride_h, gk.stride_l, pointer(d_table), pointer(ws),
+                                          bytes, stream(p.device)));
+    return {dq, dk, dv};
+  }
   int64_t bytes = p.bwd_bytes.load(std::memory_order_relaxed);
   if (bytes < 0) p.bwd_bytes.store(bytes = g_lib.bwd_workspace(&a), std::memory_order_relaxed);  // (sizes and bias alone decide)
   const Tensor ws = workspace(bytes, p.device);
-  const ra_tensor o = view(out), gq = view(dq), gk = view(dk);
   check("ra_bwd_call", g_lib.bwd_call(rows, n_rows, &a, o.ptr, row_dtype(out.scalar_type()), o.stride_b, o.stride_h, o.stride_l,
                                       row_dtype(dtype) | RA_DTYPE_VIA_BF16, dq.data_ptr(), gq.stride_b, gq.stride_h, gq.stride_l,
                                       dk.data_ptr(), dv.data_ptr(), gk.stride_b, gk.stride_h, gk.stride_l, pointer(ws), bytes,
@@ -197,87 +238,141 @@ variable_list run_backward(Plan& p, float scale, const variable_list& kept, cons
   return {dq, dk, dv};
 }
 
+// The forward of a node: its operands as the kernels take them are kept, with the output and the logsumexp.
+variable_list node_forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, c10::intrusive_ptr<Call> call,
+                           at::ScalarType out_dtype, at::ScalarType final_dtype, bool any_grad, const Tensor& table = {}, const Tensor& seed = {}) {
+  const Plan& p = *call->plan;
+  call->dim = q.size(3);
+  const at::ScalarType dtype = call->given[0] = q.scalar_type();
+  call->given[1] = k.scalar_type();
+  call->given[2] = v.scalar_type();
+  const bool same = dtype == call->given[1] && dtype == call->given[2];
+  if (call->with_terms && same && dtype == at::kHalf) call->type = out_dtype = at::kHalf;
+  const at::ScalarType type = call->type;
+  ra_rows rows[3];
+  int n_rows = 0;
+  variable_list kept;
+  if (same && !is_operand(q, p.D, type)) {
+    const int64_t nq = p.B * p.Lq * p.H * p.D, nk = p.B * p.Lk * p.H * p.D;
+    Tensor buf = empty({nq + 2 * nk}, type, q.device());
+    char* at = (char*)buf.data_ptr();
+    if (rows_of(rows[0], q, at, type, p.D) && rows_of(rows[1], k, at + 2 * nq, type, p.D) && rows_of(rows[2], v, at + 2 * (nq + nk), type, p.D)) {
+      n_rows = 3;
+      kept = {buf};
+    }
+  }
+  if (!n_rows) {
+    kept = {q, k, v};
+    Tensor* x[3] = {&kept[0], &kept[1], &kept[2]};
+    operands(x, 3, p.D, type);
+  }
+  Tensor rest;
+  if (call->with_terms) {
+    if (any_grad && out_dtype != at::kFloat) rest = empty({p.B, p.Lq, p.H, p.D}, type, p.device);
+    call->terms.t.operands = row_dtype(type);
+    call->terms.point_at(table, seed, rest);
+  }
+  variable_list got = run_forward(p, call->scale, kept, rows, n_rows, out_dtype, call->with_terms ? &call->terms : nullptr);
+  Tensor out = got[0], lse = got[1];
+  kept.push_back(out);
+  kept.push_back(lse);
+  if (call->with_terms) {
+    kept.push_back(table);
+    kept.push_back(seed);
+    kept.push_back(rest);
+  }
+  ctx->save_for_backward(kept);
+  ctx->mark_non_differentiable({lse});
+  ctx->set_materialize_grads(false);  // no zero fill for the logsumexp's gradient
+  const int64_t dim = call->dim;
+  ctx->saved_data["call"] = c10::IValue::make_capsule(std::move(call));
+  if (out_dtype != final_dtype || (dim != p.D && any_grad)) {
+    Tensor* t = &out;
+    convert(&t, &final_dtype, 1, dim);
+  }
+  return {out, lse};
+}
+
+// The gradients of q, k, v and, under terms, the table, where they are wanted.
+variable_list node_backward(AutogradContext* ctx, const variable_list& grads_in) {
+  const auto call = c10::static_intrusive_pointer_cast<Call>(ctx->saved_data["call"].toCapsule());
+  Plan& p = *call->plan;
+  variable_list kept = ctx->get_saved_variables();
+  Terms terms;
+  Tensor d_table;
+  if (call->with_terms) {
+    const Tensor table = kept[kept.size() - 3];
+    terms = call->terms;
+    terms.point_at(table, kept[kept.size() - 2], kept.back());
+    if (table.defined() && ctx->needs_input_grad(3)) d_table = at::empty(table.sizes(), table.options(), at::MemoryFormat::Contiguous);
+    kept.resize(kept.size() - 3);
+  }
+  const Tensor lse = kept.back(), out = kept[kept.size() - 2];
+  kept.resize(kept.size() - 2);
+  Tensor go = grads_in[0];
+  if (!go.defined()) go = at::zeros(out.sizes(), out.options().dtype(call->type));  // nothing came back for the output
+  // as the caller wants them, where that takes no cut
+  const bool direct = call->dim == p.D && row_dtype(call->given[0]) >= 0 && call->given[0] == call->given[1] && call->given[0] == call->given[2];
+  const at::ScalarType dtype = direct ? call->given[0] : call->type;
+  ra_rows rows;
+  int n_rows = 0;
+  Tensor made = go;
+  if (!is_operand(go, p.D, call->type) && go.device() == p.device) {
+    made = empty({p.B, p.Lq, p.H, p.D}, call->type, p.device);
+    n_rows = rows_of(rows, go, made.data_ptr(), call->type, p.D);
+  }
+  if (!n_rows) {
+    made = go;
+    Tensor* t = &made;
+    operands(&t, 1, p.D, call->type);
+  }
+  variable_list grads =
+      run_backward(p, call->scale, kept, out, lse, &rows, n_rows, made, dtype, call->with_terms ? &terms : nullptr, d_table);
+  Tensor* todo[3];
+  at::ScalarType to[3];
+  int n = 0;
+  for (int i = 0; i < 3; ++i)
+    if (ctx->needs_input_grad(i) && (call->dim != p.D || call->given[i] != dtype)) {
+      todo[n] = &grads[i];
+      to[n++] = call->given[i];
+    }
+  if (n) convert(todo, to, n, call->dim);
+  for (int i = 0; i < 3; ++i)
+    if (!ctx->needs_input_grad(i)) grads[i] = Tensor();
+  if (call->with_terms) grads.push_back(d_table);
+  return grads;
+}
+
 class WholeCall : public torch::autograd::Function<WholeCall> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, c10::intrusive_ptr<Plan> plan,
                                double scale, at::ScalarType out_dtype, at::ScalarType final_dtype, bool any_grad) {
-    const Plan& p = *plan;
     auto call = c10::make_intrusive<Call>();
-    call->plan = plan;
+    call->plan = std::move(plan);
     call->scale = (float)scale;
-    call->dim = q.size(3);
-    const at::ScalarType dtype = call->given[0] = q.scalar_type();
-    call->given[1] = k.scalar_type();
-    call->given[2] = v.scalar_type();
-    ra_rows rows[3];
-    int n_rows = 0;
-    variable_list kept;
-    if (dtype == call->given[1] && dtype == call->given[2] && !is_operand(q, p.D)) {
-      const int64_t nq = p.B * p.Lq * p.H * p.D, nk = p.B * p.Lk * p.H * p.D;
-      Tensor buf = empty({nq + 2 * nk}, at::kBFloat16, q.device());
-      char* at = (char*)buf.data_ptr();
-      if (rows_of(rows[0], q, at, at::kBFloat16, p.D) && rows_of(rows[1], k, at + 2 * nq, at::kBFloat16, p.D) &&
-          rows_of(rows[2], v, at + 2 * (nq + nk), at::kBFloat16, p.D)) {
-        n_rows = 3;
-        kept = {buf};
-      }
-    }
-    if (!n_rows) {
-      kept = {q, k, v};
-      Tensor* x[3] = {&kept[0], &kept[1], &kept[2]};
-      operands(x, 3, p.D);
-    }
-    variable_list got = run_forward(p, call->scale, kept, rows, n_rows, out_dtype);
-    Tensor out = got[0], lse = got[1];
-    kept.push_back(out);
-    kept.push_back(lse);
-    ctx->save_for_backward(kept);
-    ctx->mark_non_differentiable({lse});
-    ctx->set_materialize_grads(false);  // no zero fill for the logsumexp's gradient
-    ctx->saved_data["call"] = c10::IValue::make_capsule(call);
-    if (out_dtype != final_dtype || (call->dim != p.D && any_grad)) {
-      Tensor* t = &out;
-      convert(&t, &final_dtype, 1, call->dim);
-    }
-    return {out, lse};
+    return node_forward(ctx, q, k, v, std::move(call), out_dtype, final_dtype, any_grad);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
-    const auto call = c10::static_intrusive_pointer_cast<Call>(ctx->saved_data["call"].toCapsule());
-    Plan& p = *call->plan;
-    variable_list kept = ctx->get_saved_variables();
-    const Tensor lse = kept.back(), out = kept[kept.size() - 2];
-    kept.resize(kept.size() - 2);
-    Tensor go = grads_in[0];
-    if (!go.defined()) go = at::zeros(out.sizes(), out.options().dtype(at::kBFloat16));  // nothing came back for the output
-    // as the caller wants them, where that takes no cut
-    const bool direct = call->dim == p.D && row_dtype(call->given[0]) >= 0 && call->given[0] == call->given[1] && call->given[0] == call->given[2];
-    const at::ScalarType dtype = direct ? call->given[0] : at::kBFloat16;
-    ra_rows rows;
-    int n_rows = 0;
-    Tensor made = go;
-    if (!is_operand(go, p.D) && go.device() == p.device) {
-      made = empty({p.B, p.Lq, p.H, p.D}, at::kBFloat16, p.device);
-      n_rows = rows_of(rows, go, made.data_ptr(), at::kBFloat16, p.D);
-    }
-    if (!n_rows) {
-      made = go;
-      Tensor* t = &made;
-      operands(&t, 1, p.D);
-    }
-    variable_list grads = run_backward(p, call->scale, kept, out, lse, &rows, n_rows, made, dtype);
-    Tensor* todo[3];
-    at::ScalarType to[3];
-    int n = 0;
-    for (int i = 0; i < 3; ++i)
-      if (ctx->needs_input_grad(i) && (call->dim != p.D || call->given[i] != dtype)) {
-        todo[n] = &grads[i];
-        to[n++] = call->given[i];
-      }
-    if (n) convert(todo, to, n, call->dim);
-    for (int i = 0; i < 3; ++i)
-      if (!ctx->needs_input_grad(i)) grads[i] = Tensor();
-    return {grads[0], grads[1], grads[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    variable_list grads = node_backward(ctx, grads_in);
+    grads.resize(8);
+    return grads;
+  }
+};
+
+// With a relative bias or dropout.
+class TermsCall : public torch::autograd::Function<TermsCall> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<Tensor> table,
+                               c10::optional<Tensor> seed, c10::intrusive_ptr<Call> call, at::ScalarType out_dtype, at::ScalarType final_dtype,
+                               bool any_grad) {
+    return node_forward(ctx, q, k, v, std::move(call), out_dtype, final_dtype, any_grad, table.value_or(Tensor()), seed.value_or(Tensor()));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    variable_list grads = node_backward(ctx, grads_in);
+    grads.resize(9);
+    return grads;
   }
 };
 
@@ -299,6 +394,19 @@ PyObject* init(PyObject*, PyObject* args) {
   g_lib.convert = reinterpret_cast<decltype(g_lib.convert)>(static_cast<uintptr_t>(c));
   Py_INCREF(check_fn);
   Py_XSETREF(g_lib.check, check_fn);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// init_terms(address of ra_fwd_terms, of ra_bwd_terms, of ra_fwd_terms_workspace, of ra_bwd_terms_workspace)
+PyObject* init_terms(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  unsigned long long f, b, fw, bw;
+  if (!PyArg_ParseTuple(args, "KKKK", &f, &b, &fw, &bw)) return nullptr;
+  g_lib.fwd_terms = reinterpret_cast<decltype(g_lib.fwd_terms)>(static_cast<uintptr_t>(f));
+  g_lib.bwd_terms = reinterpret_cast<decltype(g_lib.bwd_terms)>(static_cast<uintptr_t>(b));
+  g_lib.fwd_terms_workspace = reinterpret_cast<decltype(g_lib.fwd_terms_workspace)>(static_cast<uintptr_t>(fw));
+  g_lib.bwd_terms_workspace = reinterpret_cast<decltype(g_lib.bwd_terms_workspace)>(static_cast<uintptr_t>(bw));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -381,6 +489,66 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     check_operands(*p, q, k, v);
     const bool any_grad = q.requires_grad() || k.requires_grad() || v.requires_grad();
     got = WholeCall::apply(q, k, v, p, scale, dtype, final_dtype, any_grad);
+  }
+  return tuple_of(std::move(got));
+  END_HANDLE_TH_ERRORS
+}
+
+// attend_terms(q, k, v, plan, scale, the kernels' output dtype, the caller's, position of the first query, of the first key, table or None,
+// two_sided, bucket starts of a side (int32s as bytes), drop, seed: an int or a tensor) -> output, logsumexp [1, b, h, l]
+PyObject* attend_terms(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 14, "attend_terms(q, k, v, plan, scale, dtype, dtype, q_offset, kv_offset, table, two_sided, starts, drop, seed)");
+  const Tensor& q = tensor_of(args[0]);
+  Tensor k = tensor_of(args[1]), v = tensor_of(args[2]);
+  auto call = c10::make_intrusive<Call>();
+  call->plan = plan_of(args[3]);
+  call->scale = (float)scale_of(args[4]);
+  call->with_terms = true;
+  const at::ScalarType dtype = dtype_of(args[5]), final_dtype = dtype_of(args[6]);
+  Terms& x = call->terms;
+  std::memset(&x, 0, sizeof(x));
+  x.q_offset = PyLong_AsLongLong(args[7]);
+  x.kv_offset = PyLong_AsLongLong(args[8]);
+  c10::optional<Tensor> with_table;
+  if (args[9] != Py_None) {
+    const Tensor& table = tensor_of(args[9]);
+    with_table = table;
+    const int two = PyObject_IsTrue(args[10]);
+    char* bytes;
+    Py_ssize_t size;
+    if (two < 0 || PyBytes_AsStringAndSize(args[11], &bytes, &size)) throw python_error();
+    TORCH_CHECK_VALUE(size % sizeof(int32_t) == 0 && size <= (Py_ssize_t)sizeof(x.starts), "up to ", RA_MAX_SIDE, " int32 starts are expected");
+    std::memcpy(x.starts, bytes, size);
+    const int64_t rows = (two ? 2 : 1) * (size / (Py_ssize_t)sizeof(int32_t));
+    TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == rows && table.size(1) == call->plan->H && row_dtype(table.scalar_type()) >= 0 &&
+                          table.device() == call->plan->device,
+                      "a table of ", rows, " x ", call->plan->H, " on the device of q is expected, not ", table.sizes(), " of ", table.scalar_type());
+    x.t.table_dtype = row_dtype(table.scalar_type());
+    x.t.table_stride_bucket = table.stride(0);
+    x.t.table_stride_head = table.stride(1);
+    x.t.n_buckets = (int32_t)rows;
+    x.t.two_sided = two;
+  }
+  x.t.drop = (uint32_t)PyLong_AsUnsignedLong(args[12]);
+  c10::optional<Tensor> seed;
+  if (THPVariable_Check(args[13])) {
+    seed = THPVariable_Unpack(args[13]);
+    TORCH_CHECK_VALUE(seed->numel() == 1 && seed->scalar_type() == at::kLong && seed->device() == call->plan->device,
+                      "a seed tensor holds one int64 on the device of q");
+  } else if (args[13] != Py_None) {
+    x.t.seed = PyLong_AsUnsignedLongLongMask(args[13]);
+  }
+  if (PyErr_Occurred()) throw python_error();
+  variable_list got;
+  {
+    pybind11::gil_scoped_release no_gil;  // (allocations may wait for the GPU)
+    for (Tensor* t : {&k, &v})
+      if (t->device() != q.device()) *t = t->to(q.device());
+    check_operands(*call->plan, q, k, v);
+    const bool any_grad =
+        at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (with_table && with_table->requires_grad()));
+    got = TermsCall::apply(q, k, v, with_table, seed, call, dtype, final_dtype, any_grad);
   }
   return tuple_of(std::move(got));
   END_HANDLE_TH_ERRORS
@@ -506,8 +674,10 @@ PyObject* require_pair(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef g_methods[] = {{"init", init, METH_VARARGS, nullptr},
+                           {"init_terms", init_terms, METH_VARARGS, nullptr},
                            {"plan", plan, METH_VARARGS, nullptr},
                            {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
+                           {"attend_terms", (PyCFunction)(void (*)(void))attend_terms, METH_FASTCALL, nullptr},
                            {"require_pair", (PyCFunction)(void (*)(void))require_pair, METH_FASTCALL, nullptr},
                            {"convert", (PyCFunction)(void (*)(void))convert_arrays, METH_FASTCALL, nullptr},
                            {"operands", (PyCFunction)(void (*)(void))operand_arrays, METH_FASTCALL, nullptr},

@@ -149,14 +149,50 @@ struct StatArgs {
   const void* dout;  // of dout_dtype, dout_d elements a row; dout_vec: whole chunks of eight lie on their own alignment
   long long dsb, dsh, dsl;
   int dout_d, dout_vec;
-  bf16_t* copy;  // where the converted dO goes, [b, l, h, D]; nullptr: it is bf16 of D elements as it is
+  bf16_t* copy;  // where the converted dO goes, [b, l, h, D], of the operands' type; nullptr: it is that, of D elements, as it is
   const float* lse;
   float inv_res;
+  float keep;  // what dropout leaves of the weights: -delta is stored times it
+  const void* rest;  // see TermArgs
   float *stat, *delta;
   int B, H, L;
   int heads, loads, n_l, n_h;  // (the launcher's)
 };
 hipError_t launch_pair_stat(const StatArgs& a, int out_f32, int dout_dtype, int D, hipStream_t stream);
+hipError_t launch_terms_stat(const StatArgs& a, bool half, int out_f32, int dout_dtype, int D, hipStream_t stream);  // (of calls with TermArgs)
+
+// The terms that need arguments of their own: a learned relative position bias by buckets, and dropout of the weights.
+constexpr int kMaxSide = 64;  // buckets of one side
+struct TermArgs {
+  // bias: table[bucket, head] of table_dtype (RA_DTYPE_*), strides in elements.  A side has `side` buckets of distances, the b-th from
+  // start[b] on; two_sided: keys behind the query take the buckets from `side` on, else all of them bucket 0.
+  const void* table;
+  long long table_sb, table_sh;
+  int table_dtype, side, two_sided;
+  int start[kMaxSide];
+  // its gradient (nullptr: none): sums of a workgroup, [B * H, tiles of 128 queries, n_split][kGradRow] (see table_grad_kernel), and where it goes
+  float* grad_part;
+  void* grad;
+  int derive;  // the end whose bucket is derived from the others (see BiasGrad): -1 the past's, 1 the future's, 0 neither
+  int half;  // the operands are fp16, not bf16
+  // What the rounded output lacks, of the operands' type and laid out as the output: the backward's delta is taken from both, as exactly as the
+  // gradients can use it (nullptr: no backward will come, or the output is fp32).
+  void* rest;
+  // dropout (drop 0: none): weights whose 16 random bits are below `drop` are left out; keep = 1 - drop / 65536
+  unsigned drop;
+  float keep, inv_keep;
+  const unsigned long long* seed_at;  // nullptr: seed
+  unsigned long long seed;
+};
+constexpr int kGradRow = 2 * kMaxSide + 2;  // a sum for each bucket, and whether a pair of the derived bucket was there
+struct PairFwdTermArgs : PairFwdArgs {
+  TermArgs t;
+};
+hipError_t launch_fwd_terms(const PairFwdTermArgs& a, int D, hipStream_t stream);
+// dK and dV beside dQ, then what has been shared, and the table's gradient
+hipError_t launch_bwd_terms(const PairBwdArgs& dkdv, const PairBwdArgs& dq, const TermArgs& t, int D, hipStream_t stream);
+// (of a launch whose rows are shared)
+hipError_t launch_pair_sum(const PairBwdArgs* dkdv, const PairBwdArgs* dq, int D, hipStream_t stream);
 
 // Arrays of rows that are converted and padded (or cut) to another head dim (ra_convert).
 constexpr int kMaxConvert = 4;

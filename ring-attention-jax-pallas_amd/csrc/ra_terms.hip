@@ -1,0 +1,61 @@
+// The pair kernels with the terms that take arguments of their own, the relative bias and dropout, and the sum of the bias's gradient.
+#include "ra_terms_launch.h"
+
+namespace ra {
+
+// The relative bias's gradient from the workgroups' sums: a workgroup per head, 256 / 2^k lanes of rows for the buckets, always in the same order.
+__global__ __launch_bounds__(256) void table_grad_kernel(const TermArgs t, const int* part_n, int B, int H, int tiles, int n_split) {
+  __shared__ float s_sum[256], s_reached[4];
+  const int n = t.two_sided ? 2 * t.side : t.side, h = blockIdx.x, tid = threadIdx.x;
+  int width = 2;
+  while (width < n) width *= 2;
+  const int u = tid % width, first = tid / width, step = 256 / width;
+  float sum = 0.f, reached = 0.f;
+  const int rows = B * tiles * n_split;
+  for (int i = first; i < rows; i += step) {
+    const int tile = i / n_split % tiles, b = i / n_split / tiles;
+    const long long at = ((long long)b * H + h) * tiles + tile;
+    if (part_n != nullptr && i % n_split >= max(part_n[at], 1)) continue;  // a share that there is not
+    const float* row = t.grad_part + (at * n_split + i % n_split) * kGradRow;
+    if (u < n) sum += row[u];
+    reached = fmaxf(reached, row[2 * kMaxSide]);
+  }
+  s_sum[tid] = sum;
+  reached = __any(reached > 0.f) ? 1.f : 0.f;
+  if ((tid & 63) == 0) s_reached[tid >> 6] = reached;
+  __syncthreads();
+  if (tid < width)
+    for (int i = 1; i < step; ++i) sum += s_sum[tid + i * width];
+  __syncthreads();
+  if (tid < n) s_sum[tid] = sum;
+  __syncthreads();
+  if (tid >= n) return;
+  // the derived bucket: minus all the others
+  const int derived = t.derive > 0 ? n - 1 : 0;
+  if (t.derive != 0 && tid == derived && s_reached[0] + s_reached[1] + s_reached[2] + s_reached[3] > 0.f) {
+    sum = 0.f;
+    for (int i = 0; i < n; ++i) sum -= i == derived ? 0.f : s_sum[i];
+  }
+  const long long at = (long long)table_row(tid, t.side) * H + h;
+  if (t.table_dtype == RA_DTYPE_F32) ((float*)t.grad)[at] = sum;
+  else if (t.table_dtype == RA_DTYPE_F16) ((_Float16*)t.grad)[at] = (_Float16)sum;
+  else ((bf16_t*)t.grad)[at] = (bf16_t)sum;
+}
+
+hipError_t launch_fwd_terms(const PairFwdTermArgs& a, int D, hipStream_t stream) {
+  return a.t.half ? launch_fwd_f16(a, D, stream) : launch_fwd<3>(a, D, stream);
+}
+
+hipError_t launch_terms_stat(const StatArgs& a, bool half, int out_f32, int dout_dtype, int D, hipStream_t stream) {
+  return half ? launch_stat_f16(a, out_f32, dout_dtype, D, stream) : launch_stat<bf16_t>(a, out_f32, dout_dtype, D, stream);
+}
+
+hipError_t launch_bwd_terms(const PairBwdArgs& dkdv, const PairBwdArgs& dq, const TermArgs& t, int D, hipStream_t stream) {
+  hipError_t e = t.half ? launch_bwd_f16(dkdv, dq, t, D, stream) : launch_bwd<3>(dkdv, dq, t, D, stream);
+  if (e != hipSuccess || (e = launch_pair_sum(&dkdv, &dq, D, stream)) != hipSuccess || t.grad_part == nullptr) return e;
+  const int tiles = (dq.a.Lq + kPairRows - 1) / kPairRows;
+  hipLaunchKernelGGL(table_grad_kernel, dim3((unsigned)dq.a.H), dim3(256), 0, stream, t, dq.part_n, dq.a.B, dq.a.H, tiles, dq.n_split);
+  return hipGetLastError();
+}
+
+}  // namespace ra

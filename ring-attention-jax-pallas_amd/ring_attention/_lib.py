@@ -24,6 +24,7 @@ RA_DTYPE_F32 = 1
 RA_DTYPE_F16 = 2  # ra_convert and the gradients of ra_bwd_whole
 RA_DTYPE_VIA_BF16 = 16
 RA_MAX_CONVERT = 4  # arrays per ra_convert
+RA_MAX_SIDE = 64  # buckets of one side of a relative bias
 
 
 class RaTensor(C.Structure):
@@ -76,6 +77,14 @@ class RaRows(C.Structure):  # (packed by csrc/ra_host.cc in the package's own ca
     ]
 
 
+class RaTerms(C.Structure):  # (filled by csrc/ra_host.cc in the package's own calls)
+    _fields_ = [
+        ("table", C.c_void_p), ("table_stride_bucket", C.c_int64), ("table_stride_head", C.c_int64),
+        ("table_dtype", C.c_int32), ("n_buckets", C.c_int32), ("two_sided", C.c_int32), ("operands", C.c_int32),
+        ("drop", C.c_uint32), ("starts", C.POINTER(C.c_int32)), ("seed_at", C.c_void_p), ("seed", C.c_uint64), ("rest", C.c_void_p),
+    ]
+
+
 EXPORTS = {
     "ra_version": (C.c_int, []),
     "ra_last_error": (C.c_char_p, []),
@@ -122,6 +131,13 @@ EXPORTS = {
     "ra_bwd_call": (C.c_int, [C.c_char_p, C.c_int32, C.c_char_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64,
                               C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
                               C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "ra_fwd_terms_workspace": (C.c_int64, [C.POINTER(RaFwdStepParams), C.POINTER(RaTerms)]),
+    "ra_fwd_terms": (C.c_int, [C.c_char_p, C.c_int32, C.POINTER(RaFwdStepParams), C.POINTER(RaTerms), C.c_void_p, C.c_int32, C.c_int64, C.c_int64,
+                               C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "ra_bwd_terms_workspace": (C.c_int64, [C.POINTER(RaBwdStepParams), C.POINTER(RaTerms)]),
+    "ra_bwd_terms": (C.c_int, [C.c_char_p, C.c_int32, C.POINTER(RaBwdStepParams), C.POINTER(RaTerms), C.c_void_p, C.c_int32, C.c_int64, C.c_int64,
+                               C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
+                               C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "ra_convert": (C.c_int, [C.c_char_p, C.c_int32, C.c_void_p]),  # ra_rows blocks, packed
     "ra_fwd_finalize_passes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64,
                                          C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int32, C.c_int32,
@@ -185,6 +201,8 @@ def host():
         lib = load()
         module.init(*(C.cast(f, C.c_void_p).value for f in (lib.ra_fwd_call, lib.ra_bwd_call, lib.ra_bwd_whole_workspace,
                                                                  lib.ra_convert)), check)
+        module.init_terms(*(C.cast(f, C.c_void_p).value for f in (lib.ra_fwd_terms, lib.ra_bwd_terms, lib.ra_fwd_terms_workspace,
+                                                                       lib.ra_bwd_terms_workspace)))
         _host = module
     return _host
 

@@ -10,19 +10,23 @@ Terms add up exactly as additive biases do (0 / -inf masks and finite ALiBi pena
     bias_fn = prefix_lm_bias() + segment_bias()           # ring.py:399-406
     bias_fn = sliding_window_bias(4096)                   # causal window
     bias_fn = segment_bias() + alibi_bias(slopes)
+    bias_fn = causal_bias() + relative_bias(table)        # learned, with a gradient
 
 The per-token arrays keep the reference's kwarg names (ring.py:411-420):
 ``q_segment_ids`` / ``kv_segment_ids``, ``q_positions`` / ``kv_positions``,
 ``q_prefix_mask`` / ``kv_prefix_mask``; the q-side ones go into ``bias_q_kwargs`` and the
 kv-side ones into ``bias_kv_kwargs``.  Positions are optional: when absent a token's
-position is its index in the global sequence.  Positions that are consecutive inside every
+position is its index in the global sequence; an int is the position of the first token, which the
+others follow.  Positions that are consecutive inside every
 shard and equal across the batch cost nothing (the kernels take one offset per shard); any other
 positions are honoured by materialising the terms per ring step as a dense block, the slow path
 of a callable ``bias_fn``.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, replace
+import functools
+import struct
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -34,6 +38,52 @@ from . import _lib
 DENSE_SUMMARY = True
 
 
+@functools.lru_cache(maxsize=64)
+def _bucket_starts(side: int, max_distance: int) -> bytes:
+    """The least distance of each of a side's buckets, as int32s.  The first half of the buckets hold a distance each; bucket
+    ``exact + i`` starts where ``exact + (side - exact) log(n / exact) / log(max_distance / exact)`` reaches it, which is, in
+    whole numbers, at the least n with ``n^k exact^i >= max_distance^i exact^k``, k = side - exact: a logarithm
+    in floating point puts distances next to a border on either side of it."""
+    exact = side // 2
+    k = side - exact
+    starts = list(range(exact + 1))
+    for i in range(1, k):
+        lo, hi = starts[-1], max_distance  # (at max_distance it holds for every i <= k)
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** k * exact ** i >= max_distance ** i * exact ** k:
+                hi = mid
+            else:
+                lo = mid + 1
+        starts.append(lo)
+    return struct.pack(f"{side}i", *starts)
+
+
+@dataclass(frozen=True)
+class RelativeBias:
+    """See ``relative_bias``.  ``table`` is None in what a plan keeps: a plan knows nothing about the values."""
+    table: Optional[torch.Tensor]  # [num_buckets, H]
+    max_distance: int = 128
+    bidirectional: bool = True
+
+    def validate(self) -> None:
+        t = self.table
+        if t is None or t.dim() != 2:
+            raise ValueError("a relative bias needs a table [num_buckets, heads]")
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise ValueError(f"the table of a relative bias must be float32, bfloat16 or float16, not {t.dtype}")
+        side = t.shape[0] // 2 if self.bidirectional else t.shape[0]
+        if not 2 <= side <= _lib.RA_MAX_SIDE or (self.bidirectional and t.shape[0] % 2):
+            raise ValueError(f"a relative bias has 2 to {_lib.RA_MAX_SIDE} buckets a side, as many on both (got a table of {t.shape[0]} rows)")
+        if not side // 2 < self.max_distance < 1 << 24:
+            raise ValueError(f"max_distance must lie above the {side // 2} distances that have a bucket of their own and below 2^24 "
+                             f"(got {self.max_distance})")
+
+    @property
+    def starts(self) -> bytes:
+        return _bucket_starts(self.table.shape[0] // (2 if self.bidirectional else 1), self.max_distance)
+
+
 @dataclass(frozen=True)
 class BiasFn:
     causal: bool = False
@@ -41,6 +91,7 @@ class BiasFn:
     segments: bool = False
     prefix: bool = False
     alibi_slopes: Optional[torch.Tensor] = None  # [H] float32
+    relative: Optional[RelativeBias] = None
 
     def __add__(self, other: "BiasFn") -> "BiasFn":
         if not isinstance(other, BiasFn):
@@ -53,8 +104,10 @@ class BiasFn:
             slopes = self.alibi_slopes + other.alibi_slopes
         else:
             slopes = self.alibi_slopes if self.alibi_slopes is not None else other.alibi_slopes
+        if self.relative is not None and other.relative is not None:
+            raise ValueError("a bias has one relative term at most")
         out = BiasFn(self.causal or other.causal, window, self.segments or other.segments,
-                     self.prefix or other.prefix, slopes)
+                     self.prefix or other.prefix, slopes, other.relative if self.relative is None else self.relative)
         out.validate()
         return out
 
@@ -82,7 +135,8 @@ class BiasFn:
 
     @property
     def needs_positions(self) -> bool:
-        return self.causal or self.prefix or self.window is not None or self.alibi_slopes is not None
+        return (self.causal or self.prefix or self.window is not None or self.alibi_slopes is not None
+                or self.relative is not None)
 
 
 def causal_bias() -> BiasFn:
@@ -118,6 +172,23 @@ def alibi_slopes(num_heads: int) -> torch.Tensor:
                         dtype=torch.float32)
 
 
+def relative_bias(table: torch.Tensor, max_distance: int = 128, bidirectional: bool = True) -> BiasFn:
+    """``table[bucket(kv_pos - q_pos), h]`` added to the scaled scores of head h: a bias that is learned for buckets of the distance
+    between key and query.
+
+    ``table`` is ``[num_buckets, heads]`` (float32, bfloat16 or float16, any strides) and receives a gradient, of its dtype and of the
+    precision that the gradients of q, k and v have.  Half of the buckets are for keys behind the query's position and half for
+    the others (``bidirectional``), or all of them for the latter and every key behind the position in bucket 0.  Of a side's n
+    buckets the first n // 2 hold one distance each and the rest grow with the logarithm of the distance up to
+    ``max_distance``; the last one holds all beyond.  At most 64 buckets a side.
+
+    It runs on whole sequences: ``ring_attention`` and its kin with positions that follow on from shard to shard (arbitrary ones, a callable bias
+    and the block functions refuse it).  Nothing of the size of the scores is stored."""
+    b = BiasFn(relative=RelativeBias(table, int(max_distance), bool(bidirectional)))
+    b.relative.validate()
+    return b
+
+
 @dataclass
 class BlockBias:
     """A BiasFn bound to ONE (query shard, key/value shard) pair: what ``bias_fn(...)``
@@ -138,6 +209,8 @@ class BlockBias:
         it: the forward step and both halves of the backward step of a pair share it)."""
         s = _lib.RaBias()
         fn = self.fn
+        if fn.relative is not None:
+            raise ValueError("a relative bias runs on whole sequences (ring_attention), not on a block")
         s.flags = fn.flags
         s.window = fn.window or 0
         s.q_offset = int(self.q_offset)

@@ -30,13 +30,14 @@ import collections
 import ctypes as C
 import functools
 import math
-from dataclasses import dataclass
+import operator
+from dataclasses import dataclass, replace
 from typing import Callable, Optional, Union
 
 import torch
 
 from . import _lib
-from .bias import BiasFn, BlockBias
+from .bias import BiasFn, BlockBias, RelativeBias
 
 # The reference's two values (ring.py:255,296-312) plus the two launch schemes by name:
 #   "pallas"    its default, "fused kernels": the library picks the launch scheme - the whole ring
@@ -68,6 +69,28 @@ class RingAxis:
     """Stands in for the mesh axis the reference shards sequences over."""
     name: str
     size: int
+
+
+@dataclass(frozen=True)
+class Dropout:
+    """Dropout of the attention weights: each is left out with probability ``p`` and the others are divided by ``1 - p``.  ``p`` lies in
+    [0, 1) and is taken in steps of 1 / 65536; with 0 nothing is left out.
+
+    Which weights are left out follows from ``seed`` and the places of query, key, head and batch row in the arrays alone, by a counter-based
+    generator (Philox 4x32 of seven rounds): the backward draws the same again, no mask is stored, and the size of the ring changes
+    nothing.  The same seed gives the same mask, so every call of a step needs its own.  ``seed`` is an int (its low 64 bits count), or a tensor of one
+    int64 on the device of q, which is read when the kernels run: a captured graph then draws a new mask in every replay for which
+    the tensor has been changed.  (It must not change between a forward and its backward; autograd refuses that.)"""
+    p: float
+    seed: Union[int, torch.Tensor] = 0
+
+    @property
+    def threshold(self) -> int:
+        """``p`` in steps of 1 / 65536, checked."""
+        p = float(self.p)
+        if not 0.0 <= p < 1.0 or round(p * 65536) > 65535:
+            raise ValueError(f"dropout must lie in [0, 1 - 2^-16] (got {self.p})")
+        return round(p * 65536)
 
 
 def _axis_size(axis_name) -> int:
@@ -439,10 +462,15 @@ class _RingPlan:
                             kw[name] = t
                     return
                 self.q_off, self.kv_off = q_off, kv_off
+            if fn.relative is not None:
+                self.fn = replace(self.fn, relative=None)  # (a call brings its own table: ``attend_terms``)
 
     def _offsets(self, pos, S, L, name):
         """One position offset per shard if the positions are consecutive inside every shard and
-        equal across the batch (what the in-kernel terms take); None otherwise."""
+        equal across the batch (what the in-kernel terms take); None otherwise.  An int: the position of the first
+        token, the others follow."""
+        if isinstance(pos, int):
+            return [_first_position(pos, S, name) + r * L for r in range(S // L)]
         if tuple(pos.shape) != (self.B, S):
             raise ValueError(f"{name} must have shape {(self.B, S)}, got {tuple(pos.shape)}")
         pos = pos.to(torch.int64)
@@ -494,6 +522,23 @@ class _RingPlan:
                 plan.q_off, plan.kv_off = self.q_off[::g], self.kv_off[::g]
                 return plan._whole() if plan.n == 1 else plan
         return self
+
+    def single(self) -> "_RingPlan":
+        """The plan of the whole sequence as one pair, for the terms that only run there."""
+        got = self.__dict__.get("_single")
+        if got is None:
+            if self.callable is not None or any(off != [off[0] + r * L for r in range(self.n)]
+                                                for off, L in ((self.q_off, self.Lq), (self.kv_off, self.Lk))):
+                raise ValueError("a relative bias and dropout need positions that follow on over the whole sequence, the same ones in "
+                                 "every batch row, and no callable bias")
+            plan = self
+            if self.n > 1:
+                plan = object.__new__(_RingPlan)
+                plan.__dict__.update({a: x for a, x in self.__dict__.items() if not a.startswith("_")})
+                plan.n, plan.Lq, plan.Lk = 1, self.n * self.Lq, self.n * self.Lk
+                plan.q_off, plan.kv_off = self.q_off[:1], self.kv_off[:1]
+            got = self.__dict__["_single"] = plan._whole()
+        return got
 
     def _whole(self) -> "_RingPlan":
         """A plan of one shard in the head dim that the whole-sequence calls take: the next multiple of 32
@@ -553,6 +598,12 @@ class _RingPlan:
             None if self.kv_seg is None else self.kv_seg[:, sl_k],
             None if self.q_pre is None else self.q_pre[:, sl_q],
             None if self.kv_pre is None else self.kv_pre[:, sl_k])
+
+
+def _first_position(pos: int, S: int, name: str) -> int:
+    if not 0 <= pos <= _lib.RA_MAX_POSITION - S:
+        raise ValueError(f"{name}: positions must lie in [0, {_lib.RA_MAX_POSITION}) (got {pos} for the first of {S})")
+    return pos
 
 
 def _positional_bias_callable(fn: BiasFn):
@@ -650,7 +701,7 @@ def _plan_for(q, k, n, bias_fn, q_kwargs, kv_kwargs) -> "_RingPlan":
     fn_key = bias_fn
     if isinstance(bias_fn, BiasFn):
         fn_key = (bias_fn.causal, bias_fn.window, bias_fn.segments, bias_fn.prefix,
-                  None if bias_fn.alibi_slopes is None else ident(bias_fn.alibi_slopes))
+                  None if bias_fn.alibi_slopes is None else ident(bias_fn.alibi_slopes), bias_fn.relative is not None)
     elif bias_fn is not None:
         fn_key = ("callable", id(bias_fn))
     kw_key = tuple(tuple(sorted((a, ident(t)) for a, t in (kw or {}).items())) for kw in (q_kwargs, kv_kwargs))
@@ -978,14 +1029,50 @@ class _RingAttentionFn(torch.autograd.Function):
 
 def ring_attention_with_lse(q, k, v, axis_name, bias_fn: Union[BiasFn, Callable, None] = None, bias_q_kwargs=None,
                             bias_kv_kwargs=None, sm_scale: Optional[float] = None,
-                            block_impl: str = "pallas", out_dtype=None):
+                            block_impl: str = "pallas", out_dtype=None, dropout: Optional[Dropout] = None):
     """``ring_attention`` that also returns the logsumexp ``[b, h, S]`` (the ``L`` residual of
-    ring.py:135)."""
-    out, lse, plan = _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, block_impl, out_dtype)
+    ring.py:135), of all weights whatever ``dropout`` leaves out."""
+    out, lse, plan = _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, block_impl, out_dtype, dropout)
     return out, lse.permute(1, 2, 0, 3).reshape(plan.B, plan.H, plan.n * plan.Lq)
 
 
-def _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, block_impl, out_dtype=None):
+_NO_TABLE = RelativeBias(None)
+
+
+def _terms_call(q, k, v, n, fn: Optional[BiasFn], q_kwargs, kv_kwargs, sm_scale, out_dtype, final_dtype, drop: int, seed):
+    """A call with a relative bias or dropout: one launch over the whole sequence (``attend_terms`` of ``csrc/ra_host.cc``).  The table, the seed and
+    positions that are given as an int are the call's own, so that a plan serves every step of a training or decoding loop."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("a relative bias and dropout cannot be traced")
+    relative = None
+    offsets = [None, None]
+    kwargs = [dict(q_kwargs or {}), dict(kv_kwargs or {})]
+    if isinstance(fn, BiasFn):
+        for i, (name, x) in enumerate((("q_positions", q), ("kv_positions", k))):
+            if isinstance(kwargs[i].get(name), int):
+                offsets[i] = _first_position(kwargs[i].pop(name), x.shape[1], name)
+        relative = fn.relative
+        if relative is not None:
+            relative.validate()
+            if relative.table.shape[1] != q.shape[2]:
+                raise ValueError(f"the table of a relative bias must have a column per head ({q.shape[2]}), got {tuple(relative.table.shape)}")
+            fn = replace(fn, relative=_NO_TABLE)
+    plan = _plan_for(q, k, n, fn, *kwargs).single()
+    if isinstance(seed, torch.Tensor):
+        if seed.numel() != 1 or seed.dtype != torch.int64 or seed.device != q.device:
+            raise ValueError(f"a dropout seed is an int or a tensor of one int64 on {q.device}")
+    elif drop:
+        seed = operator.index(seed)
+    table, two_sided, starts = None, False, None
+    if relative is not None:
+        table, two_sided, starts = relative.table.to(q.device), relative.bidirectional, relative.starts
+    q_off, kv_off = (plan_off if off is None else off for off, plan_off in zip(offsets, (plan.q_off[0], plan.kv_off[0])))
+    out, lse = _lib.host().attend_terms(q, k, v, plan.native(q), float(sm_scale), out_dtype, final_dtype, q_off, kv_off, table, two_sided, starts,
+                                        drop, seed if drop else None)
+    return out, lse, plan
+
+
+def _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, block_impl, out_dtype=None, dropout=None):
     if block_impl not in _IMPLS:
         raise ValueError(block_impl)
     if bias_fn is not None and not isinstance(bias_fn, BiasFn) and not callable(bias_fn):
@@ -1013,6 +1100,16 @@ def _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale
         out_dtype = torch.float32 if in_dtype == torch.float32 else torch.bfloat16
     if d_true > 128:
         raise ValueError("head dims above 128 are not supported")
+    if dropout is not None and not isinstance(dropout, Dropout):
+        raise TypeError("dropout must be a ring_attention.Dropout")
+    drop = 0 if dropout is None else dropout.threshold
+    if drop or (isinstance(bias_fn, BiasFn) and bias_fn.relative is not None):
+        final_dtype = out_dtype if in_dtype in (torch.float32, torch.bfloat16) else in_dtype
+        out, lse, plan = _terms_call(q, k, v, n, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, out_dtype, final_dtype, drop,
+                                     dropout.seed if drop else None)
+        if out.shape[-1] != d_true:
+            out = out[..., :d_true]
+        return out, lse, plan
     plan = _plan_for(q, k, _walked_ring_size(n, qs[1], ks[1], bias_fn), bias_fn, bias_q_kwargs,
                      bias_kv_kwargs)
     fused = _launch_whole_ring(block_impl, plan)
@@ -1031,7 +1128,8 @@ def _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale
 
 
 def ring_attention(q, k, v, axis_name, bias_fn: Union[BiasFn, Callable, None] = None, bias_q_kwargs=None,
-                   bias_kv_kwargs=None, sm_scale: Optional[float] = None, block_impl: str = "pallas"):
+                   bias_kv_kwargs=None, sm_scale: Optional[float] = None, block_impl: str = "pallas",
+                   dropout: Optional[Dropout] = None):
     """Ring attention - general (reference ``ring_attention``, ring.py:246-325).
 
     Args:
@@ -1041,32 +1139,37 @@ def ring_attention(q, k, v, axis_name, bias_fn: Union[BiasFn, Callable, None] = 
         bias_fn: optional block-wise attention bias: a ``BiasFn`` description (evaluated inside the
             kernels, masked tiles skipped) or, as in the reference, any callable
             ``bias_fn(**q_kwargs, **kv_kwargs)`` returning the additive ``[b, h | 1, lq, lk]`` block
-            of one (query shard, key/value shard) pair; no gradient flows into it (ring.py:243).
+            of one (query shard, key/value shard) pair; no gradient flows into it (ring.py:243).  Of a ``BiasFn`` the
+            table of a ``relative_bias`` has one.
         bias_q_kwargs / bias_kv_kwargs: query- / key-aligned ``[b, S, ...]`` arrays the bias needs;
             for a ``BiasFn``: ``q_segment_ids``, ``q_positions``, ``q_prefix_mask`` and their
-            ``kv_`` twins.
+            ``kv_`` twins.  Positions may be an int, that of the first token: a token behind a cache of n others has
+            ``q_positions=n``.
         sm_scale: softmax scale, 1/sqrt(d) if unspecified.
         block_impl: the reference's ``"pallas"`` (its default, ring.py:255: the library picks the
             launch scheme - the whole ring per launch unless ``bias_fn`` is a callable) and
             ``"jax"`` (one kernel launch per ring step), or the launch schemes by name: ``"hip"``
             (launch per step) and ``"hip_fused"`` (one launch for all ring passes: the kernels walk
             the shards themselves); anything else raises ``ValueError`` as the reference does
-            (ring.py:312).  Every value runs the same kernels on the same bf16 operands.
+            (ring.py:312).  Every value runs the same kernels on the same bf16 operands.  (A relative bias and dropout: one launch over the
+            whole sequence, whatever the value.)
+        dropout: a ``Dropout`` of the attention weights; none by default.  Not with a callable ``bias_fn``.
     Returns:
-        attention output ``[b, S, h, d]``; differentiable w.r.t. q, k, v.
+        attention output ``[b, S, h, d]``; differentiable w.r.t. q, k, v and the table of a relative bias.
     """
-    return _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, block_impl)[0]
+    return _attend(q, k, v, axis_name, bias_fn, bias_q_kwargs, bias_kv_kwargs, sm_scale, block_impl, dropout=dropout)[0]
 
 
 def ring_self_attention(q, k, v, mesh, pspec=None, sm_scale: Optional[float] = None,
                         causal: bool = False, segment_ids=None, positions=None, prefix_mask=None,
-                        block_impl: str = "pallas"):
+                        block_impl: str = "pallas", relative: Optional[BiasFn] = None, dropout: Optional[Dropout] = None):
     """Ring attention for self-attention (reference ``ring_self_attention``, ring.py:328-449).
 
     Supports full bidirectional attention (default), block-sparse attention via
     ``segment_ids``, causal attention (requires ``positions``) and prefix-LM attention via
     ``prefix_mask`` (requires ``positions``), and their combinations.  ``mesh`` gives the
-    ring size (``RingAxis`` or int); ``pspec`` is accepted for signature compatibility."""
+    ring size (``RingAxis`` or int); ``pspec`` is accepted for signature compatibility.  ``relative``: a learned bias
+    (``relative_bias(table, ...)``) on top; ``dropout``: a ``Dropout`` of the attention weights."""
     if causal:
         assert positions is not None, "positions are requried for causal attention"
         assert prefix_mask is None, "causal attention does not support prefix_mask"
@@ -1074,10 +1177,12 @@ def ring_self_attention(q, k, v, mesh, pspec=None, sm_scale: Optional[float] = N
         assert positions is not None, "positions are requried for prefixlm attention"
         assert not causal
     fn = BiasFn(causal=causal, segments=segment_ids is not None, prefix=prefix_mask is not None)
-    has_bias = causal or segment_ids is not None or prefix_mask is not None
+    has_bias = causal or segment_ids is not None or prefix_mask is not None or relative is not None
+    if relative is not None:
+        fn = fn + relative
     q_kw = {"q_segment_ids": segment_ids, "q_positions": positions, "q_prefix_mask": prefix_mask}
     kv_kw = {"kv_segment_ids": segment_ids, "kv_positions": positions, "kv_prefix_mask": prefix_mask}
     return ring_attention(q, k, v, mesh, bias_fn=fn if has_bias else None,
                           bias_q_kwargs=q_kw if has_bias else None,
                           bias_kv_kwargs=kv_kw if has_bias else None, sm_scale=sm_scale,
-                          block_impl=block_impl)
+                          block_impl=block_impl, dropout=dropout)
