@@ -601,6 +601,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
   __shared__ unsigned char s_flag[GENERAL ? kPairListTiles : 1];
   __shared__ int s_red[20];
   __shared__ std::conditional_t<REL, BiasLds<kBiasKeys, false>, NoLds> s_bias;
+  __shared__ __attribute__((aligned(16))) unsigned s_words[DROP ? 4 : 1][DROP ? 256 : 1];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -692,7 +693,15 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     ends = load_bias(a.t, h, kLog2e / a.scale2, s_bias);
     __syncthreads();
   }
-  if constexpr (DROP) load_seed(a.t, seed0, seed1);
+  PhiloxRow philox;
+  int pair = 0;
+  WordTurn turn = {};
+  if constexpr (DROP) {
+    load_seed(a.t, seed0, seed1);
+    philox.init(qi >> 2, hh, seed0, seed1);
+    pair = PhiloxRow::pair(lane);
+    turn.init(s_words[DROP ? wave : 0], lane);
+  }
 
   TileLoader<D, kPairKeys, DL> ldk, ldv;
   ldk.init(a.k.ptr + b * a.k.sb + h * a.k.sh, a.k.sl, a.Lk, wave, lane);
@@ -716,7 +725,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
   // pipe has room, as matrix products of four ones and a lane's own four values (a column of a 4x4 block is one lane).  us, forward, dot
   // products | matrix products: D=64 causal + ALiBi 4096, B=2, H=16 118 | 111, unmasked 8192, H=16 322 | 320; D=32 causal 8192, H=16 143 |
   // 137; D=128 causal 4096, H=16 95 | 98, documents + ALiBi 32768 1694 | 1703.
-  constexpr bool SUM_MFMA = DL <= 64 && !DROP;
+  constexpr bool SUM_MFMA = DL <= 64 || DROP;  // (a dot product between two matrix instructions holds the second one up for 11 to 19 cycles, this one for 11 a pair)
   f32x4 lr_acc = {0.f, 0.f, 0.f, 0.f};
   f32x16 oacc[DB];
 #pragma unroll
@@ -776,6 +785,19 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       if (alibi_on && !one_side) tests |= kTestAlibi;
     }
     if (!wt.plain(j)) tests |= kTestPos;
+    // Dropout's bits, of a group of eight weights and the next: word e / 2 for elements e and e + 1.  The first two groups' are made beside the
+    // scores, the others' beside the products of the groups before.
+    unsigned words[2][4], drawing[4];
+    auto draw = [&](int ks, int from, int to) {  // some of the kDraws steps for group ks
+      if constexpr (DROP) {
+#pragma unroll
+        for (int i = from; i < to; ++i) {
+          if (i < PhiloxRow::kSteps) philox.step(i, drawing, (kt0 >> 1) + 8 * ks + pair, hh, seed0, seed1);
+          else turn.run(words[ks & 1], drawing);
+        }
+      }
+    };
+    constexpr int kDraws = PhiloxRow::kSteps + 1;
     f32x16 S[2], zero;
     float beyond = 0.f, far = 0.f, far_rest = 0.f;  // what the scores of the second key block, and the exponents of all, lack
 #pragma unroll
@@ -808,6 +830,12 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     for (int op = 2; op < 2 * KS; ++op) {
       if (op + PFK < 2 * KS) kf[op + PFK] = k_frag(op + PFK);
       S[op & 1] = mma(kf[op], qf[op >> 1], S[op & 1]);
+      if constexpr (DROP) {
+        constexpr int N = 2 * KS - 2, all = 2 * kDraws;
+        const int from = all * (op - 2) / N, to = all * (op - 1) / N;
+        draw(0, min(from, kDraws), min(to, kDraws));
+        draw(1, max(from - kDraws, 0), max(to - kDraws, 0));
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
@@ -882,22 +910,9 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     // output product: group ks + 1 is worked on while the matrix unit multiplies with group ks.
     X8 pf[4];
     float rs0 = 0.f, rs1 = 0.f;
-    unsigned words[4];  // dropout's, of a group: word e / 2 for elements e and e + 1
+    unsigned pair0 = 0;
     auto soft = [&](int ks, int e) {  // elements e, e + 1 of group ks
       const int r = 8 * (ks & 1) + e;
-      if constexpr (DROP) {
-        if (e == 0) {
-          const int at = opaque_lane(lane);
-          Philox x;
-          x.start((kt0 >> 1) + 8 * ks + 2 * (at >> 5) + 4 * ((at >> 1) & 1) + (at & 1), (qw + (at & 31)) >> 2, hh);
-          x.rounds<0, kPhiloxRounds>(seed0, seed1);
-          words[0] = x.c0;
-          words[1] = x.c1;
-          words[2] = x.c2;
-          words[3] = x.c3;
-          quad_transpose(words, at);
-        }
-      }
       const float p0 = fast_exp2(fmaf(S[ks >> 1][r], a.scale2, ks < 2 ? neg_m : neg_m1));
       const float p1 = fast_exp2(fmaf(S[ks >> 1][r + 1], a.scale2, ks < 2 ? neg_m : neg_m1));
       rs0 += p0;
@@ -908,8 +923,13 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       unsigned pw = __builtin_bit_cast(unsigned, pr);
       asm volatile("" : "+v"(pw), "+v"(rs0), "+v"(rs1));
       if constexpr (DROP) {  // (the sums are those of all weights)
-        lr_acc[0] = dot2(__builtin_bit_cast(X2, pw), ones2, lr_acc[0]);
-        pw = (stays_low(words[e / 2], a.t.drop) ? pw & 0xffffu : 0u) | (stays_high(words[e / 2], a.t.drop) ? pw & 0xffff0000u : 0u);
+        if (e % 4 == 0) {
+          pair0 = pw;
+        } else {
+          typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+          lr_acc = mma_4x4<HALF>(ones4, __builtin_bit_cast(i16x4, (u32x2){pair0, pw}), lr_acc);
+        }
+        pw = keep_pair(pw, words[ks & 1][e / 2], a.t.drop);
       }
       pr = __builtin_bit_cast(X2, pw);
       pf[ks][e] = pr[0];
@@ -939,6 +959,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
 #pragma unroll
         for (int e = 4 * db / DB; e < 4 * (db + 1) / DB; ++e) soft(ks + 1, 2 * e);
       }
+      if (ks < 2) draw(ks + 2, kDraws * db / DB, kDraws * (db + 1) / DB);
       __builtin_amdgcn_sched_barrier(0);
     }
     l_run += rs0 + rs1;
@@ -1094,50 +1115,60 @@ struct DqLds {
   unsigned char flag[MODE ? kPairListTiles : 1];
   int red[20];
   std::conditional_t<has_rel(MODE), BiasLds<kBiasKeys, true>, NoLds> bias;
+  __attribute__((aligned(has_drop(MODE) ? 16 : 1))) std::conditional_t<has_drop(MODE), unsigned[4][256], NoLds> words;
 };
 
 // The gradient of the relative bias: the sums of dS over the pairs of each bucket.  A lane holds the row of a query, and dS in 32 bits, so
 // that is where they are taken, in an order that does not change.
-//  * Blocks on the way from one end of the distances to the other: the diagonals of a block are summed first, by fetching each of a lane's
-//    16 values from the lane that has the same diagonal (lane l of a half then has those of 4 half - l and of 32 more), and
-//    then the diagonals of a bucket, over the wave.  Lane u keeps bucket u's sum and that of bucket 64 + u.
+//  * Blocks on the way from one end of the distances to the other: a lane l of half g holds keys off + 4 g, off = 0 .. 3, 8 .. 11, .., of query l,
+//    so what the lane off further holds lies on the same diagonal: sixteen fetches across the wave sum the 63 diagonals, a lane having a
+//    part of two.  They are put in the order of d and summed up from the first one on; lane u then takes bucket u (and 64 + u) as the difference of two of these
+//    sums.
 //  * Blocks of a constant bias: a sum per lane for either end.  Where more than half of all pairs lie at one end (TermArgs::derive), no
 //    work is done for that one: its bucket is minus all the others' sum, since the dS of a row add up to zero (P adds up to one, and delta is the mean of
 //    dP).  That is the more exact way too: an error of delta is the same in every pair of a row, weighted with P, and adds up
 //    over a bucket that holds most of the row.  A bucket that no pair has keeps its zero (reached).
 struct BiasGrad {
-  float low, high;    // buckets 0 .. 63 and 64 .. 127 by lane
+  float low_sum, high_sum;  // buckets 0 .. 63 and 64 .. 127 by lane
   float past, ahead;  // the ends
   bool reached;
   RA_DEV void init() {
-    low = high = past = ahead = 0.f;
+    low_sum = high_sum = past = ahead = 0.f;
     reached = false;
   }
   RA_DEV void add(int u, float x, int lane) {  // u, x uniform
-    if (u < 64) low += lane == u ? x : 0.f;
-    else high += lane == u - 64 ? x : 0.f;
+    if (u < 64) low_sum += lane == u ? x : 0.f;
+    else high_sum += lane == u - 64 ? x : 0.f;
   }
-  // x: dS of the block whose first distance (of lane 0's query, first key) is value `at` of the tile; the diagonals' buckets are lds.ordered[buf]
+  // x: dS of the block in which lane 0's query and the first key are `base` apart
   template <typename Lds>
-  RA_DEV void add_block(const f32x16& x, const Lds& lds, int buf, int at, int lane) {
-    const int l32 = lane & 31, g = lane >> 5;
-    float d0 = 0.f, d1 = 0.f;  // of the diagonals 4 g - l32 and 32 more
+  RA_DEV void add_block(const f32x16& x, const Lds& lds, int n_buckets, int base, int lane) {
+    float d0 = 0.f, d1 = 0.f;  // of the diagonals 4 g - l, and 32 more than 4 (1 - g) - l (from the other half's lanes)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int off = 8 * (r / 4) + r % 4;
-      const int from = ((l32 + off) & 31) | (g << 5);
-      const float y = __uint_as_float((unsigned)__builtin_amdgcn_ds_bpermute(from << 2, (int)__float_as_uint(x[r])));
-      const bool second = l32 + off >= 32;
-      d0 += second ? 0.f : y;
-      d1 += second ? y : 0.f;
+      const float y = lane_at(4 * lane + 4 * off, x[r]);
+      if (off == 0) {
+        d0 = y;
+        continue;
+      }
+      // lanes whose fetch has passed the end of their half
+      unsigned half;  // (volatile: a constant is not worth a scalar register through the loop)
+      asm volatile("s_mov_b32 %0, %1" : "=s"(half) : "i"((int)(0xffffffffu << (32 - off))));
+      d1 += where_or_0((lane_mask)half << 32 | half, y);
+      d0 += y;
     }
-    const int i0 = at + 4 * g - l32;  // (d1 of the lanes up to 4 is 0, and its bucket whatever lies behind)
-    const int u0 = lds.ordered[buf][i0], u1 = lds.ordered[buf][min(i0 + 32, kBiasKeys - 1)];
-    const int first = __builtin_amdgcn_readfirstlane((int)lds.ordered[buf][at - 31]);
-    const int last = __builtin_amdgcn_readfirstlane((int)lds.ordered[buf][at + 31]);
-    for (int u = first; u <= last; ++u) {
-      add(u, wave_sum((u0 == u ? d0 : 0.f) + (u1 == u ? d1 : 0.f)), lane);
-    }
+    d0 -= d1;
+    // in lane e the diagonal base + e - 31: its parts are in lanes 31 - e and 67 - e (mod 64), in d0 or d1 by the half
+    const float low = lane < 32 ? d0 : d1, high = lane < 32 ? d1 : d0;
+    const float upto = wave_scan(lane_at(4 * 31 - 4 * lane, low) + lane_at(4 * 67 - 4 * lane, high));
+    auto bucket = [&](int u) {
+      const int hi = min(lds.hi[u] - base, 31) + 31, lo = max(lds.lo[u] - base, -31) + 31;
+      const float a = lane_at(4 * hi, upto), b = lane_at(4 * lo - 4, upto);
+      return hi >= lo ? (lo > 0 ? a - b : a) : 0.f;
+    };
+    low_sum += bucket(lane);
+    if (n_buckets > 64) high_sum += bucket(64 + lane);
   }
 };
 template <int MODE>
@@ -1264,14 +1295,20 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
   BiasEnds ends = {};
   BiasGrad bias_grad;
   bool bias_grad_on = false;
+  int n_buckets = 0;
   unsigned seed0 = 0, seed1 = 0;
   if constexpr (REL) {
     ends = load_bias(terms, h, kLog2e / a.scale_res, lds.bias);
     bias_grad.init();
     bias_grad_on = terms.grad_part != nullptr;
+    n_buckets = terms.two_sided ? 2 * terms.side : terms.side;
     __syncthreads();
   }
-  if constexpr (DROP) load_seed(terms, seed0, seed1);
+  PhiloxRow philox;
+  if constexpr (DROP) {
+    load_seed(terms, seed0, seed1);
+    philox.init(qi >> 2, hh, seed0, seed1);
+  }
   TileLoader<D, kPairKeys, DL> ldk, ldv;
   ldk.init(a.k.ptr + b * a.k.sb + h * a.k.sh, a.k.sl, a.Lk, wave, lane);
   ldv.init(a.v.ptr + b * a.v.sb + h * a.v.sh, a.v.sl, a.Lk, wave, lane);
@@ -1330,6 +1367,23 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
       // S^T first, then dP^T with the exp2 of S in its shadow: dP^T takes no registers while the terms
       // of a biased tile are evaluated
       constexpr int PF = KS < 3 ? KS : 3;  // operand fetches in flight ahead of the matrix instruction that uses them
+      unsigned words[2][4], drawing[4];  // dropout's, see fwd_pair_kernel
+      constexpr int kDraws = PhiloxRow::kSteps + 1;
+      auto draw = [&](int from, int to) {  // some of the 2 kDraws steps for both groups
+        if constexpr (DROP) {
+#pragma unroll
+          for (int i = from; i < to; ++i) {
+            const int half = i / kDraws, at = i % kDraws % PhiloxRow::kSteps ? lane : opaque_lane(lane);  // (nothing of it is kept: registers are short here)
+            if (i % kDraws < PhiloxRow::kSteps) {
+              philox.step(i % kDraws, drawing, (kt0 >> 1) + 16 * kb + 8 * half + PhiloxRow::pair(at), hh, seed0, seed1);
+            } else {
+              WordTurn turn;
+              turn.init(lds.words[wave], at);
+              turn.run(words[half], drawing);
+            }
+          }
+        }
+      };
       f32x16 S, zero;
       float neg_row = neg_lse2;  // added to the scores in the exponent
 #pragma unroll
@@ -1365,13 +1419,13 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
         for (int op = 1; op < KS; ++op) {
           if (op + PF < KS) fr[op + PF] = nat_frag(s_k[BUF], op + PF);
           S = mma(fr[op], qf[op], S);
+          draw(2 * kDraws * (op - 1) / (KS - 1), 2 * kDraws * op / (KS - 1));
           __builtin_amdgcn_sched_barrier(0);
         }
       }
       __builtin_amdgcn_s_setprio(0);
       float rel = 0.f;      // the relative bias where it is constant
       int side = 0;         // -1, 1: of the past's bucket, of the future's
-      const int bias_at = 32 * kb + (kPairRows - 1) - 32 * wave;
       if constexpr (REL) {
         const int at = opaque_lane(lane);
         const int d_lo = (kv_off + kt0 + 32 * kb) - (q_off + qw + 31);
@@ -1382,7 +1436,7 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
           rel = ends.ahead;
           side = 1;
         } else {
-          const float* value = &lds.bias.value[BUF][bias_at + 4 * (at >> 5) - (at & 31)];
+          const float* value = &lds.bias.value[BUF][32 * kb + 4 * (at >> 5) + (kPairRows - 1) - 32 * wave - (at & 31)];
 #pragma unroll
           for (int r = 0; r < 16; ++r) S[r] += value[8 * (r / 4) + r % 4];
         }
@@ -1427,23 +1481,17 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
         }
       }
       if constexpr (DROP) {
-        // (eight weights per call, see fwd_pair_kernel)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int at = opaque_lane(lane);
-          Philox x;
-          x.start((kt0 >> 1) + 16 * kb + 8 * half + 2 * (at >> 5) + 4 * ((at >> 1) & 1) + (at & 1), (qw + (at & 31)) >> 2, hh);
-          x.rounds<0, kPhiloxRounds>(seed0, seed1);
-          unsigned words[4] = {x.c0, x.c1, x.c2, x.c3};
-          quad_transpose(words, at);
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
-            P[8 * half + e] = stays_low(words[e / 2], terms.drop) ? P[8 * half + e] : neg_delta;
-            P[8 * half + e + 1] = stays_high(words[e / 2], terms.drop) ? P[8 * half + e + 1] : neg_delta;
+            P[8 * half + e] = stays_low(words[half][e / 2], terms.drop) ? P[8 * half + e] : neg_delta;
+            P[8 * half + e + 1] = stays_high(words[half][e / 2], terms.drop) ? P[8 * half + e + 1] : neg_delta;
           }
         }
       }
       if constexpr (REL) {
+        S *= P;
         if (bias_grad_on) {
           if (side != 0) {
             if (side == terms.derive) {
@@ -1451,15 +1499,12 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
             } else {
               float t = 0.f;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) t = fmaf(S[r], P[r], t);
+              for (int r = 0; r < 16; ++r) t += S[r];
               if (side < 0) bias_grad.past += t;
               else bias_grad.ahead += t;
             }
           } else {
-            f32x16 x;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = S[r] * P[r];
-            bias_grad.add_block(x, lds.bias, BUF, bias_at, opaque_lane(lane));
+            bias_grad.add_block(S, lds.bias, n_buckets, (kv_off + kt0 + 32 * kb) - (q_off + qw), opaque_lane(lane));
           }
         }
       }
@@ -1468,8 +1513,8 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
       X8 dsf[2];
       auto grad = [&](int ks, int e) {  // elements e, e + 1 of group ks
         X2 pr;
-        pr[0] = (T)(S[8 * ks + e] * P[8 * ks + e]);
-        pr[1] = (T)(S[8 * ks + e + 1] * P[8 * ks + e + 1]);
+        pr[0] = (T)(REL ? S[8 * ks + e] : S[8 * ks + e] * P[8 * ks + e]);
+        pr[1] = (T)(REL ? S[8 * ks + e + 1] : S[8 * ks + e + 1] * P[8 * ks + e + 1]);
         unsigned pw = __builtin_bit_cast(unsigned, pr);
         asm volatile("" : "+v"(pw));
         pr = __builtin_bit_cast(X2, pw);
@@ -1515,13 +1560,13 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
 
   if constexpr (REL) {
     if (bias_grad_on) {
-      const int n = terms.two_sided ? 2 * terms.side : terms.side;
+      const int n = n_buckets;
       float* const s_sum = (float*)s_k;  // [4][2 kMaxSide], and whether the derived bucket was there
       __syncthreads();                   // (nobody reads the tiles any more)
       bias_grad.add(0, wave_sum(bias_grad.past), lane);
       bias_grad.add(n - 1, wave_sum(bias_grad.ahead), lane);
-      s_sum[wave * 2 * kMaxSide + lane] = bias_grad.low;
-      s_sum[wave * 2 * kMaxSide + 64 + lane] = bias_grad.high;
+      s_sum[wave * 2 * kMaxSide + lane] = bias_grad.low_sum;
+      s_sum[wave * 2 * kMaxSide + 64 + lane] = bias_grad.high_sum;
       if (lane == 0) s_sum[8 * kMaxSide + wave] = bias_grad.reached ? 1.f : 0.f;
       __syncthreads();
       float* const part = terms.grad_part + (((long long)hh * nqt + qt) * p.n_split + split) * kGradRow;
@@ -1829,6 +1874,26 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       if (alibi_on && !one_side) tests |= kTestAlibi;
     }
     if (!wt.plain(j)) tests |= kTestPos;
+    // Dropout's bits: for the queries c = 0 .. 3 of a group bb of four, two halves a word.  A lane makes the calls of the groups of its
+    // own parity, for its key and the next lane's, and hands over what is the other's.
+    unsigned halves[4][2], x[4];
+    PhiloxKey philox;
+    constexpr int kDraws = PhiloxKey::kSteps + 1;
+    auto draw = [&](int i) {  // the i-th of 2 kDraws steps for the two calls
+      if constexpr (DROP) {
+        const int at = opaque_lane(lane), odd = at & 1, n = i / kDraws;
+        if (i == 0) philox.init((kw + (at & 31)) >> 1, hh, seed0, seed1);
+        if (i % kDraws < PhiloxKey::kSteps) return philox.step(i % kDraws, x, (qt0 >> 2) + 2 * (2 * n + odd) + (at >> 5), hh, seed0, seed1);
+        const unsigned is_odd = lane_bit(at, 0);
+        const unsigned own = 0x05040100u + 0x02020202u * odd, other = 0x07060302u - 0x02020202u * odd;  // (v_perm selectors: both words' halves)
+        const unsigned m0 = __builtin_amdgcn_perm(x[1], x[0], own), m1 = __builtin_amdgcn_perm(x[3], x[2], own);
+        const unsigned r0 = lane_dpp<0xb1>(__builtin_amdgcn_perm(x[1], x[0], other)), r1 = lane_dpp<0xb1>(__builtin_amdgcn_perm(x[3], x[2], other));
+        halves[2 * n][0] = choose(is_odd, r0, m0);
+        halves[2 * n][1] = choose(is_odd, r1, m1);
+        halves[2 * n + 1][0] = choose(is_odd, m0, r0);
+        halves[2 * n + 1][1] = choose(is_odd, m1, r1);
+      }
+    };
     constexpr int PF = KS < 3 ? KS : 3;  // operand fetches in flight ahead of the matrix instruction that uses them
     f32x16 S;
 #pragma unroll
@@ -1857,6 +1922,8 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       for (int op = 0; op < KS; ++op) {
         if (op + PF < KS) fr[op + PF] = nat_frag(s_q[BUF], op + PF);
         S = mma(fr[op], kf[op], S);
+#pragma unroll
+        for (int i = 2 * kDraws * op / KS; i < 2 * kDraws * (op + 1) / KS; ++i) draw(i);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -1894,25 +1961,6 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       }
       apply_terms<false, DENSE, GENERAL>(S, tests, tb, (q_off + qt0 + 4 * g) - (kv_off + ki), k_seg, k_pre,
                                          &s_seg[GENERAL ? BUF : 0][4 * g], &s_pre[GENERAL ? BUF : 0][4 * g]);
-    }
-    // Dropout's bits: for the queries c = 0 .. 3 of a group bb of four, two halves a word.  A lane makes the calls of the groups of its
-    // own parity, for its key and the next lane's, and hands over what is the other's.
-    unsigned halves[4][2];
-    if constexpr (DROP) {
-      const int at = opaque_lane(lane), odd = at & 1;
-      const unsigned own = odd ? 0x07060302u : 0x05040100u, other = odd ? 0x05040100u : 0x07060302u;  // (v_perm selectors: both words' halves)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        Philox x;
-        x.start((kw + (at & 31)) >> 1, (qt0 >> 2) + 2 * (2 * n + odd) + (at >> 5), hh);
-        x.rounds<0, kPhiloxRounds>(seed0, seed1);
-        const unsigned m0 = __builtin_amdgcn_perm(x.c1, x.c0, own), m1 = __builtin_amdgcn_perm(x.c3, x.c2, own);
-        const unsigned r0 = quad_dpp<0xb1>(__builtin_amdgcn_perm(x.c1, x.c0, other)), r1 = quad_dpp<0xb1>(__builtin_amdgcn_perm(x.c3, x.c2, other));
-        halves[2 * n][0] = odd ? r0 : m0;
-        halves[2 * n][1] = odd ? r1 : m1;
-        halves[2 * n + 1][0] = odd ? m0 : r0;
-        halves[2 * n + 1][1] = odd ? m1 : r1;
-      }
     }
     // dP with exp2(S) in its shadow
     X8 pf[2], dsf[2];
@@ -1958,10 +2006,6 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
           pr[1] = (T)x1;
           unsigned pw = __builtin_bit_cast(unsigned, pr);
           asm volatile("" : "+v"(x0), "+v"(x1), "+v"(pw));
-          if constexpr (DROP) {
-            const unsigned w = halves[r / 4][r % 4 / 2];
-            pw = (stays_low(w, terms.drop) ? pw & 0xffffu : 0u) | (stays_high(w, terms.drop) ? pw & 0xffff0000u : 0u);
-          }
           pr = __builtin_bit_cast(X2, pw);
           S[r] = x0;
           S[r + 1] = x1;
@@ -1980,14 +2024,21 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     if constexpr (DROP) {
-      // a weight that is left out has dP = 0 (P started from -delta)
+      // a weight that is left out has no part in dV, and dP = 0 (P started from -delta)
 #pragma unroll
       for (int bb = 0; bb < 4; ++bb) {
         const f32x4 t = *(const f32x4*)&s_stat[BUF][1][8 * bb + 4 * (opaque_lane(lane) >> 5)];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const unsigned w = halves[bb][c / 2];
-          P[4 * bb + c] = (c & 1 ? stays_high(w, terms.drop) : stays_low(w, terms.drop)) ? P[4 * bb + c] : t[c];
+        for (int c = 0; c < 4; c += 2) {
+          const int r = 4 * bb + c;
+          const lane_mask m0 = lanes_low(halves[bb][c / 2], terms.drop), m1 = lanes_high(halves[bb][c / 2], terms.drop);
+          X2 pr;
+          pr[0] = (T)where_or_0(m0, S[r]);
+          pr[1] = (T)where_or_0(m1, S[r + 1]);
+          pf[r >> 3][r & 7] = pr[0];
+          pf[r >> 3][(r & 7) + 1] = pr[1];
+          P[r] = where(m0, P[r], t[c]);
+          P[r + 1] = where(m1, P[r + 1], t[c + 1]);
         }
       }
     }
@@ -2138,7 +2189,7 @@ RA_DEV const auto& terms_of(const BothArgsOf<MODE>& p) {
   else return (const NoLds&)p;  // (nothing of it is read)
 }
 template <int DL, int MODE>
-__global__ __launch_bounds__(kPairThreads, DL <= 64 && MODE < 3 ? 3 : 2) void bwd_pair_kernel(const BothArgsOf<MODE> p) {
+__global__ __launch_bounds__(kPairThreads, DL <= 64 ? 3 : 2) void bwd_pair_kernel(const BothArgsOf<MODE> p) {
   __shared__ union Lds {
     DqLds<DL, MODE> dq;
     DkdvLds<DL, MODE> dkdv;

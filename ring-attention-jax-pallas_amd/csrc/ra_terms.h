@@ -1,5 +1,7 @@
 // Device code of the terms that take arguments of their own (TermArgs): the relative position bias by buckets, and dropout.
 #pragma once
+#include <type_traits>
+
 #include "ra_launch.h"
 
 namespace ra {
@@ -10,53 +12,130 @@ namespace ra {
 // seed as key and the counter (j / 2, i / 4, hh, 0); query i's word is the (i % 4)-th, an even key's half the low one.  A call serves eight weights
 // whichever side the kernel's lanes own: four neighbouring lanes with a query each exchange words, and two with a key each halves.
 // ------------------------------------------------------------------------------------------------
-struct Philox {
-  unsigned c0, c1, c2, c3;
-  RA_DEV void start(unsigned k_pair, unsigned q_group, unsigned hh) {
-    c0 = k_pair;
-    c1 = q_group;
-    c2 = hh;
-    c3 = 0;
+constexpr unsigned kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u, kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
+RA_DEV unsigned xor3(unsigned a, unsigned b, unsigned c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+// The r-th round (of 1 .. 7) on the words c; k0, k1: the seed.
+RA_DEV void philox_round(int r, unsigned (&c)[4], unsigned k0, unsigned k1) {
+  const unsigned long long a = (unsigned long long)c[0] * kPhiloxM0, b = (unsigned long long)c[2] * kPhiloxM1;
+  c[0] = xor3((unsigned)(b >> 32), c[1], k0 + (r - 1) * kPhiloxW0);
+  c[1] = (unsigned)b;
+  c[2] = xor3((unsigned)(a >> 32), c[3], k1 + (r - 1) * kPhiloxW1);
+  c[3] = (unsigned)a;
+}
+// The words c of four neighbouring lanes turned round, through a kilobyte of LDS that is the wave's own: word x of a lane becomes the lane's own word of
+// the x-th lane.  (In registers that is sixteen vector instructions, of some 75 that dropout costs a lane's eight weights; LDS has room beside the tiles'
+// operands, and gives all of its banks to either side.)  No barrier: a wave's LDS instructions are carried out in order.
+struct WordTurn {
+  unsigned *to, *from;
+  RA_DEV void init(unsigned* lds, int lane) {
+    to = lds + 4 * ((lane >> 2) + 16 * (lane & 3));
+    from = lds + 4 * (lane >> 2) + (lane & 3);
   }
-  // rounds [FROM, TO) under the key k0, k1
-  template <int FROM, int TO>
-  RA_DEV void rounds(unsigned k0, unsigned k1) {
+  RA_DEV void run(unsigned (&w)[4], const unsigned (&c)[4]) const {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    *(u32x4*)to = (u32x4){c[0], c[1], c[2], c[3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r = FROM; r < TO; ++r) {
-      const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-      const unsigned x0 = k0 + (unsigned)r * 0x9E3779B9u, x1 = k1 + (unsigned)r * 0xBB67AE85u;
-      c0 = (unsigned)(b >> 32) ^ c1 ^ x0;
-      c1 = (unsigned)b;
-      c2 = (unsigned)(a >> 32) ^ c3 ^ x1;
-      c3 = (unsigned)a;
-    }
+    for (int x = 0; x < 4; ++x) w[x] = from[64 * x];
   }
 };
-constexpr int kPhiloxRounds = 7;
+// A call in steps, which the kernels lay between their matrix instructions: a round waits for the one before, and a wave that makes them in one go
+// waits with it.  What the first rounds leave to do where a lane keeps its query (two of fourteen products are the same in every call) ...
+struct PhiloxRow {
+  static constexpr int kSteps = 6;
+  unsigned a_high, a_low;  // of the second round's first product, the high word with its key
+  static RA_DEV int pair(int lane) { return 2 * (lane >> 5) + 4 * ((lane >> 1) & 1) + (lane & 1); }  // of the sixteen keys of a group: where its call's two are
+  RA_DEV void init(unsigned q_group, unsigned hh, unsigned k0, unsigned k1) {
+    const unsigned long long b = (unsigned long long)hh * kPhiloxM1;
+    const unsigned long long a = (unsigned long long)((unsigned)(b >> 32) ^ q_group ^ k0) * kPhiloxM0;
+    a_high = (unsigned)(a >> 32) ^ (k1 + kPhiloxW1);
+    a_low = (unsigned)a;
+  }
+  RA_DEV void step(int i, unsigned (&c)[4], unsigned k_pair, unsigned hh, unsigned k0, unsigned k1) const {
+    asm volatile("" : "+s"(k0), "+s"(k1));  // (the keys of the rounds are made again, not kept: scalar registers are short)
+    if (i > 0) return philox_round(i + 2, c, k0, k1);
+    const unsigned long long a = (unsigned long long)k_pair * kPhiloxM0;
+    const unsigned long long b = (unsigned long long)((unsigned)(a >> 32) ^ k1) * kPhiloxM1;
+    c[0] = xor3((unsigned)(b >> 32), hh * kPhiloxM1, k0 + kPhiloxW0);
+    c[1] = (unsigned)b;
+    c[2] = a_high ^ (unsigned)a;
+    c[3] = a_low;
+  }
+};
+// ... and where it keeps its key (four, in the two calls for a block; kept through the loop they cost the backward's kernels spills).
+struct PhiloxKey {
+  static constexpr int kSteps = 5;
+  unsigned a_low, b_low, a3_high, a3_low;  // of the first round's and the second's products, with keys; of the third's first
+  RA_DEV void init(unsigned k_pair, unsigned hh, unsigned k0, unsigned k1) {
+    const unsigned long long a = (unsigned long long)k_pair * kPhiloxM0;
+    const unsigned long long b = (unsigned long long)((unsigned)(a >> 32) ^ k1) * kPhiloxM1;
+    a_low = (unsigned)a ^ (k1 + kPhiloxW1);
+    b_low = (unsigned)b ^ (k0 + 2 * kPhiloxW0);
+    const unsigned long long a3 = (unsigned long long)((unsigned)(b >> 32) ^ (hh * kPhiloxM1) ^ (k0 + kPhiloxW0)) * kPhiloxM0;
+    a3_high = (unsigned)(a3 >> 32) ^ (k1 + 2 * kPhiloxW1);
+    a3_low = (unsigned)a3;
+  }
+  RA_DEV void step(int i, unsigned (&c)[4], unsigned q_group, unsigned hh, unsigned k0, unsigned k1) const {
+    asm volatile("" : "+s"(k0), "+s"(k1));
+    if (i > 0) return philox_round(i + 3, c, k0, k1);
+    const unsigned first = (unsigned)(((unsigned long long)hh * kPhiloxM1) >> 32) ^ k0;
+    const unsigned long long a = (unsigned long long)(q_group ^ first) * kPhiloxM0;
+    const unsigned long long b = (unsigned long long)((unsigned)(a >> 32) ^ a_low) * kPhiloxM1;
+    c[0] = (unsigned)(b >> 32) ^ b_low;
+    c[1] = (unsigned)b;
+    c[2] = a3_high ^ (unsigned)a;
+    c[3] = a3_low;
+  }
+};
 
 template <int CTRL>
-RA_DEV unsigned quad_dpp(unsigned x) {
-  return (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
+RA_DEV unsigned lane_dpp(unsigned x) {  // (patterns that read every lane)
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
 }
-// The words w0 .. w3 of four neighbouring lanes turned round: word x of a lane becomes the lane's own word of lane x.
-RA_DEV void quad_transpose(unsigned (&w)[4], int lane) {
-  const bool b0 = lane & 1, b1 = lane & 2;
-#pragma unroll
-  for (int x = 0; x < 4; x += 2) {
-    const unsigned got = quad_dpp<0xb1>(b0 ? w[x] : w[x + 1]);
-    w[x] = b0 ? got : w[x];
-    w[x + 1] = b0 ? w[x + 1] : got;
-  }
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const unsigned got = quad_dpp<0x4e>(b1 ? w[x] : w[x + 2]);
-    w[x] = b1 ? got : w[x];
-    w[x + 2] = b1 ? w[x + 2] : got;
-  }
-}
+// All ones in the lanes whose number has the bit, and a choice by such a mask.
+RA_DEV unsigned lane_bit(int lane, int bit) { return (unsigned)((int)((unsigned)lane << (31 - bit)) >> 31); }
+RA_DEV unsigned choose(unsigned mask, unsigned a, unsigned b) { return (mask & a) | (~mask & b); }
 // Whether the weight of a word's half stays.
 RA_DEV bool stays_low(unsigned w, unsigned drop) { return (unsigned short)w >= (unsigned short)drop; }
 RA_DEV bool stays_high(unsigned w, unsigned drop) { return w >= drop << 16; }
+// ... as a mask of lanes, to be used more than once: such a mask is kept out of VCC, which a v_cndmask reads in 4 cycles right behind the compare and in
+// some 20 every further time (any other scalar pair: 4).
+typedef unsigned long long lane_mask;
+RA_DEV lane_mask lanes_low(unsigned w, unsigned drop) {
+  lane_mask m;
+  asm("v_cmp_ge_u16_e64 %0, %1, %2" : "=s"(m) : "v"(w), "s"(drop));
+  return m;
+}
+RA_DEV lane_mask lanes_high(unsigned w, unsigned drop) {
+  lane_mask m;
+  asm("v_cmp_ge_u32_e64 %0, %1, %2" : "=s"(m) : "v"(w), "s"(drop << 16));
+  return m;
+}
+RA_DEV float where(lane_mask m, float a, float b) {
+  float x;
+  asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(x) : "v"(b), "v"(a), "s"(m));
+  return x;
+}
+RA_DEV float where_or_0(lane_mask m, float a) {
+  float x;
+  asm("v_cndmask_b32_e64 %0, 0, %1, %2" : "=v"(x) : "v"(a), "s"(m));
+  return x;
+}
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+// 1 in the halves of two 16-bit values that are at least `least`, which is 1 or more
+RA_DEV u16x2 at_least(unsigned w, unsigned least) {
+  // (packed instructions by name: the compiler makes two compares, two choices and a merge of it)
+  unsigned d;
+  asm("v_pk_sub_u16 %0, %1, %2 clamp" : "=v"(d) : "v"(w), "s"((least - 1) * 0x10001u));
+  asm("v_pk_min_u16 %0, %0, 1 op_sel_hi:[1,0]" : "+v"(d));
+  return __builtin_bit_cast(u16x2, d);
+}
+// Two 16-bit elements, of which those stay whose halves of `w` do.
+RA_DEV unsigned keep_pair(unsigned pair, unsigned w, unsigned drop) {
+  return __builtin_bit_cast(unsigned, (u16x2)(__builtin_bit_cast(u16x2, pair) * at_least(w, drop)));
+}
 
 // The seed's words, as uniform values.
 RA_DEV void load_seed(const TermArgs& t, unsigned& k0, unsigned& k1) {
@@ -82,10 +161,10 @@ RA_DEV int table_row(int ordered, int side) { return ordered >= side ? ordered :
 // N: the distances of a tile
 template <int N, bool GRAD>
 struct BiasLds {
-  float value[2][N];             // of the tiles of the two buffers
-  unsigned char ordered[GRAD ? 2 : 1][GRAD ? N : 4];  // their buckets
-  float table[2 * kMaxSide];     // of this head, in the order of d
+  float value[2][N];          // of the tiles of the two buffers
+  float table[2 * kMaxSide];  // of this head, in the order of d
   int start[kMaxSide];
+  int lo[GRAD ? 2 * kMaxSide : 1], hi[GRAD ? 2 * kMaxSide : 1];  // the distances of a bucket (in that order; hi < lo: none)
 };
 RA_DEV float load_table(const TermArgs& t, int row, int h) {
   const long long at = row * t.table_sb + h * t.table_sh;
@@ -98,9 +177,24 @@ struct BiasEnds {
   int far, future;    // d <= -far, d >= future
   float past, ahead;
 };
-template <typename Lds>
-RA_DEV BiasEnds load_bias(const TermArgs& t, int h, float unit, Lds& lds) {
+template <int N, bool GRAD>
+RA_DEV BiasEnds load_bias(const TermArgs& t, int h, float unit, BiasLds<N, GRAD>& lds) {
   const int tid = threadIdx.x, n = t.two_sided ? 2 * t.side : t.side;
+  if constexpr (GRAD) {
+    if (tid < 2 * kMaxSide) {
+      constexpr int kFar = 1 << 30;
+      const bool ahead = tid >= t.side;
+      const int b = ahead ? tid - t.side : t.side - 1 - tid;
+      int lo = 0, hi = -1;
+      if (tid < n) {
+        const int from = t.start[b], to = b + 1 < t.side ? t.start[b + 1] - 1 : kFar;  // |d|
+        lo = ahead ? max(from, 1) : -to;
+        hi = ahead ? to : b == 0 && !t.two_sided ? kFar : -from;
+      }
+      lds.lo[tid] = lo;
+      lds.hi[tid] = hi;
+    }
+  }
   if (tid < n) lds.table[tid] = load_table(t, table_row(tid, t.side), h) * unit;
   if (tid < kMaxSide) lds.start[tid] = tid < t.side ? t.start[tid] : 0x7fffffff;
   BiasEnds e;
@@ -120,7 +214,6 @@ RA_DEV void write_bias(const TermArgs& t, const BiasEnds& e, BiasLds<N, GRAD>& l
   if (i < N) {
     const int u = ordered_bucket(lds.start, t.side, t.two_sided, d_lo + i);
     lds.value[buf][i] = lds.table[u];
-    if constexpr (GRAD) lds.ordered[buf][i] = (unsigned char)u;
   }
 }
 
@@ -135,12 +228,29 @@ RA_DEV void store_rest(void* base, long long at, const f32x4& x) {
 
 // Sum over a wave, in every lane.
 RA_DEV float wave_sum(float x) {
-  x += __uint_as_float(quad_dpp<0xb1>(__float_as_uint(x)));
-  x += __uint_as_float(quad_dpp<0x4e>(__float_as_uint(x)));
-  x += __uint_as_float(quad_dpp<0x141>(__float_as_uint(x)));
-  x += __uint_as_float(quad_dpp<0x140>(__float_as_uint(x)));
+  x += __uint_as_float(lane_dpp<0xb1>(__float_as_uint(x)));
+  x += __uint_as_float(lane_dpp<0x4e>(__float_as_uint(x)));
+  x += __uint_as_float(lane_dpp<0x141>(__float_as_uint(x)));
+  x += __uint_as_float(lane_dpp<0x140>(__float_as_uint(x)));
   auto lane = [&](int l) { return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(x), l)); };
   return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
+
+// Sums of a wave's lanes up to and including each.
+RA_DEV float wave_scan(float x) {
+  auto add = [&](auto ctrl, auto rows) {
+    x += __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using All = std::integral_constant<int, 0xf>;
+  add(std::integral_constant<int, 0x111>{}, All{});  // one lane to the right inside rows of 16, two, four, eight
+  add(std::integral_constant<int, 0x112>{}, All{});
+  add(std::integral_constant<int, 0x114>{}, All{});
+  add(std::integral_constant<int, 0x118>{}, All{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // the last lane of a row to the next row, of the first half to the second
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return x;
+}
+// lane (from / 4) mod 64's value
+RA_DEV float lane_at(int from, float x) { return __uint_as_float((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(x))); }
 
 }  // namespace ra
