@@ -5,12 +5,15 @@
 // The library's entry points come in as addresses (init), so that it runs on the build that the package has loaded.  forward and backward
 // are the call without its node and conversions.
 #include <Python.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/types.h>
@@ -300,6 +303,7 @@ variable_list node_backward(AutogradContext* ctx, const variable_list& grads_in)
   variable_list kept = ctx->get_saved_variables();
   Terms terms;
   Tensor d_table;
+  const c10::OptionalDeviceGuard on(call->with_terms ? c10::optional<at::Device>(p.device) : c10::nullopt);
   if (call->with_terms) {
     const Tensor table = kept[kept.size() - 3];
     terms = call->terms;
@@ -494,6 +498,17 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A leaf whose gradient accumulator another graph keeps alive on another stream: the backward of a captured call would make that stream wait for the
+// capture, which ends the process.
+void check_capture(const Tensor& t) {
+  if (!t.requires_grad() || !t.is_leaf()) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!accumulator) return;
+  const auto s = accumulator->stream();
+  TORCH_CHECK(!s || s->id() == c10::hip::getCurrentHIPStream().id(),
+              "a call on tensors that a live autograd graph of another stream leads to cannot be captured: drop that graph (its outputs) first");
+}
+
 // attend_terms(q, k, v, plan, scale, the kernels' output dtype, the caller's, position of the first query, of the first key, table or None,
 // two_sided, bucket starts of a side (int32s as bytes), drop, seed: an int or a tensor) -> output, logsumexp [1, b, h, l]
 PyObject* attend_terms(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -543,8 +558,13 @@ PyObject* attend_terms(PyObject*, PyObject* const* args, Py_ssize_t n) {
   variable_list got;
   {
     pybind11::gil_scoped_release no_gil;  // (allocations may wait for the GPU)
+    const c10::DeviceGuard on(q.device());
     for (Tensor* t : {&k, &v})
       if (t->device() != q.device()) *t = t->to(q.device());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+      for (const Tensor* t : {&q, static_cast<const Tensor*>(&k), static_cast<const Tensor*>(&v)}) check_capture(*t);
+      if (with_table) check_capture(*with_table);
+    }
     check_operands(*call->plan, q, k, v);
     const bool any_grad =
         at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (with_table && with_table->requires_grad()));

@@ -689,10 +689,6 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
 
   BiasEnds ends = {};
   unsigned seed0 = 0, seed1 = 0;
-  if constexpr (REL) {
-    ends = load_bias(a.t, h, kLog2e / a.scale2, s_bias);
-    __syncthreads();
-  }
   PhiloxRow philox;
   int pair = 0;
   WordTurn turn = {};
@@ -715,7 +711,9 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       if (kv_seg && wave == 0) global_to_lds4(kv_seg + kk, RA_LDS_ADDR(&s_seg[0][0]) + buf * (kPairKeys * 4));
       if (kv_pre && wave == 1) global_to_lds4(kv_pre + kk, RA_LDS_ADDR(&s_pre[0][0]) + buf * (kPairKeys * 4));
     }
-    if constexpr (REL) write_bias(a.t, ends, s_bias, buf, (kv_off + k0) - (q_off + q0 + kPairRows - 1));
+  };
+  auto bias_tile = [&](int j, int buf) {
+    if constexpr (REL) write_bias(a.t, ends, s_bias, buf, (kv_off + j * kPairKeys) - (q_off + q0 + kPairRows - 1));
   };
 
   float m_run = RA_NEG_INF;  // exponent reference (log2 domain), moves lazily
@@ -777,6 +775,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     if (i + 1 < i_hi) {
       walk.next(i + 1);
       issue_tile(walk.tile(), BUF ^ 1);
+      bias_tile(walk.tile(), BUF ^ 1);
     }
     if (dead) return;
     const bool one_side = alibi_on && (j < wt.past || j >= wt.future);
@@ -981,6 +980,11 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
   if (i_lo < i_hi) {
     walk.start(GENERAL && use_list, s_list, j_lo, i_lo, i_hi, every_test);
     issue_tile(walk.tile(), 0);
+    if constexpr (REL) {  // (behind the first tile's loads)
+      ends = load_bias(a.t, h, kLog2e / a.scale2, s_bias);
+      __syncthreads();
+      bias_tile(walk.tile(), 0);
+    }
     for (int i = i_lo; i < i_hi; i += 2) {
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < i_hi) step(std::integral_constant<int, 1>{}, i + 1);
@@ -1069,7 +1073,12 @@ __global__ __launch_bounds__(256) void pair_combine_kernel(const FwdArgsOf<MODE>
   const int n_piece = a.part_n[hh * ((a.Lq + kPairRows - 1) / kPairRows) + li / kPairRows];
   if (n_piece <= 1) return;  // written by its only workgroup
   float m = RA_NEG_INF;
-  for (int s = 0; s < n_piece; ++s) m = fmaxf(m, a.part_s[4 * (s * rows + row)]);
+  if constexpr (MODE >= 3) {  // (a token's keys may have many shares)
+#pragma unroll 8
+    for (int s = 0; s < n_piece; ++s) m = fmaxf(m, a.part_s[4 * (s * rows + row)]);
+  } else {
+    for (int s = 0; s < n_piece; ++s) m = fmaxf(m, a.part_s[4 * (s * rows + row)]);
+  }
   const float m_safe = (m == RA_NEG_INF) ? 0.f : m;
   float l = 0.f, lr = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -1298,11 +1307,9 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
   int n_buckets = 0;
   unsigned seed0 = 0, seed1 = 0;
   if constexpr (REL) {
-    ends = load_bias(terms, h, kLog2e / a.scale_res, lds.bias);
     bias_grad.init();
     bias_grad_on = terms.grad_part != nullptr;
     n_buckets = terms.two_sided ? 2 * terms.side : terms.side;
-    __syncthreads();
   }
   PhiloxRow philox;
   if constexpr (DROP) {
@@ -1321,7 +1328,9 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
       if (kv_seg && wave == 0) global_to_lds4(kv_seg + kk, RA_LDS_ADDR(&s_seg[0][0]) + buf * (kPairKeys * 4));
       if (kv_pre && wave == 1) global_to_lds4(kv_pre + kk, RA_LDS_ADDR(&s_pre[0][0]) + buf * (kPairKeys * 4));
     }
-    if constexpr (REL) write_bias(terms, ends, lds.bias, buf, (kv_off + k0) - (q_off + q0 + kPairRows - 1));
+  };
+  auto bias_tile = [&](int j, int buf) {
+    if constexpr (REL) write_bias(terms, ends, lds.bias, buf, (kv_off + j * kPairKeys) - (q_off + q0 + kPairRows - 1));
   };
 
   f32x16 acc[DB];
@@ -1354,6 +1363,7 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
     if (i + 1 < i_hi) {
       walk.next(i + 1);
       issue_tile(walk.tile(), BUF ^ 1);
+      bias_tile(walk.tile(), BUF ^ 1);
     }
     if (dead) return;
     const bool one_side = alibi_on && (j < wt.past || j >= wt.future);
@@ -1552,6 +1562,11 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
   if (i_lo < i_hi) {
     walk.start(GENERAL && use_list, s_list, j_lo, i_lo, i_hi, every_test);
     issue_tile(walk.tile(), 0);
+    if constexpr (REL) {
+      ends = load_bias(terms, h, kLog2e / a.scale_res, lds.bias);
+      __syncthreads();
+      bias_tile(walk.tile(), 0);
+    }
     for (int i = i_lo; i < i_hi; i += 2) {
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < i_hi) step(std::integral_constant<int, 1>{}, i + 1);
@@ -1796,10 +1811,6 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
   }
   BiasEnds ends = {};
   unsigned seed0 = 0, seed1 = 0;
-  if constexpr (REL) {
-    ends = load_bias(terms, h, kLog2e / a.scale_res, lds.bias);
-    __syncthreads();
-  }
   if constexpr (DROP) load_seed(terms, seed0, seed1);
   TileLoader<D, kPairQueries, DL> ldq, ldo;
   ldq.init(a.q.ptr + b * a.q.sb + h * a.q.sh, a.q.sl, a.Lq, wave, lane);
@@ -1824,7 +1835,9 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       if (q_seg && wave == 1) global_to_lds4_s(q_seg + r0, 4 * row, RA_LDS_ADDR(&s_seg[0][0]) + buf * 256);
       if (q_pre && wave == 2) global_to_lds4_s(q_pre + r0, 4 * row, RA_LDS_ADDR(&s_pre[0][0]) + buf * 256);
     }
-    if constexpr (REL) write_bias(terms, ends, lds.bias, buf, (kv_off + k0) - (q_off + r0 + kPairQueries - 1));
+  };
+  auto bias_tile = [&](int j, int buf) {
+    if constexpr (REL) write_bias(terms, ends, lds.bias, buf, (kv_off + k0) - (q_off + j * kPairQueries + kPairQueries - 1));
   };
 
   f32x16 dk[DB], dv[DB];
@@ -1866,6 +1879,7 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
     if (i + 1 < i_hi) {
       walk.next(i + 1);
       issue_tile(walk.tile(), BUF ^ 1);
+      bias_tile(walk.tile(), BUF ^ 1);
     }
     if (dead) return;
     const bool one_side = alibi_on && (j < wt.past || j >= wt.future);
@@ -2082,6 +2096,11 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
     ldv.issue(k0, RA_LDS_ADDR(&s_v[0]), wave, lane);
     walk.start(GENERAL && use_list, s_list, j_lo, i_lo, i_hi, every_test);
     issue_tile(walk.tile(), 0);
+    if constexpr (REL) {
+      ends = load_bias(terms, h, kLog2e / a.scale_res, lds.bias);
+      __syncthreads();
+      bias_tile(walk.tile(), 0);
+    }
     for (int i = i_lo; i < i_hi; i += 2) {
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < i_hi) step(std::integral_constant<int, 1>{}, i + 1);

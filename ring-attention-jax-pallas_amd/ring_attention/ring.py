@@ -1044,20 +1044,21 @@ def _terms_call(q, k, v, n, fn: Optional[BiasFn], q_kwargs, kv_kwargs, sm_scale,
     positions that are given as an int are the call's own, so that a plan serves every step of a training or decoding loop."""
     if torch._C._get_tracing_state() is not None:
         raise RuntimeError("a relative bias and dropout cannot be traced")
-    relative = None
-    offsets = [None, None]
-    kwargs = [dict(q_kwargs or {}), dict(kv_kwargs or {})]
+    relative = q_off = kv_off = None
     if isinstance(fn, BiasFn):
-        for i, (name, x) in enumerate((("q_positions", q), ("kv_positions", k))):
-            if isinstance(kwargs[i].get(name), int):
-                offsets[i] = _first_position(kwargs[i].pop(name), x.shape[1], name)
+        if q_kwargs and isinstance(q_kwargs.get("q_positions"), int):
+            q_kwargs = dict(q_kwargs)
+            q_off = _first_position(q_kwargs.pop("q_positions"), q.shape[1], "q_positions")
+        if kv_kwargs and isinstance(kv_kwargs.get("kv_positions"), int):
+            kv_kwargs = dict(kv_kwargs)
+            kv_off = _first_position(kv_kwargs.pop("kv_positions"), k.shape[1], "kv_positions")
         relative = fn.relative
         if relative is not None:
             relative.validate()
             if relative.table.shape[1] != q.shape[2]:
                 raise ValueError(f"the table of a relative bias must have a column per head ({q.shape[2]}), got {tuple(relative.table.shape)}")
-            fn = replace(fn, relative=_NO_TABLE)
-    plan = _plan_for(q, k, n, fn, *kwargs).single()
+            fn = BiasFn(fn.causal, fn.window, fn.segments, fn.prefix, fn.alibi_slopes, _NO_TABLE)
+    plan = _plan_for(q, k, n, fn, q_kwargs, kv_kwargs).single()
     if isinstance(seed, torch.Tensor):
         if seed.numel() != 1 or seed.dtype != torch.int64 or seed.device != q.device:
             raise ValueError(f"a dropout seed is an int or a tensor of one int64 on {q.device}")
@@ -1066,9 +1067,8 @@ def _terms_call(q, k, v, n, fn: Optional[BiasFn], q_kwargs, kv_kwargs, sm_scale,
     table, two_sided, starts = None, False, None
     if relative is not None:
         table, two_sided, starts = relative.table.to(q.device), relative.bidirectional, relative.starts
-    q_off, kv_off = (plan_off if off is None else off for off, plan_off in zip(offsets, (plan.q_off[0], plan.kv_off[0])))
-    out, lse = _lib.host().attend_terms(q, k, v, plan.native(q), float(sm_scale), out_dtype, final_dtype, q_off, kv_off, table, two_sided, starts,
-                                        drop, seed if drop else None)
+    out, lse = _lib.host().attend_terms(q, k, v, plan.native(q), float(sm_scale), out_dtype, final_dtype, plan.q_off[0] if q_off is None else q_off,
+                                        plan.kv_off[0] if kv_off is None else kv_off, table, two_sided, starts, drop, seed if drop else None)
     return out, lse, plan
 
 

@@ -303,6 +303,66 @@ def test_operand_and_table_layouts(device):
     assert not gk[2:].any() and not gk[:, :, 4:].any() and not gv[:, 170:].any()
 
 
+def test_one_head_of_keys_for_all(device):
+    """Keys and values that are expanded over the heads: their gradients are the heads' sum, which autograd takes in bf16."""
+    c = Case(device, B=2, H=4, Sq=140, relative="both", p=0.1)
+    k, v = (x[:, :, :1].contiguous().requires_grad_(True) for x in (c.k, c.v))
+    out = c.call(k=k.expand(-1, -1, 4, -1), v=v.expand(-1, -1, 4, -1))[0]
+    gk, gv = torch.autograd.grad(out, (k, v), c.do)
+    c.k, c.v = (x.detach().expand(-1, -1, 4, -1).contiguous() for x in (k, v))
+    w = c.want()
+    _close("out", out.detach(), w.out, w.out_off)
+    for name, got in (("dk", gk), ("dv", gv)):
+        want, off = getattr(w, name), getattr(w, name + "_off")
+        # (a sum in bf16 of four: at most three more roundings of partial sums, and the result's)
+        _close(name, got, want.sum(2, keepdim=True), off.sum(2, keepdim=True) + 4 * 2.0 ** -8 * want.abs().sum(2, keepdim=True))
+
+
+def test_cache_of_more_than_two_to_the_31_elements(device):
+    S, H, D = 262400, 64, 128
+    k, v = (torch.empty(1, S, H, D, device=device, dtype=torch.bfloat16).normal_() for _ in range(2))
+    assert k.numel() > 1 << 31
+    q = torch.randn(1, 1, H, D, device=device).to(torch.bfloat16)
+    table = torch.randn(32, H, device=device)
+    fn = ra.causal_bias() + ra.relative_bias(table, bidirectional=False)
+    out, lse = ra.ring_attention_with_lse(q, k, v, 1, fn, {"q_positions": S - 1}, dropout=ra.Dropout(0.1, 5))
+    bucket = T.bucket_of(torch.arange(S, device=device)[None] - (S - 1), 32, 128, False)
+    for h in (0, H - 1):
+        j = torch.arange(S, device=device)[None]
+        zero = torch.zeros_like(j)
+        w0 = T.philox((j // 2, zero, zero + h, zero), (5, 0), 7)[0]
+        keep = (((w0 >> 16 * (j % 2)) & 0xFFFF) >= 6554)[None, None]
+        w = T.Attention(q[:, :, h:h + 1], k[:, :, h:h + 1], v[:, :, h:h + 1], bias=table[:, h].double()[bucket][None], keep=keep, threshold=6554)
+        _close("out", out[:, :, h:h + 1], w.out, w.out_off)
+        _close("lse", lse[:, h:h + 1], w.lse, w.lse_off)
+
+
+def test_capture_beside_a_live_graph_of_the_same_leaves(device):
+    c = Case(device, Sq=40, relative="both", p=0.1)
+    leaf = c.q.detach().clone().requires_grad_(True)
+    alive = c.call(leaf)[0]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="live autograd graph"):
+        with torch.cuda.graph(graph):
+            c.call(leaf)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = torch.autograd.grad(c.call(leaf)[0], leaf, c.do)[0]
+    want = c.grads()[2][0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+
+
+def test_empty_arrays_are_refused(device):
+    c = Case(device, Sq=16, relative="both", p=0.1)
+    for q, k in ((c.q[:, :0], c.k), (c.q, c.k[:, :0]), (c.q[:0], c.k[:0]), (c.q[:, :, :0], c.k[:, :, :0])):
+        with pytest.raises((RuntimeError, ValueError)):
+            c.call(q=q, k=k, v=k)
+
+
 def test_other_dtypes_are_rounded_to_bf16(device):
     c = Case(device, B=1, H=2, Sq=190, D=80, relative="one", mask="causal", p=0.2)
     leaves = [x.float().requires_grad_(True) for x in (c.q, c.k, c.v)]
