@@ -705,6 +705,13 @@ bool long_stretches(const ra_bias& bias, int D, int64_t wgs, int64_t total, int6
 // 4096: 88 -> 63 us; H=4, 16384: 375 -> 340 us).  At most kMaxSplit shares, and none under kMinChunk tiles, which
 // cost more in partial results (528 bytes per row and share) than they gain.
 constexpr int kMinChunk = 6, kMaxSplit = 64;
+// With a relative bias or dropout (`always`), where a tile takes longer and nothing else is measured against: shares down to a third of that if the rows
+// are few, or one tile of them.  Kernels of a call, us, shares of six | of two (twice that for dK and dV): a token behind 1000 keys, H=8, D=64, bias 12.8 + 4.0 | 8.8 + 3.5,
+// 5000, H=16, D=128 16.8 + 5.9 | 15.8 + 4.4, 128 of 3000, H=8, D=128 19.4 + 4.1 | 17.7 + 5.7; training, dropout, causal 512, H=4, D=64 52.5 | 36.1, both 78.8 |
+// 63.5 (H=8, D=128), 1024, H=4, D=64 72.7 | 60.5, unmasked 512, H=4 58.3 | 48.2; not even rows on 64 workgroups, unmasked 1000, H=8, D=128 78.0 | 82.2.
+int min_chunk(bool always, bool even, int64_t rows, int64_t wgs, int most, int tiles) {
+  return always && (rows == 1 || wgs <= (even ? 32 : 64)) && most > tiles ? tiles / 3 : tiles;
+}
 bool has_lists(const ra_bias& b) { return b.flags & (RA_BIAS_SEGMENT | RA_BIAS_PREFIX | RA_BIAS_DENSE); }
 // Whether all of a head's resident tiles have about the same work.
 bool even_rows(int64_t total, int most, int64_t rows) { return total * 20 >= (int64_t)most * rows * 17; }
@@ -790,9 +797,7 @@ PairPlan plan_fwd_pair(const ra_fwd_step_params& p, bool always = false) {
     r.chunk_tiles = (most + 1) / 2;
     r.n_split = 2;
   }
-  // (a few rows' partial results are next to nothing: a token behind 1000 keys, 8 heads, D=64, with a relative bias 22.6 us a call as shares of six tiles, 19.0 of two)
-  const int min_chunk = always && p.Lq <= 16 ? 2 : kMinChunk;
-  if (r.pair) plan_split(r, heads, rows, total, most, min_chunk, 4 * heads * p.Lq * p.D, p.bias, false);
+  if (r.pair) plan_split(r, heads, rows, total, most, min_chunk(always, even, rows, wgs, most, kMinChunk), 4 * heads * p.Lq * p.D, p.bias, false);
   if (one_by_one(p.bias, total, most, rows)) r.group = 1;
   return r;
 }
@@ -808,7 +813,7 @@ struct TileCount {
 PairPlan plan_dq_pair(const ra_bwd_step_params& p, const TileCount& c, bool beside, bool always) {
   PairPlan r{true, 1, std::max(c.most, 1), kHeadGroup};
   if (!always && long_stretches(p.bias, p.D, c.heads * c.rows, c.total, c.rows, 160)) r.pair = false;
-  else plan_split(r, c.heads, c.rows, c.total, c.most, kMinChunk, 4 * c.heads * p.Lq * p.D, p.bias, beside);
+  else plan_split(r, c.heads, c.rows, c.total, c.most, min_chunk(always, c.even, c.rows, c.heads * c.rows, c.most, kMinChunk), 4 * c.heads * p.Lq * p.D, p.bias, beside);
   if (one_by_one(p.bias, c.total, c.most, c.rows)) r.group = 1;
   return r;
 }
@@ -831,7 +836,7 @@ PairPlan plan_dkdv_pair(const ra_bwd_step_params& p, const TileCount& c, bool be
   if (one_round && beside) tiles = c.even && wgs <= kPairSlots ? 224 : kWholeRow;
   if (!always && long_stretches(p.bias, p.D, one_round ? kPairSlots + 1 : wgs, c.total, c.rows, tiles)) r.pair = false;
   else if (c.heads * p.Lq + 31 >= (int64_t)1 << 30) r.pair = false;  // one 32-bit byte offset reaches both statistics of a tile's 32 rows
-  else plan_split(r, c.heads, c.rows, c.total, c.most, 2 * kMinChunk, 8 * c.heads * p.Lk * p.D, p.bias, beside);
+  else plan_split(r, c.heads, c.rows, c.total, c.most, min_chunk(always, c.even, c.rows, wgs, c.most, 2 * kMinChunk), 8 * c.heads * p.Lk * p.D, p.bias, beside);
   if (one_by_one(p.bias, c.total, c.most, c.rows)) r.group = 1;
   return r;
 }
