@@ -1953,7 +1953,11 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       } else {
         const float* value = &lds.bias.value[BUF][32 * wave + (at & 31) + (kPairQueries - 1) - 4 * (at >> 5)];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[r] += value[-(8 * (r / 4) + r % 4)];
+        for (int bb = 0; bb < 4; ++bb) {  // (four at a time, for want of registers)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) S[4 * bb + c] += value[-(8 * bb + c)];
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     if (tests) {

@@ -200,17 +200,20 @@ RA_DEV BiasEnds load_bias(const TermArgs& t, int h, float unit, BiasLds<N, GRAD>
   BiasEnds e;
   e.far = t.start[t.side - 1];
   e.future = t.two_sided ? e.far : 0;
-  e.past = load_table(t, t.side - 1, h) * kLog2e;
-  e.ahead = load_table(t, t.two_sided ? 2 * t.side - 1 : 0, h) * kLog2e;
-  e.past = __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(e.past)));
-  e.ahead = __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(e.ahead)));
+  auto uniform = [](float x) {  // (the product, not its factor: a scalar register has no product of its own, and the backward no vector register for it)
+    asm volatile("" : "+v"(x));
+    return __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(x)));
+  };
+  e.past = uniform(load_table(t, t.side - 1, h) * kLog2e);
+  e.ahead = uniform(load_table(t, t.two_sided ? 2 * t.side - 1 : 0, h) * kLog2e);
   return e;
 }
 // The values of the distances d_lo .. d_lo + N - 1 of a tile for the buffer `buf`; all threads of the workgroup.
 template <int N, bool GRAD>
 RA_DEV void write_bias(const TermArgs& t, const BiasEnds& e, BiasLds<N, GRAD>& lds, int buf, int d_lo) {
   if (d_lo + N - 1 <= -e.far || d_lo >= e.future) return;  // constant: nothing reads it
-  const int i = threadIdx.x;
+  int i = threadIdx.x;
+  asm volatile("" : "+v"(i));  // (addresses made here: one that is kept may be spilled, and its reload waits for the tile's loads)
   if (i < N) {
     const int u = ordered_bucket(lds.start, t.side, t.two_sided, d_lo + i);
     lds.value[buf][i] = lds.table[u];
