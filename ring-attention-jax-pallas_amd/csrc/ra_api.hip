@@ -734,13 +734,16 @@ bool one_by_one(const ra_bias& b, int64_t total, int most, int64_t rows) {
 // 156 | 150; 3 of 16384 (384) 284 | 326, 736 | 776; 48 of 758 33 | 27, 86 | 81.  Under a list of tiles the lengths are not known: up to half of the
 // places as many shares as places, and beyond that long rows of the forward by the count (documents of 3000 in 10000, H=5, D=64, 253
 // | 184; short ones lose: documents of 1500 in 4096, H=12, 107 | 121, and so does the backward: prefix 20000, H=3, 1103 | 1202).
+// uneven_most: workgroups of long rows of different lengths that are shared.  With dropout, whose forward takes 1.25 times as long a tile, as many as there are
+// places: not shared | shared, us, forward, causal: 16 heads of 4096, D=128 155 | 136 + 9, with a relative bias 172 | 154 + 10, D=64 125 | 109 + 6 (bias alone 120 | 114 + 9;
+// the backward, 296 | 320 + 16).
 void plan_split(PairPlan& r, int64_t heads, int64_t rows, int64_t total, int most, int min_chunk, int64_t share, const ra_bias& bias,
-                bool beside) {
+                bool beside, int uneven_most = kPairSlots * 3 / 4) {
   const int64_t wgs = heads * rows;
   if (wgs > kPairSlots || most <= min_chunk) return;
   const bool even = even_rows(total, most, rows), few = wgs <= kPairSlots / 2, lists = has_lists(bias);
   int64_t chunk = even ? (most + kPairSlots / wgs - 1) / (kPairSlots / wgs) : heads * total * 3 / (2 * kPairSlots);
-  if (!even && !few && (wgs > kPairSlots * 3 / 4 || most < 8 * min_chunk)) return;
+  if (!even && !few && (wgs > uneven_most || most < 8 * min_chunk)) return;
   if (even && lists && !few && (beside || most < 16 * min_chunk)) return;
   if (even && !(lists && few)) {
     const double pair_rate = lists || (bias.flags & RA_BIAS_ALIBI) ? 1.4 : 1.2;
@@ -776,7 +779,7 @@ bool step_on_pair(const ra_bias& bias, int B, int H, int Lq, int Lk, int D, bool
   return wgs <= kPairSlots ? !even : total < 56 * (int64_t)live;
 }
 // always: the kernels of ra_pair_kernels.h whatever the size (those of ra_terms.hip have no others)
-PairPlan plan_fwd_pair(const ra_fwd_step_params& p, bool always = false) {
+PairPlan plan_fwd_pair(const ra_fwd_step_params& p, bool always = false, bool dropout = false) {
   const int rows = (p.Lq + kPairRowsHost - 1) / kPairRowsHost;
   const int64_t heads = (int64_t)p.B * p.H, wgs = heads * rows;
   int64_t total;
@@ -797,7 +800,8 @@ PairPlan plan_fwd_pair(const ra_fwd_step_params& p, bool always = false) {
     r.chunk_tiles = (most + 1) / 2;
     r.n_split = 2;
   }
-  if (r.pair) plan_split(r, heads, rows, total, most, min_chunk(always, even, rows, wgs, most, kMinChunk), 4 * heads * p.Lq * p.D, p.bias, false);
+  if (r.pair) plan_split(r, heads, rows, total, most, min_chunk(always, even, rows, wgs, most, kMinChunk), 4 * heads * p.Lq * p.D, p.bias, false,
+                         dropout ? kPairSlots : kPairSlots * 3 / 4);
   if (one_by_one(p.bias, total, most, rows)) r.group = 1;
   return r;
 }
@@ -907,9 +911,9 @@ extern "C" {
 
 int ra_version(void) { return 1010; }
 
-static int64_t fwd_pair_workspace(const ra_fwd_step_params* p, bool any_dim, bool always = false) {
+static int64_t fwd_pair_workspace(const ra_fwd_step_params* p, bool any_dim, const ra_terms* terms = nullptr) {
   if (!p || check_dims(p->B, p->H, p->Lq, p->Lk, p->D, any_dim)) return 0;
-  const int n = plan_fwd_pair(*p, always).n_split;
+  const int n = plan_fwd_pair(*p, terms != nullptr, terms && terms->drop).n_split;
   return n > 1 ? fwd_part_bytes(*p, n) : 0;
 }
 
@@ -1006,7 +1010,7 @@ static int fwd_pair(const Before& before, const ra_fwd_step_params* p, bool any_
   if (!lse) return fail(RA_ERR_NULL, "ra_fwd_pair: lse is NULL");
   const RingResult r{out, nullptr, lse, out_dtype, 0, out_stride_b, out_stride_h, out_stride_l};
   if ((rc = check_ring_result("ra_fwd_pair", r, terms != nullptr))) return rc;
-  const PairPlan plan = plan_fwd_pair(*p, terms != nullptr);
+  const PairPlan plan = plan_fwd_pair(*p, terms != nullptr, terms && terms->drop);
   if (!plan.pair) return (rc = before.launch(stream)) ? rc : fwd_passes(p, std::vector<int>{0, 1}, 1, stream, &r);
   ra::PairFwdTermArgs a;
   memset(&a, 0, sizeof(a));
@@ -1516,7 +1520,7 @@ int ra_bwd_call(const ra_rows* before, int32_t n_before, const ra_bwd_step_param
                   dq_stride_l, dk, dv, dkv_stride_b, dkv_stride_h, dkv_stride_l, workspace, workspace_bytes, stream);
 }
 
-int64_t ra_fwd_terms_workspace(const ra_fwd_step_params* p, const ra_terms* t) { return t ? fwd_pair_workspace(p, true, true) : 0; }
+int64_t ra_fwd_terms_workspace(const ra_fwd_step_params* p, const ra_terms* t) { return t ? fwd_pair_workspace(p, true, t) : 0; }
 int64_t ra_bwd_terms_workspace(const ra_bwd_step_params* p, const ra_terms* t) { return t ? bwd_pair_workspace(p, true, t) : 0; }
 
 int ra_fwd_terms(const ra_rows* before, int32_t n_before, const ra_fwd_step_params* p, const ra_terms* t, void* out, int32_t out_dtype,
