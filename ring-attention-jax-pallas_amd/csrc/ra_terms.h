@@ -96,39 +96,33 @@ RA_DEV unsigned lane_dpp(unsigned x) {  // (patterns that read every lane)
 }
 // All ones in the lanes whose number has the bit, and a choice by such a mask.
 RA_DEV unsigned lane_bit(int lane, int bit) { return (unsigned)((int)((unsigned)lane << (31 - bit)) >> 31); }
-RA_DEV unsigned choose(unsigned mask, unsigned a, unsigned b) { return (mask & a) | (~mask & b); }
+RA_DEV unsigned choose(unsigned mask, unsigned a, unsigned b) {
+  unsigned x = (mask & a) | (~mask & b);
+  asm("" : "+v"(x));  // (one register is kept, not the two sides and their merge in every use)
+  return x;
+}
 // Whether the weight of a word's half stays.
 RA_DEV bool stays_low(unsigned w, unsigned drop) { return (unsigned short)w >= (unsigned short)drop; }
 RA_DEV bool stays_high(unsigned w, unsigned drop) { return w >= drop << 16; }
 // ... as a mask of lanes, to be used more than once: such a mask is kept out of VCC, which a v_cndmask reads in 4 cycles right behind the compare and in
-// some 20 every further time (any other scalar pair: 4).
+// some 20 every further time (any other scalar pair: 4).  (Compares and choices are the compiler's, which places the waits between a vector instruction that
+// writes a scalar pair, an exponential or a matrix instruction and the one that reads it; the empty statement keeps the pair.)
 typedef unsigned long long lane_mask;
-RA_DEV lane_mask lanes_low(unsigned w, unsigned drop) {
-  lane_mask m;
-  asm("v_cmp_ge_u16_e64 %0, %1, %2" : "=s"(m) : "v"(w), "s"(drop));
+RA_DEV lane_mask lanes(bool stays) {
+  lane_mask m = __builtin_amdgcn_ballot_w64(stays);
+  asm("" : "+s"(m));
   return m;
 }
-RA_DEV lane_mask lanes_high(unsigned w, unsigned drop) {
-  lane_mask m;
-  asm("v_cmp_ge_u32_e64 %0, %1, %2" : "=s"(m) : "v"(w), "s"(drop << 16));
-  return m;
-}
-RA_DEV float where(lane_mask m, float a, float b) {
-  float x;
-  asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(x) : "v"(b), "v"(a), "s"(m));
-  return x;
-}
-RA_DEV float where_or_0(lane_mask m, float a) {
-  float x;
-  asm("v_cndmask_b32_e64 %0, 0, %1, %2" : "=v"(x) : "v"(a), "s"(m));
-  return x;
-}
+RA_DEV lane_mask lanes_low(unsigned w, unsigned drop) { return lanes(stays_low(w, drop)); }
+RA_DEV lane_mask lanes_high(unsigned w, unsigned drop) { return lanes(stays_high(w, drop)); }
+RA_DEV float where(lane_mask m, float a, float b) { return __builtin_amdgcn_inverse_ballot_w64(m) ? a : b; }
+RA_DEV float where_or_0(lane_mask m, float a) { return where(m, a, 0.f); }
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 // 1 in the halves of two 16-bit values that are at least `least`, which is 1 or more
 RA_DEV u16x2 at_least(unsigned w, unsigned least) {
-  // (packed instructions by name: the compiler makes two compares, two choices and a merge of it)
-  unsigned d;
-  asm("v_pk_sub_u16 %0, %1, %2 clamp" : "=v"(d) : "v"(w), "s"((least - 1) * 0x10001u));
+  const unsigned short most = least - 1;
+  unsigned d = __builtin_bit_cast(unsigned, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, w), u16x2{most, most}));
+  // (by name: the compiler makes two compares, two choices and a merge of it.  Reads and writes one vector register, of a packed subtraction: no waits.)
   asm("v_pk_min_u16 %0, %0, 1 op_sel_hi:[1,0]" : "+v"(d));
   return __builtin_bit_cast(u16x2, d);
 }
