@@ -21,6 +21,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/ring_attention_hip.h"
@@ -498,15 +499,31 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// A leaf whose gradient accumulator another graph keeps alive on another stream: the backward of a captured call would make that stream wait for the
-// capture, which ends the process.
-void check_capture(const Tensor& t) {
-  if (!t.requires_grad() || !t.is_leaf()) return;
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!accumulator) return;
-  const auto s = accumulator->stream();
-  TORCH_CHECK(!s || s->id() == c10::hip::getCurrentHIPStream().id(),
-              "a call on tensors that a live autograd graph of another stream leads to cannot be captured: drop that graph (its outputs) first");
+// Leaves whose gradient accumulators another graph keeps alive on another stream: the backward of a captured call would make that stream wait for
+// the capture, which ends the process.
+void check_capture(const variable_list& inputs) {
+  const auto here = c10::hip::getCurrentHIPStream().id();
+  std::vector<torch::autograd::Node*> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  auto reach = [&](torch::autograd::Node* node) {
+    if (node && seen.insert(node).second) todo.push_back(node);
+  };
+  std::vector<std::shared_ptr<torch::autograd::Node>> accumulators;  // (held while they are looked at)
+  for (const Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad()) continue;
+    if (t.is_leaf()) accumulators.push_back(torch::autograd::impl::try_get_grad_accumulator(t));
+    reach(t.is_leaf() ? accumulators.back().get() : t.grad_fn().get());
+  }
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    if (node->num_outputs() == 0) {  // an accumulator
+      const auto s = node->stream();
+      TORCH_CHECK(!s || s->id() == here,
+                  "a call on tensors that a live autograd graph of another stream leads to cannot be captured: drop that graph (its outputs) first");
+    }
+    for (const auto& edge : node->next_edges()) reach(edge.function.get());
+  }
 }
 
 // attend_terms(q, k, v, plan, scale, the kernels' output dtype, the caller's, position of the first query, of the first key, table or None,
@@ -561,13 +578,11 @@ PyObject* attend_terms(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const c10::DeviceGuard on(q.device());
     for (Tensor* t : {&k, &v})
       if (t->device() != q.device()) *t = t->to(q.device());
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-      for (const Tensor* t : {&q, static_cast<const Tensor*>(&k), static_cast<const Tensor*>(&v)}) check_capture(*t);
-      if (with_table) check_capture(*with_table);
-    }
     check_operands(*call->plan, q, k, v);
     const bool any_grad =
         at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (with_table && with_table->requires_grad()));
+    if (any_grad && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+      check_capture({q, k, v, with_table.value_or(Tensor())});
     got = TermsCall::apply(q, k, v, with_table, seed, call, dtype, final_dtype, any_grad);
   }
   return tuple_of(std::move(got));

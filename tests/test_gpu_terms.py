@@ -337,6 +337,24 @@ def test_cache_of_more_than_two_to_the_31_elements(device):
         _close("lse", lse[:, h:h + 1], w.lse, w.lse_off)
 
 
+def test_capture_beside_a_live_graph_of_leaves_further_up(device):
+    """The same through what the arguments are computed from; without gradients such a capture is an ordinary one."""
+    c = Case(device, Sq=40, relative="both", p=0.1)
+    leaf = c.q.detach().clone().requires_grad_(True)
+    alive = c.call(leaf * 1)[0]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="live autograd graph"):
+        with torch.cuda.graph(graph):
+            c.call(leaf * 1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        held = c.call(leaf)[0]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, alive.detach())
+
+
 def test_capture_beside_a_live_graph_of_the_same_leaves(device):
     c = Case(device, Sq=40, relative="both", p=0.1)
     leaf = c.q.detach().clone().requires_grad_(True)
