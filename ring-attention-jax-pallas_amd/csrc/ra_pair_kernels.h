@@ -585,6 +585,12 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
   constexpr bool GENERAL = MODE != 0;
   constexpr bool DENSE = MODE == 2;
   constexpr bool REL = has_rel(MODE), DROP = has_drop(MODE), HALF = in_half(MODE);
+  // With a relative bias, what a weight loses when it is rounded for the matrix product goes through that as well, and the row is divided by the sum of
+  // the weights themselves.  The table's gradient needs it: most of a bucket's sum cancels (over a row, sum of P (dP - delta) = 0), and a delta = out . dO of
+  // rounded weights is off by their roundings, which cancel in no bucket: 2e-3 of the gradient of 16 buckets (672 x 672, bf16), as much as the
+  // result's own rounding.  Twice the matrix instructions for the output: forward, 16 heads of 2 x 4096, D=64 109 | 142 us, 16 of 4096, D=128, with dropout
+  // 144 | 165.
+  constexpr bool FINE = REL;
   using T = std::conditional_t<HALF, _Float16, bf16_t>;
   using X8 = vec_of<T, 8>;
   using X4 = vec_of<T, 4>;
@@ -892,7 +898,8 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       const float corr = fast_exp2(m_run - ((m_new == RA_NEG_INF) ? 0.f : m_new));
       m_run = m_new;
       l_run *= corr;
-      if constexpr (SUM_MFMA) lr_acc *= corr;
+      if constexpr (FINE) {}
+      else if constexpr (SUM_MFMA) lr_acc *= corr;
       else lr_acc[0] *= corr;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -907,7 +914,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     }
     // The 32 scores of a lane go through exp2 in four groups of eight, one group per 16 keys of the
     // output product: group ks + 1 is worked on while the matrix unit multiplies with group ks.
-    X8 pf[4];
+    X8 pf[4], lost[FINE ? 4 : 1];
     float rs0 = 0.f, rs1 = 0.f;
     unsigned pair0 = 0;
     auto soft = [&](int ks, int e) {  // elements e, e + 1 of group ks
@@ -921,7 +928,21 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       pr[1] = (T)p1;
       unsigned pw = __builtin_bit_cast(unsigned, pr);
       asm volatile("" : "+v"(pw), "+v"(rs0), "+v"(rs1));
-      if constexpr (DROP) {  // (the sums are those of all weights)
+      if constexpr (FINE) {
+        X2 lr = __builtin_bit_cast(X2, pw);
+        lr[0] = (T)(p0 - (float)lr[0]);
+        lr[1] = (T)(p1 - (float)lr[1]);
+        unsigned lw = __builtin_bit_cast(unsigned, lr);
+        asm volatile("" : "+v"(lw));
+        if constexpr (DROP) {
+          const unsigned stay = __builtin_bit_cast(unsigned, at_least(words[ks & 1][e / 2], a.t.drop));
+          lw = times_pair(lw, stay);
+          pw = times_pair(pw, stay);
+        }
+        lr = __builtin_bit_cast(X2, lw);
+        lost[ks][e] = lr[0];
+        lost[ks][e + 1] = lr[1];
+      } else if constexpr (DROP) {  // (the sums are those of all weights)
         if (e % 4 == 0) {
           pair0 = pw;
         } else {
@@ -954,6 +975,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       const int ks = op / DB, db = op % DB;
       if (op + PF < 4 * DB) fr[op + PF] = v_frag(op + PF);
       oacc[db] = mma(fr[op], pf[ks], oacc[db]);
+      if constexpr (FINE) oacc[db] = mma(fr[op], lost[ks], oacc[db]);
       if (ks < 3) {
 #pragma unroll
         for (int e = 4 * db / DB; e < 4 * (db + 1) / DB; ++e) soft(ks + 1, 2 * e);
@@ -962,7 +984,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
       __builtin_amdgcn_sched_barrier(0);
     }
     l_run += rs0 + rs1;
-    if constexpr (DROP) return;
+    if constexpr (DROP || FINE) return;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -998,7 +1020,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
   }
   // a wave without a live score leaves its rows of the carry as they are, unread (m would come back through
   // two unit conversions, a last bit off)
-  const float lr_run = lr_acc[0];
+  const float lr_run = FINE ? l_run : lr_acc[0];
   if (e->o != nullptr && __all(l_run == 0.f && lr_run == 0.f)) return;
   const float l_step = half_sum(l_run), lr_step = half_sum(lr_run);
   if (e->part_n != nullptr && split == 0 && tid == 0) e->part_n[hh * nqt + qt] = n_piece;

@@ -126,9 +126,12 @@ RA_DEV u16x2 at_least(unsigned w, unsigned least) {
   asm("v_pk_min_u16 %0, %0, 1 op_sel_hi:[1,0]" : "+v"(d));
   return __builtin_bit_cast(u16x2, d);
 }
+RA_DEV unsigned times_pair(unsigned x, unsigned y) {
+  return __builtin_bit_cast(unsigned, (u16x2)(__builtin_bit_cast(u16x2, x) * __builtin_bit_cast(u16x2, y)));
+}
 // Two 16-bit elements, of which those stay whose halves of `w` do.
 RA_DEV unsigned keep_pair(unsigned pair, unsigned w, unsigned drop) {
-  return __builtin_bit_cast(unsigned, (u16x2)(__builtin_bit_cast(u16x2, pair) * at_least(w, drop)));
+  return times_pair(pair, __builtin_bit_cast(unsigned, at_least(w, drop)));
 }
 
 // The seed's words, as uniform values.

@@ -259,6 +259,26 @@ def test_results_do_not_change_with_the_ring_or_from_call_to_call(device, relati
             assert all(torch.equal(x, y) for x, y in zip((*first[:2], *first[2]), (*got[:2], *got[2])))
 
 
+@pytest.mark.parametrize("kw", [dict(mask="", relative="both", B=2, Sq=672, D=128, buckets=16), dict(mask="causal", relative="past", Sq=700, p=0.1),
+                                dict(mask="causal", relative="past", Sq=300, dtype=torch.float16),
+                                dict(mask="", relative="both", Sq=500, D=96, p=0.3, buckets=16, dtype=torch.float16)])
+def test_table_gradient_is_free_of_the_weights_roundings(device, kw):
+    """A bucket's sum cancels to a small part of its terms, so the roundings of the forward's weights (half a step of 16 bits) must not reach it through
+    delta.  What they would do is computed here; what remains are roundings of twice 16 bits, 2^-9 of that (fp16: 2^-12, and weights below 2^-14 lose up
+    to 2^-25), and scores in 32 bits, some 2^-20 of a weight and so 2^-11 (fp16: 2^-8) of it: an eighth leaves room for both."""
+    c = Case(device, H=4, **{"B": 1, "table_dtype": torch.float32, "dtype": torch.bfloat16, **kw})
+    w = c.want()
+    got = c.grads()[2][3].double()
+    want, _ = w.table_gradient(c.bucket, c.buckets, 0.0)
+    v, do = (x.double().permute(0, 2, 1, 3) for x in (c.v, c.do))
+    weights = w.P / w.P.amax(3, keepdim=True)
+    rounded = weights.to(c.dtype).double()
+    lost = (rounded / rounded.sum(3, keepdim=True) - w.P) * (1.0 if c.keep is None else c.keep.double() / (1 - c.threshold / 65536))
+    through_delta = w.P * ((lost @ v) * do).sum(3, keepdim=True)
+    lossy = torch.stack([(through_delta * (c.bucket == u)).sum((0, 2, 3)) for u in range(c.buckets)])
+    assert float((got - want).norm()) <= float(lossy.norm()) / 8
+
+
 def test_seed_on_the_device(device):
     c = Case(device, B=1, H=2, Sq=130, p=0.5, relative="both")
     for seed in (c.dropout.seed, (1 << 64) - 3, -3):
