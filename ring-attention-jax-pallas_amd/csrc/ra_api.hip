@@ -366,7 +366,7 @@ int check_pass_counts(const int32_t* steps_per_pass, int32_t n_passes, std::vect
   return RA_OK;
 }
 
-// ---- steps on a dense block: the kernels of ra_pair.hip, one launch per step ----------------------------
+// ---- steps on a dense block: the kernels of ra_pair_kernels.h, one launch per step ----------------------------
 // What bounds such a step is the block's elementwise term (one fp32 read and add per score), which the long-stretch kernels pay
 // in generic iterations, one workgroup per compute unit with nothing beside it; the pair kernels have a second workgroup
 // there, and leave a carry or accumulator alone whose tiles are all masked.  Forward + backward, long-stretch kernels -> these:
@@ -655,11 +655,11 @@ int bwd_dkdv_passes(const ra_bwd_step_params* steps, const std::vector<int>& fir
 }
 
 // ---- one pair of sequences: which kernels, and how many workgroups share a row's keys --------------
-constexpr int kPairSlots = 512;  // workgroups of ra_pair.hip that the chip holds at once: two per compute unit
+constexpr int kPairSlots = 512;  // workgroups of ra_pair_kernels.h that the chip holds at once: two per compute unit
 constexpr int kPairRowsHost = 128, kPairKeysHost = 64;
 
 struct PairPlan {
-  bool pair;        // the kernels of ra_pair.hip
+  bool pair;        // the kernels of ra_pair_kernels.h
   int n_split;      // most workgroups that share a row's keys ...
   int chunk_tiles;  // ... each of about this many tiles
   int group;        // heads of an XCD that are taken together (see pair_decode)
@@ -686,7 +686,7 @@ void count_key_tiles(const ra_bias& bias, int Lq, int Lk, int64_t& total, int& m
 // Whether the kernels of ra_fwd.hip / ra_bwd.hip, which hold twice the rows or keys per compute unit and hide all
 // vector work in straight-line stretches, are the faster ones: nothing but positions and ALiBi masks, D = 128, a
 // grid that fills the chip, and at least `tiles` tiles per workgroup on average.  With a list of tiles (documents,
-// prefix, dense block) or D = 64 those of ra_pair.hip are (documents + ALiBi, 32768, H=16: forward 1.1 ms against 1.4,
+// prefix, dense block) or D = 64 those of ra_pair_kernels.h are (documents + ALiBi, 32768, H=16: forward 1.1 ms against 1.4,
 // dQ 1.25 against 1.53, dK/dV 1.87 against 1.88; causal documents of mean 1024, 8192, B=2, H=16: 0.29 / 0.22 / 0.30
 // against 0.39 / 0.35 / 0.42; prefix-LM 16384, H=16: 5.6 ms in total against 18; D=64, 32768 causal, H=16: 2.34 / 2.79 /
 // 3.75 against 2.39 / 3.15 / 3.92).
@@ -917,7 +917,7 @@ static int64_t fwd_pair_workspace(const ra_fwd_step_params* p, bool any_dim, con
   return n > 1 ? fwd_part_bytes(*p, n) : 0;
 }
 
-// A head dim that only the kernels of ra_pair.hip have, and those without a dense block.
+// A head dim that only the kernels of ra_pair_kernels.h have, and those without a dense block.
 static bool narrow(int D) { return D != 64 && D != 128; }
 static int check_whole_call(const char* what, int D, const ra_bias& bias) {
   if (narrow(D) && (bias.flags & RA_BIAS_DENSE))

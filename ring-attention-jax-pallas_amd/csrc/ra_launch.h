@@ -105,7 +105,7 @@ struct QRing {
   const int* kv_pre[kMaxPasses];
 };
 
-// One (query sequence, key sequence) pair on the kernels of ra_pair.hip.
+// One (query sequence, key sequence) pair on the kernels of ra_pair_kernels.h.
 struct PairFwdArgs {
   TensorArg q, k, v;
   int B, H, Lq, Lk;

@@ -11,6 +11,7 @@ namespace ra {
 // (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011: the fewest that pass all of their tests) with the
 // seed as key and the counter (j / 2, i / 4, hh, 0); query i's word is the (i % 4)-th, an even key's half the low one.  A call serves eight weights
 // whichever side the kernel's lanes own: four neighbouring lanes with a query each exchange words, and two with a key each halves.
+// Vector issue bounds the kernels with dropout.  16 heads of 8192, causal, us, without | with: D=128 forward 322 | 390 (705 TFLOP/s), backward 838 | 1037.
 // ------------------------------------------------------------------------------------------------
 constexpr unsigned kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u, kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
 RA_DEV unsigned xor3(unsigned a, unsigned b, unsigned c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
@@ -144,7 +145,9 @@ RA_DEV void load_seed(const TermArgs& t, unsigned& k0, unsigned& k1) {
 // ------------------------------------------------------------------------------------------------
 // The relative bias.  It is a function of the distance d = key - query, constant from the last bucket's start on (and, one-sided, from 0 on): a
 // block of 32 x 32 scores that lies there takes one number into its exponents, and no other work.  For the tiles on the way the
-// workgroup writes the values of a tile's distances to LDS, one a thread, while the tile is on its way, and a score reads its own.
+// workgroup writes the values of a tile's distances to LDS, one a thread, while the tile is on its way, and a score reads its own.  A token on 32768
+// keys (4 batch rows of 16 heads, padded, D=128) runs at what memory gives, the others are bound as the kernels without it: 16 heads of 2 x 4096, causal, D=64, us, without | with: backward
+// 259 | 293, forward 105 | 141 (106 but for the second product of the output, see fwd_pair_kernel).
 // ------------------------------------------------------------------------------------------------
 // Buckets in the order of d: the far past first, the far future last (one-sided: bucket 0 last).
 RA_DEV int ordered_bucket(const int* start, int side, bool two_sided, int d) {
