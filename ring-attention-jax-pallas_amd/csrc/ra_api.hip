@@ -954,21 +954,7 @@ static int check_terms(const ra_terms& t, const ra_bias& bias, int out_dtype) {
   return RA_OK;
 }
 
-// Which end of the distances holds more than half of the pairs (TermArgs::derive), by the positions of every 128th row.
-static int larger_end(const ra_terms& t, const ra_bias& bias, int Lq, int Lk) {
-  const int64_t far = t.starts[(t.two_sided ? t.n_buckets / 2 : t.n_buckets) - 1], ahead = t.two_sided ? far : 0;
-  auto keys = [&](int64_t n) { return std::min<int64_t>(std::max<int64_t>(n, 0), Lk); };
-  int64_t past = 0, future = 0, all = 0;
-  for (int64_t i = 0; i < Lq; i += kPairRowsHost) {
-    const int64_t at = bias.q_offset + std::min<int64_t>(i + kPairRowsHost / 2, Lq - 1) - bias.kv_offset;  // the middle row's position among the keys'
-    past += keys(at - far + 1);
-    future += (bias.flags & RA_BIAS_CAUSAL) ? 0 : keys(Lk - (at + ahead));
-    all += (bias.flags & RA_BIAS_CAUSAL) ? keys(at + 1) : Lk;
-  }
-  return 2 * past > all ? -1 : 2 * future > all ? 1 : 0;
-}
-
-static ra::TermArgs to_terms(const ra_terms& t, const ra_bias& bias, int Lq, int Lk) {
+static ra::TermArgs to_terms(const ra_terms& t) {
   static_assert(ra::kMaxSide == RA_MAX_SIDE, "buckets of a side");
   ra::TermArgs r;
   memset(&r, 0, sizeof(r));
@@ -980,7 +966,6 @@ static ra::TermArgs to_terms(const ra_terms& t, const ra_bias& bias, int Lq, int
     r.two_sided = t.two_sided != 0;
     r.side = r.two_sided ? t.n_buckets / 2 : t.n_buckets;
     memcpy(r.start, t.starts, sizeof(int) * r.side);
-    r.derive = larger_end(t, bias, Lq, Lk);
   }
   r.half = t.operands == RA_DTYPE_F16;
   r.rest = t.rest;
@@ -1045,7 +1030,7 @@ static int fwd_pair(const Before& before, const ra_fwd_step_params* p, bool any_
   if ((rc = before.launch(stream))) return rc;
   if (terms) {
     a.out_f32 = out_dtype;  // (any of them)
-    a.t = to_terms(*terms, p->bias, p->Lq, p->Lk);
+    a.t = to_terms(*terms);
   }
   hipError_t e = terms ? ra::launch_fwd_terms(a, p->D, (hipStream_t)stream)
                        : ra::launch_fwd_pair(a, p->D, kernel_mode(p->bias.flags), (hipStream_t)stream);
@@ -1393,7 +1378,7 @@ static int bwd_pair(const Before& before, const ra_bwd_step_params* p, bool any_
   st.dout_vec = 1;
   st.lse = c.lse;
   ra::TermArgs extra;
-  if (terms) extra = to_terms(*terms, c.bias, c.Lq, c.Lk);
+  if (terms) extra = to_terms(*terms);
   const int operand_dtype = terms ? terms->operands : RA_DTYPE_BF16;
   if (operand_dtype == RA_DTYPE_F16) {  // (a power of two would leave fp16's range where it does not leave bf16's)
     a.a.scale_p2 = 1.0f;

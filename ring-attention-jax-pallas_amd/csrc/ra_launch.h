@@ -173,7 +173,6 @@ struct TermArgs {
   // its gradient (nullptr: none): sums of a workgroup, [B * H, tiles of 128 queries, n_split][kGradRow] (see table_grad_kernel), and where it goes
   float* grad_part;
   void* grad;
-  int derive;  // the end whose bucket is derived from the others (see BiasGrad): -1 the past's, 1 the future's, 0 neither
   int half;  // the operands are fp16, not bf16
   // What the rounded output lacks, of the operands' type and laid out as the output: the backward's delta is taken from both, as exactly as the
   // gradients can use it (nullptr: no backward will come, or the output is fp32).
@@ -184,7 +183,7 @@ struct TermArgs {
   const unsigned long long* seed_at;  // nullptr: seed
   unsigned long long seed;
 };
-constexpr int kGradRow = 2 * kMaxSide + 2;  // a sum for each bucket, and whether a pair of the derived bucket was there
+constexpr int kGradRow = 2 * kMaxSide;  // a sum for each bucket
 struct PairFwdTermArgs : PairFwdArgs {
   TermArgs t;
 };

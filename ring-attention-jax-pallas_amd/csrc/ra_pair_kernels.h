@@ -1155,18 +1155,12 @@ struct DqLds {
 //    so what the lane off further holds lies on the same diagonal: sixteen fetches across the wave sum the 63 diagonals, a lane having a
 //    part of two.  They are put in the order of d and summed up from the first one on; lane u then takes bucket u (and 64 + u) as the difference of two of these
 //    sums.
-//  * Blocks of a constant bias: a sum per lane for either end.  Where more than half of all pairs lie at one end (TermArgs::derive), no
-//    work is done for that one: its bucket is minus all the others' sum, since the dS of a row add up to zero (P adds up to one, and delta is the mean of
-//    dP).  That is the more exact way too: an error of delta is the same in every pair of a row, weighted with P, and adds up
-//    over a bucket that holds most of the row.  A bucket that no pair has keeps its zero (reached).
+//  * Blocks of a constant bias: a sum per lane for either end.  (The dS of a row add up to zero, so one end could be had as minus the others' sum.  It
+//    would hold the roundings of all of them, whatever its own weight: no bucket's sum is taken from another's.)
 struct BiasGrad {
   float low_sum, high_sum;  // buckets 0 .. 63 and 64 .. 127 by lane
   float past, ahead;  // the ends
-  bool reached;
-  RA_DEV void init() {
-    low_sum = high_sum = past = ahead = 0.f;
-    reached = false;
-  }
+  RA_DEV void init() { low_sum = high_sum = past = ahead = 0.f; }
   RA_DEV void add(int u, float x, int lane) {  // u, x uniform
     if (u < 64) low_sum += lane == u ? x : 0.f;
     else high_sum += lane == u - 64 ? x : 0.f;
@@ -1526,15 +1520,11 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
         S *= P;
         if (bias_grad_on) {
           if (side != 0) {
-            if (side == terms.derive) {
-              bias_grad.reached = bias_grad.reached || rel != RA_NEG_INF;  // (that masks all of its pairs)
-            } else {
-              float t = 0.f;
+            float t = 0.f;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) t += S[r];
-              if (side < 0) bias_grad.past += t;
-              else bias_grad.ahead += t;
-            }
+            for (int r = 0; r < 16; ++r) t += S[r];
+            if (side < 0) bias_grad.past += t;
+            else bias_grad.ahead += t;
           } else {
             bias_grad.add_block(S, lds.bias, n_buckets, (kv_off + kt0 + 32 * kb) - (q_off + qw), opaque_lane(lane));
           }
@@ -1598,13 +1588,12 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
   if constexpr (REL) {
     if (bias_grad_on) {
       const int n = n_buckets;
-      float* const s_sum = (float*)s_k;  // [4][2 kMaxSide], and whether the derived bucket was there
+      float* const s_sum = (float*)s_k;  // [4][2 kMaxSide]
       __syncthreads();                   // (nobody reads the tiles any more)
       bias_grad.add(0, wave_sum(bias_grad.past), lane);
       bias_grad.add(n - 1, wave_sum(bias_grad.ahead), lane);
       s_sum[wave * 2 * kMaxSide + lane] = bias_grad.low_sum;
       s_sum[wave * 2 * kMaxSide + 64 + lane] = bias_grad.high_sum;
-      if (lane == 0) s_sum[8 * kMaxSide + wave] = bias_grad.reached ? 1.f : 0.f;
       __syncthreads();
       float* const part = terms.grad_part + (((long long)hh * nqt + qt) * p.n_split + split) * kGradRow;
       if (tid < n) {
@@ -1613,8 +1602,6 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
         for (int w = 0; w < 4; ++w) t += s_sum[w * 2 * kMaxSide + tid];
         part[tid] = DROP ? t * terms.inv_keep : t;
       }
-      if (tid == n)
-        part[2 * kMaxSide] = fmaxf(fmaxf(s_sum[8 * kMaxSide], s_sum[8 * kMaxSide + 1]), fmaxf(s_sum[8 * kMaxSide + 2], s_sum[8 * kMaxSide + 3]));
     }
   }
   const auto* e = kernel_args<PairBwdArgs>(args_at);

@@ -8,15 +8,15 @@ namespace ra {
 // buckets, H=16; now 6.1 to 6.7, of which the 0.5 MB would be 0.1 at a large copy's rate).
 constexpr int kGradThreads = 512, kGradAhead = 8;
 __global__ __launch_bounds__(kGradThreads) void table_grad_kernel(const TermArgs t, const int* part_n, int B, int H, int tiles, int n_split) {
-  __shared__ float s_sum[kGradThreads], s_reached[kGradThreads / 64];
+  __shared__ float s_sum[kGradThreads];
   const int n = t.two_sided ? 2 * t.side : t.side, h = blockIdx.x, tid = threadIdx.x;
   int width = 2;
   while (width < n) width *= 2;
   const int u = tid % width, first = tid / width, step = kGradThreads / width;
-  float sum = 0.f, reached = 0.f;
+  float sum = 0.f;
   const int rows = B * tiles * n_split;
   for (int i0 = first; i0 < rows; i0 += kGradAhead * step) {
-    float x[kGradAhead], r[kGradAhead];
+    float x[kGradAhead];
     int pieces[kGradAhead];
 #pragma unroll
     for (int a = 0; a < kGradAhead; ++a) {
@@ -25,33 +25,17 @@ __global__ __launch_bounds__(kGradThreads) void table_grad_kernel(const TermArgs
       const float* row = t.grad_part + (at * n_split + i % n_split) * kGradRow;
       pieces[a] = part_n != nullptr ? max(part_n[at], 1) : 1;
       x[a] = row[min(u, n - 1)];  // (of a share that there is not: whatever lies there)
-      r[a] = row[2 * kMaxSide];
     }
 #pragma unroll
     for (int a = 0; a < kGradAhead; ++a) {
       const int i = i0 + a * step;
-      const bool there = i < rows && i % n_split < pieces[a];
-      sum += there ? x[a] : 0.f;
-      reached = there ? fmaxf(reached, r[a]) : reached;
+      sum += i < rows && i % n_split < pieces[a] ? x[a] : 0.f;
     }
   }
   s_sum[tid] = sum;
-  reached = __any(reached > 0.f) ? 1.f : 0.f;
-  if ((tid & 63) == 0) s_reached[tid >> 6] = reached;
-  __syncthreads();
-  if (tid < width)
-    for (int i = 1; i < step; ++i) sum += s_sum[tid + i * width];
-  __syncthreads();
-  if (tid < n) s_sum[tid] = sum;
   __syncthreads();
   if (tid >= n) return;
-  // the derived bucket: minus all the others
-  const int derived = t.derive > 0 ? n - 1 : 0;
-  for (int w = 0; w < kGradThreads / 64; ++w) reached = fmaxf(reached, s_reached[w]);
-  if (t.derive != 0 && tid == derived && reached > 0.f) {
-    sum = 0.f;
-    for (int i = 0; i < n; ++i) sum -= i == derived ? 0.f : s_sum[i];
-  }
+  for (int i = 1; i < step; ++i) sum += s_sum[tid + i * width];
   const long long at = (long long)table_row(tid, t.side) * H + h;
   if (t.table_dtype == RA_DTYPE_F32) ((float*)t.grad)[at] = sum;
   else if (t.table_dtype == RA_DTYPE_F16) ((_Float16*)t.grad)[at] = (_Float16)sum;

@@ -1,0 +1,72 @@
+"""Gradients of a relative bias's table bucket by bucket: what a bucket gets is the sum over its own pairs, whatever the others hold."""
+import pytest
+import torch
+
+import ring_attention as ra
+from oracle import terms_oracle as T
+
+pytestmark = pytest.mark.gpu
+
+
+class Call:
+    """A call with a bias whose table is `table` [buckets, H]; ids: (q side, kv side) of a segment term, window: of a window term."""
+
+    def __init__(self, device, table, *, Sq, Sk=None, B=1, D=64, q_off=0, causal=False, window=None, ids=None, two=True, distance=128, p=0.0,
+                 dtype=torch.bfloat16, seed=0):
+        Sk = Sq if Sk is None else Sk
+        g = torch.Generator().manual_seed(seed)
+        H = table.shape[1]
+        self.q, self.k, self.v, self.do = (torch.randn(B, S, H, D, generator=g).to(device, dtype) for S in (Sq, Sk, Sk, Sq))
+        self.table = table.to(device)
+        at = torch.arange(Sk, device=device)[None] - q_off - torch.arange(Sq, device=device)[:, None]
+        self.buckets, self.bucket = table.shape[0], T.bucket_of(at, table.shape[0], distance, two)
+        self.fn = ra.causal_bias() if causal else None
+        add = lambda t: t if self.fn is None else self.fn + t  # noqa: E731
+        if window is not None:
+            self.fn = add(ra.sliding_window_bias(window, causal=causal))
+        self.q_kw, self.kv_kw = ({"q_positions": q_off} if q_off else {}), {}
+        if ids is not None:
+            self.fn = add(ra.segment_bias())
+            self.q_kw["q_segment_ids"], self.kv_kw["kv_segment_ids"] = (x.to(device) for x in ids)
+        self.term = dict(max_distance=distance, bidirectional=two)
+        self.live = T.scores_mask(Sq, Sk, q_off=q_off, causal=causal, window=window, segments=ids, device=device).expand(B, 1, Sq, Sk)
+        self.dropout = ra.Dropout(p, 99) if p else None
+        self.threshold = round(p * 65536)
+        self.keep = T.keep_mask(99, self.threshold, B, H, Sq, Sk, device) if p else None
+        self.eps = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -10
+
+    def gradient(self):
+        leaf = self.table.clone().requires_grad_(True)
+        term = ra.relative_bias(leaf, **self.term)
+        out = ra.ring_attention(self.q, self.k, self.v, 1, term if self.fn is None else self.fn + term, self.q_kw, self.kv_kw, dropout=self.dropout)
+        return torch.autograd.grad(out, leaf, self.do)[0]
+
+    def reached(self):
+        """Which buckets a live pair lies in."""
+        got = torch.zeros(self.buckets, dtype=torch.bool, device=self.table.device)
+        got[self.bucket.expand(self.live.shape)[self.live].unique()] = True
+        return got
+
+
+def _documents(B, S, n):
+    ids = (torch.arange(S) // n).to(torch.int32)[None].expand(B, S).contiguous()
+    return ids, ids
+
+
+def _table(buckets, H, seed=3):
+    return torch.randn(buckets, H, generator=torch.Generator().manual_seed(seed))
+
+
+ENDS = [dict(Sq=300, causal=True, window=100, two=False), dict(Sq=701, causal=True, window=113, two=False, D=128, p=0.2),
+        dict(Sq=600, ids=_documents(2, 600, 50), B=2), dict(Sq=600, causal=True, ids=_documents(1, 600, 90), two=False, dtype=torch.float16)]
+
+
+@pytest.mark.parametrize("kw", ENDS)
+def test_an_end_that_other_terms_mask_gets_zero(device, kw):
+    """Keys far away are there by their positions, but a window or documents leave none of them: the last bucket's gradient is zero, not a remainder of
+    the others'."""
+    c = Call(device, _table(32, 3), **kw)
+    empty = ~c.reached()
+    assert empty.any()
+    grad = c.gradient()
+    assert (grad[~empty] != 0).any() and (grad[empty] == 0).all(), grad[empty]
