@@ -1153,8 +1153,9 @@ struct DqLds {
 // that is where they are taken, in an order that does not change.
 //  * Blocks on the way from one end of the distances to the other: a lane l of half g holds keys off + 4 g, off = 0 .. 3, 8 .. 11, .., of query l,
 //    so what the lane off further holds lies on the same diagonal: sixteen fetches across the wave sum the 63 diagonals, a lane having a
-//    part of two.  They are put in the order of d and summed up from the first one on; lane u then takes bucket u (and 64 + u) as the difference of two of these
-//    sums.
+//    part of two.  They are put in the order of d and summed up, each bucket's from its own first one on; lane u then takes the sum at the last one of
+//    bucket u (and 64 + u).  (Differences of sums from the block's first diagonal on cost a step less in each addition and leave a bucket without a live pair,
+//    or of little weight, a rounding of its neighbours.)
 //  * Blocks of a constant bias: a sum per lane for either end.  (The dS of a row add up to zero, so one end could be had as minus the others' sum.  It
 //    would hold the roundings of all of them, whatever its own weight: no bucket's sum is taken from another's.)
 struct BiasGrad {
@@ -1165,9 +1166,10 @@ struct BiasGrad {
     if (u < 64) low_sum += lane == u ? x : 0.f;
     else high_sum += lane == u - 64 ? x : 0.f;
   }
-  // x: dS of the block in which lane 0's query and the first key are `base` apart
+  // x: dS of the block in which lane 0's query and the first key are `base` apart; its lowest distance is the at-th of the tile in the buffer `buf`
   template <typename Lds>
-  RA_DEV void add_block(const f32x16& x, const Lds& lds, int n_buckets, int base, int lane) {
+  RA_DEV void add_block(const f32x16& x, const Lds& lds, int n_buckets, int buf, int at, int base, int lane) {
+    const int first = lds.first[buf][at + lane] - at;
     float d0 = 0.f, d1 = 0.f;  // of the diagonals 4 g - l, and 32 more than 4 (1 - g) - l (from the other half's lanes)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -1180,17 +1182,17 @@ struct BiasGrad {
       // lanes whose fetch has passed the end of their half
       unsigned half;  // (volatile: a constant is not worth a scalar register through the loop)
       asm volatile("s_mov_b32 %0, %1" : "=s"(half) : "i"((int)(0xffffffffu << (32 - off))));
-      d1 += where_or_0((lane_mask)half << 32 | half, y);
-      d0 += y;
+      const lane_mask m = (lane_mask)half << 32 | half;
+      d1 += where_or_0(m, y);
+      d0 += where(m, 0.f, y);
     }
-    d0 -= d1;
     // in lane e the diagonal base + e - 31: its parts are in lanes 31 - e and 67 - e (mod 64), in d0 or d1 by the half
     const float low = lane < 32 ? d0 : d1, high = lane < 32 ? d1 : d0;
-    const float upto = wave_scan(lane_at(4 * 31 - 4 * lane, low) + lane_at(4 * 67 - 4 * lane, high));
+    const float upto = wave_scan(lane_at(4 * 31 - 4 * lane, low) + lane_at(4 * 67 - 4 * lane, high), lane, first);
     auto bucket = [&](int u) {
       const int hi = min(lds.hi[u] - base, 31) + 31, lo = max(lds.lo[u] - base, -31) + 31;
-      const float a = lane_at(4 * hi, upto), b = lane_at(4 * lo - 4, upto);
-      return hi >= lo ? (lo > 0 ? a - b : a) : 0.f;
+      const float sum = lane_at(4 * hi, upto);
+      return hi >= lo ? sum : 0.f;
     };
     low_sum += bucket(lane);
     if (n_buckets > 64) high_sum += bucket(64 + lane);
@@ -1526,7 +1528,7 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
             if (side < 0) bias_grad.past += t;
             else bias_grad.ahead += t;
           } else {
-            bias_grad.add_block(S, lds.bias, n_buckets, (kv_off + kt0 + 32 * kb) - (q_off + qw), opaque_lane(lane));
+            bias_grad.add_block(S, lds.bias, n_buckets, BUF, kPairRows - 32 * (wave + 1) + 32 * kb, (kv_off + kt0 + 32 * kb) - (q_off + qw), opaque_lane(lane));
           }
         }
       }

@@ -161,10 +161,12 @@ RA_DEV int table_row(int ordered, int side) { return ordered >= side ? ordered :
 // N: the distances of a tile
 template <int N, bool GRAD>
 struct BiasLds {
+  static_assert(N <= 256, "first");
   float value[2][N];          // of the tiles of the two buffers
   float table[2 * kMaxSide];  // of this head, in the order of d
   int start[kMaxSide];
   int lo[GRAD ? 2 * kMaxSide : 1], hi[GRAD ? 2 * kMaxSide : 1];  // the distances of a bucket (in that order; hi < lo: none)
+  unsigned char first[2][GRAD ? N : 1];  // where the bucket of a tile's distance begins among them
 };
 RA_DEV float load_table(const TermArgs& t, int row, int h) {
   const long long at = row * t.table_sb + h * t.table_sh;
@@ -217,6 +219,7 @@ RA_DEV void write_bias(const TermArgs& t, const BiasEnds& e, BiasLds<N, GRAD>& l
   if (i < N) {
     const int u = ordered_bucket(lds.start, t.side, t.two_sided, d_lo + i);
     lds.value[buf][i] = lds.table[u];
+    if constexpr (GRAD) lds.first[buf][i] = (unsigned char)max(lds.lo[u] - d_lo, 0);
   }
 }
 
@@ -239,18 +242,20 @@ RA_DEV float wave_sum(float x) {
   return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
-// Sums of a wave's lanes up to and including each.
-RA_DEV float wave_scan(float x) {
-  auto add = [&](auto ctrl, auto rows) {
-    x += __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+// Sums of a wave's lanes from lane `first` (each lane's own, the same for all lanes on the way to it) up to and including each.  A sum takes nothing from
+// lanes before its first one, not even to subtract it again.
+RA_DEV float wave_scan(float x, int lane, int first) {
+  auto add = [&](auto ctrl, auto rows, bool same) {
+    const float y = __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    x += same ? y : 0.f;
   };
   using All = std::integral_constant<int, 0xf>;
-  add(std::integral_constant<int, 0x111>{}, All{});  // one lane to the right inside rows of 16, two, four, eight
-  add(std::integral_constant<int, 0x112>{}, All{});
-  add(std::integral_constant<int, 0x114>{}, All{});
-  add(std::integral_constant<int, 0x118>{}, All{});
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // the last lane of a row to the next row, of the first half to the second
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  add(std::integral_constant<int, 0x111>{}, All{}, lane - 1 >= first);  // one lane to the right inside rows of 16, two, four, eight
+  add(std::integral_constant<int, 0x112>{}, All{}, lane - 2 >= first);
+  add(std::integral_constant<int, 0x114>{}, All{}, lane - 4 >= first);
+  add(std::integral_constant<int, 0x118>{}, All{}, lane - 8 >= first);
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}, (lane & 48) > first);  // the last lane of a row to the next row, of the first half to the second
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}, 32 > first);
   return x;
 }
 // lane (from / 4) mod 64's value

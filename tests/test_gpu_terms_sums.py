@@ -1,4 +1,6 @@
 """Gradients of a relative bias's table bucket by bucket: what a bucket gets is the sum over its own pairs, whatever the others hold."""
+import math
+
 import pytest
 import torch
 
@@ -47,6 +49,19 @@ class Call:
         got[self.bucket.expand(self.live.shape)[self.live].unique()] = True
         return got
 
+    def want(self):
+        """[buckets, H] in 64 bits, and how far off a sum over a bucket's own pairs in 32 bits may be."""
+        bias = self.table.double()[self.bucket].permute(2, 0, 1)
+        w = T.Attention(self.q, self.k, self.v, do=self.do, live=self.live, bias=bias, keep=self.keep, threshold=self.threshold, eps=self.eps)
+        got, off = [], []
+        for u in range(self.buckets):
+            at = self.bucket == u
+            got.append(w.dS[:, :, at].sum((0, 2)))
+            # a pair's part in 32 bits; every sum on the way (of 16 of a lane, its blocks, a wave, workgroups, diagonals: fewer than 256 one
+            # after the other) is of this bucket's pairs, half a step of 32 bits each
+            off.append((w.dS_off32 + 256 * 2.0 ** -24 * w.dS.abs())[:, :, at].sum((0, 2)))
+        return torch.stack(got), torch.stack(off) + 1e-36
+
 
 def _documents(B, S, n):
     ids = (torch.arange(S) // n).to(torch.int32)[None].expand(B, S).contiguous()
@@ -58,7 +73,8 @@ def _table(buckets, H, seed=3):
 
 
 ENDS = [dict(Sq=300, causal=True, window=100, two=False), dict(Sq=701, causal=True, window=113, two=False, D=128, p=0.2),
-        dict(Sq=600, ids=_documents(2, 600, 50), B=2), dict(Sq=600, causal=True, ids=_documents(1, 600, 90), two=False, dtype=torch.float16)]
+        dict(Sq=600, ids=_documents(2, 600, 50), B=2), dict(Sq=600, causal=True, ids=_documents(1, 600, 90), two=False, dtype=torch.float16),
+        dict(Sq=1000, window=90, p=0.1)]
 
 
 @pytest.mark.parametrize("kw", ENDS)
@@ -70,3 +86,15 @@ def test_an_end_that_other_terms_mask_gets_zero(device, kw):
     assert empty.any()
     grad = c.gradient()
     assert (grad[~empty] != 0).any() and (grad[empty] == 0).all(), grad[empty]
+
+
+@pytest.mark.parametrize("kw", [dict(Sq=500, two=True), dict(Sq=500, causal=True, two=False, D=128), dict(Sq=400, two=True, p=0.2, dtype=torch.float16)])
+def test_buckets_of_little_weight_are_their_own_sums(device, kw):
+    """The last buckets of either side hold most pairs, others a diagonal or a few between others, and all of these next to no weight (a learned bias of
+    -40): their gradients are that small."""
+    table, small = _table(32, 2), [0, 3, 10, 15, 18, 22, 31]
+    table[small] = -40.0
+    c = Call(device, table, **kw)
+    grad, (want, off) = c.gradient().double(), c.want()
+    for u in small:
+        assert ((grad[u] - want[u]).abs() <= off[u] + 2.0 ** -24 * want[u].abs()).all(), (u, grad[u], want[u], off[u])
