@@ -1201,6 +1201,26 @@ struct BiasGrad {
 template <int MODE>
 using TermsOf = std::conditional_t<(MODE >= 3), TermArgs, NoLds>;
 
+// fp16's range is short for dS and for the weights of dV: a weight of one key in 4096 lies next to its smallest normal number, 2^-14, and dS is that times
+// dO.  So both are rounded in units of their own.  Weights: 2^-14, as a constant in the exponent.  dS: a power of two
+// that follows the largest one met so far, as a softmax follows its maximum: where a block holds a larger one than `most`, the sums so far go down to the
+// new unit.  The largest is put 16 to 32 times below `most`, which few blocks pass later on, and its rounding is a normal number's down to 2^-24 of it.  dQ has
+// a unit for each query, dK one for the 32 keys of a wave.  Backward without units | with them, us: bias, 771 tokens, 4 x 12 heads, D=64 58 | 62; dropout,
+// 1047 x 4791, 2 x 8 heads, D=96 205 | 211.
+constexpr float kWeightBits = 14.f, kWeightUnit = 1.f / 16384;
+struct DsUnit {
+  float most;  // the power of two that 2^15 stands for
+  RA_DEV void init() { most = 0x1p-80f; }
+  RA_DEV float scale() const { return __uint_as_float(((127u + 15 + 127) << 23) - __float_as_uint(most)); }
+  RA_DEV float unit() const { return most * 0x1p-15f; }
+  // The unit that holds x > most too; what the sums have to be multiplied with.  (An infinity stays one.)
+  RA_DEV float fit(float x) {
+    const float old = most;
+    most = __uint_as_float(min(__float_as_uint(x) & 0x7f800000u, (127u + 95) << 23) + (5u << 23));
+    return old / most;
+  }
+};
+
 // args_at: where p lies in the kernel's arguments
 template <int DL, int MODE>
 RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, DqLds<DL, MODE>& lds, int args_at) {
@@ -1356,6 +1376,8 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+  DsUnit ds_unit;  // (of fp16 operands)
+  ds_unit.init();
   const FragOffsets<D> fo(lane);
   const bool wave_on = qw < a.Lq;
   const bool alibi_on = GENERAL && (flags & RA_BIAS_ALIBI);
@@ -1518,8 +1540,8 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
           }
         }
       }
+      if constexpr (REL || HALF) S *= P;
       if constexpr (REL) {
-        S *= P;
         if (bias_grad_on) {
           if (side != 0) {
             float t = 0.f;
@@ -1532,13 +1554,27 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
           }
         }
       }
+      float ds_scale = 1.f;
+      if constexpr (HALF) {
+        float mx = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(S[r]));
+        if (__any(mx > ds_unit.most)) {
+          const float m = half_max(mx);  // (both halves hold the query)
+          float corr = 1.f;
+          if (m > ds_unit.most) corr = ds_unit.fit(m);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] *= corr;
+        }
+        ds_scale = ds_unit.scale();
+      }
       // dS in two groups of eight keys per lane: the second one is worked on while the matrix unit
       // multiplies with the first
       X8 dsf[2];
       auto grad = [&](int ks, int e) {  // elements e, e + 1 of group ks
         X2 pr;
-        pr[0] = (T)(REL ? S[8 * ks + e] : S[8 * ks + e] * P[8 * ks + e]);
-        pr[1] = (T)(REL ? S[8 * ks + e + 1] : S[8 * ks + e + 1] * P[8 * ks + e + 1]);
+        pr[0] = (T)(HALF ? S[8 * ks + e] * ds_scale : REL ? S[8 * ks + e] : S[8 * ks + e] * P[8 * ks + e]);
+        pr[1] = (T)(HALF ? S[8 * ks + e + 1] * ds_scale : REL ? S[8 * ks + e + 1] : S[8 * ks + e + 1] * P[8 * ks + e + 1]);
         unsigned pw = __builtin_bit_cast(unsigned, pr);
         asm volatile("" : "+v"(pw));
         pr = __builtin_bit_cast(X2, pw);
@@ -1608,8 +1644,9 @@ RA_DEV void dq_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid, D
   }
   const auto* e = kernel_args<PairBwdArgs>(args_at);
   auto mul = [&] {
-    if constexpr (DROP) return e->a.sm_scale * terms.inv_keep;
-    else return e->a.sm_scale;
+    const float unit = HALF ? e->a.sm_scale * ds_unit.unit() : e->a.sm_scale;
+    if constexpr (DROP) return unit * terms.inv_keep;
+    else return unit;
   };
   if (e->part_n != nullptr && split == 0 && tid == 0) e->part_n[hh * nqt + qt] = n_piece;
   if (!q_valid) return;
@@ -1856,6 +1893,8 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+  DsUnit ds_unit;  // (of fp16 operands)
+  ds_unit.init();
   const FragOffsets<D> fo(lane);
   const bool wave_on = kw < a.Lk;
   const bool alibi_on = GENERAL && (flags & RA_BIAS_ALIBI);
@@ -1991,6 +2030,7 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
       apply_terms<false, DENSE, GENERAL>(S, tests, tb, (q_off + qt0 + 4 * g) - (kv_off + ki), k_seg, k_pre,
                                          &s_seg[GENERAL ? BUF : 0][4 * g], &s_pre[GENERAL ? BUF : 0][4 * g]);
     }
+    if constexpr (HALF) rel += kWeightBits;
     // dP with exp2(S) in its shadow
     X8 pf[2], dsf[2];
     f32x16 P;
@@ -2028,8 +2068,8 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
 #pragma unroll
         for (int e = 8 * op / KS; e < 8 * (op + 1) / KS; ++e) {
           const int r = 2 * e;
-          float x0 = fast_exp2(REL ? fmaf(S[r], a.scale_res, rel) : S[r] * a.scale_res);
-          float x1 = fast_exp2(REL ? fmaf(S[r + 1], a.scale_res, rel) : S[r + 1] * a.scale_res);
+          float x0 = fast_exp2(REL || HALF ? fmaf(S[r], a.scale_res, rel) : S[r] * a.scale_res);
+          float x1 = fast_exp2(REL || HALF ? fmaf(S[r + 1], a.scale_res, rel) : S[r + 1] * a.scale_res);
           X2 pr;
           pr[0] = (T)x0;
           pr[1] = (T)x1;
@@ -2075,6 +2115,17 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
     {
       constexpr int NOP = 4 * DB;  // the dV products, then the dK products
       X8 fr[NOP];
+      float mx = 0.f, ds_scale = 1.f;
+      auto round_ds = [&](int r, float x0, float x1) {
+        X2 pr;
+        pr[0] = (T)x0;
+        pr[1] = (T)x1;
+        unsigned pw = __builtin_bit_cast(unsigned, pr);
+        asm volatile("" : "+v"(pw));
+        pr = __builtin_bit_cast(X2, pw);
+        dsf[r >> 3][r & 7] = pr[0];
+        dsf[r >> 3][(r & 7) + 1] = pr[1];
+      };
       auto t_op = [&](int op) { return tr_frag(op < 2 * DB ? s_do[BUF] : s_q[BUF], op % (2 * DB)); };
 #pragma unroll
       for (int op = 0; op < PF; ++op) fr[op] = t_op(op);
@@ -2088,17 +2139,38 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
 #pragma unroll
           for (int e = 8 * op / (2 * DB); e < 8 * (op + 1) / (2 * DB); ++e) {
             const int r = 2 * e;
-            X2 pr;
-            pr[0] = (T)(S[r] * P[r]);
-            pr[1] = (T)(S[r + 1] * P[r + 1]);
-            unsigned pw = __builtin_bit_cast(unsigned, pr);
-            asm volatile("" : "+v"(pw));
-            pr = __builtin_bit_cast(X2, pw);
-            dsf[r >> 3][r & 7] = pr[0];
-            dsf[r >> 3][(r & 7) + 1] = pr[1];
+            if constexpr (HALF) {
+              P[r] *= S[r];
+              P[r + 1] *= S[r + 1];
+              mx = fmaxf(mx, fmaxf(fabsf(P[r]), fabsf(P[r + 1])));
+              asm volatile("" : "+v"(mx));
+            } else {
+              round_ds(r, S[r] * P[r], S[r + 1] * P[r + 1]);
+            }
           }
         } else {
+          if constexpr (HALF) {
+            if (op == 2 * DB) {
+              if (__any(mx > ds_unit.most)) {
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+                const float corr = ds_unit.fit(mx);
+                ds_unit.most = __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(ds_unit.most)));
+#pragma unroll
+                for (int x = 0; x < DB; ++x) dk[x] *= corr;
+              }
+              ds_scale = ds_unit.scale();
+#pragma unroll
+              for (int r = 0; r < 8; r += 2) round_ds(r, P[r] * ds_scale, P[r + 1] * ds_scale);
+            }
+          }
           dk[db] = mma(dsf[ks], fr[op], dk[db]);
+          if constexpr (HALF) {
+            if (ks == 0) {
+#pragma unroll
+              for (int e = 4 * db / DB; e < 4 * (db + 1) / DB; ++e) round_ds(8 + 2 * e, P[8 + 2 * e] * ds_scale, P[9 + 2 * e] * ds_scale);
+            }
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -2124,12 +2196,15 @@ RA_DEV void dkdv_pair(const PairBwdArgs& p, const TermsOf<MODE>& terms, int bid,
 
   const auto* e = kernel_args<PairBwdArgs>(args_at);
   auto dk_mul = [&] {
-    if constexpr (DROP) return e->a.sm_scale * terms.inv_keep;
-    else return e->a.sm_scale;
+    const float unit = HALF ? e->a.sm_scale * (ds_unit.unit() * kWeightUnit) : e->a.sm_scale;
+    if constexpr (DROP) return unit * terms.inv_keep;
+    else return unit;
   };
-  if constexpr (DROP) {
+  if constexpr (DROP || HALF) {
+    float unit = HALF ? kWeightUnit : 1.f;
+    if constexpr (DROP) unit *= terms.inv_keep;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) dv[db] *= terms.inv_keep;
+    for (int db = 0; db < DB; ++db) dv[db] *= unit;
   }
   if (e->part_n != nullptr && split == 0 && tid == 0) e->part_n[hh * nkt + kt] = n_piece;
   // lane l32 holds column 32 db + l32 of rows kw + 4 g + 8 (r / 4) + r % 4
