@@ -722,6 +722,9 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     if constexpr (REL) write_bias(a.t, ends, s_bias, buf, (kv_off + j * kPairKeys) - (q_off + q0 + kPairRows - 1));
   };
 
+  // In fp16 a weight is off by up to 2^-25 of the reference's: 2^17 keys of 2^-26 beside one of 1 are lost, 2e-3 of the row.  So the largest weight is 2^6
+  // (and up to 2^14 before the reference moves) there.
+  constexpr float kLead = HALF ? 6.f : 0.f;
   float m_run = RA_NEG_INF;  // exponent reference (log2 domain), moves lazily
   float m_true = RA_NEG_INF;
   float l_run = 0.f;  // row sum of the probabilities ...
@@ -893,8 +896,8 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
     if constexpr (REL) mx = half_max(fmaxf(fmaf(mx0, a.scale2, rel[0]), fmaf(mx1 + beyond, a.scale2, rel[1]))) + far;
     else mx = GENERAL ? fmaf(half_max(fmaxf(mx0, mx1 + beyond)), a.scale2, far) : half_max(fmaxf(mx0, mx1)) * a.scale2;
     m_true = fmaxf(m_true, mx);
-    if (__any(mx > m_run + 8.0f)) {
-      const float m_new = fmaxf(m_run, mx);
+    if (__any(mx > m_run + (8.0f + kLead))) {
+      const float m_new = fmaxf(m_run, mx - kLead);
       const float corr = fast_exp2(m_run - ((m_new == RA_NEG_INF) ? 0.f : m_new));
       m_run = m_new;
       l_run *= corr;

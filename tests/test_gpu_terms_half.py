@@ -1,7 +1,11 @@
 """fp16 calls with a relative bias or dropout where dS or the weights lie outside fp16's range, and the gradients inside it."""
+import math
+
 import pytest
 import torch
 
+import ring_attention as ra
+from oracle import terms_oracle as T
 from test_gpu_terms import EPS, Case
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +108,33 @@ def test_no_output_gradient_and_an_infinite_one(device, form):
     assert not torch.isfinite(dq[0, 77]).any()
     others = torch.arange(150, device=device) != 77
     _near("dq", dq[:, others], w.dq[:, others])
+
+
+@pytest.mark.parametrize("sink", [0, 70000, 131071])
+@pytest.mark.parametrize("relative,p", [(True, 0.0), (False, 0.2), (True, 0.2)])
+def test_many_small_weights_beside_a_large_one(device, sink, relative, p):
+    """131072 keys of 2^-26 of one key's weight are 2e-3 of a row, of so many rows that each stays with one workgroup.  A weight is off by 2^-31 of the largest
+    at most (half of 2^-24, the largest being 2^6 or more), divided by what dropout leaves."""
+    n, H, Sq = 131072, 8, 16384
+    q, k, v = (torch.zeros(1, S, H, 64, device=device, dtype=torch.float16) for S in (Sq, n, n))
+    q[..., 0] = 1
+    k[:, sink, :, 0] = 18.015625
+    v[:] = 1
+    v[:, sink] = 0
+    fn = ra.relative_bias(torch.zeros(32, H, device=device)) if relative else None
+    out, lse = ra.ring_attention_with_lse(q, k, v, 1, fn, sm_scale=1.0, dropout=ra.Dropout(p, 5) if p else None)
+    small = math.exp(-18.015625)
+    total = 1 + (n - 1) * small
+    # (a logsumexp of 18: steps of 2^-19, and of the sums and exponentials some 2^-18)
+    assert ((lse.double() - (18.015625 + math.log(total))).abs() <= 2.0 ** -16).all()
+    i, j = torch.tensor([0, 77, 9000, Sq - 1], device=device)[:, None], torch.arange(n, device=device)[None]
+    zero = torch.zeros_like(i * j)
+    for h in (0, H - 1):
+        kept = torch.ones_like(zero)
+        if p:
+            word = torch.stack(T.philox((zero + j // 2, zero + i // 4, zero + h, zero), (5, 0), 7)).gather(0, (zero + i % 4)[None])[0]
+            kept = ((word >> 16 * (zero + j % 2)) & 0xFFFF) >= round(p * 65536)
+        kept[:, sink] = 0
+        want = kept.sum(1).double() * small / total / (1 - round(p * 65536) / 65536)
+        got = out[0, i[:, 0], h].double()
+        assert ((got - want[:, None]).abs() <= HALF * want[:, None] + 2.0 ** -25 + n * 2.0 ** -31 / (1 - p)).all(), (got[:, 0], want)
