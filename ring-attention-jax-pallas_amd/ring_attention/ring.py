@@ -449,8 +449,8 @@ class _RingPlan:
                     # are materialised per ring step from the position arrays and streamed as a
                     # dense block, like a callable bias_fn.
                     def full(t, S):
-                        if t is None:
-                            t = torch.arange(S, device=dev)[None].expand(self.B, S)
+                        if t is None or isinstance(t, int):
+                            t = (torch.arange(S, device=dev) + (t or 0))[None].expand(self.B, S)
                         return t.to(device=dev, dtype=torch.int64)
                     self.callable = _positional_bias_callable(fn)
                     self.fn = None
