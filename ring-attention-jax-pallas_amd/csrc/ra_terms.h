@@ -151,8 +151,8 @@ RA_DEV void load_seed(const TermArgs& t, unsigned& k0, unsigned& k1) {
 // ------------------------------------------------------------------------------------------------
 // Buckets in the order of d: the far past first, the far future last (one-sided: bucket 0 last).
 RA_DEV int ordered_bucket(const int* start, int side, bool two_sided, int d) {
-  const int n = two_sided ? abs(d) : max(-d, 0);
-  int b = 0;  // the last bucket that starts at n or below (start[0] is 0; what lies behind `side` starts nowhere)
+  const int n = two_sided ? abs(d) : -d;
+  int b = 0;  // the last bucket that starts at n or below (start[0] is 0; what lies behind `side` starts nowhere), and 0 ahead of a one-sided bias
 #pragma unroll
   for (int step = kMaxSide / 2; step > 0; step >>= 1) b += start[b + step] <= n ? step : 0;
   return d > 0 && two_sided ? side + b : side - 1 - b;
@@ -201,7 +201,7 @@ RA_DEV BiasEnds load_bias(const TermArgs& t, int h, float unit, BiasLds<N, GRAD>
   if (tid < kMaxSide) lds.start[tid] = tid < t.side ? t.start[tid] : 0x7fffffff;
   BiasEnds e;
   e.far = t.start[t.side - 1];
-  e.future = t.two_sided ? e.far : 0;
+  e.future = t.two_sided ? e.far : t.start[1] > 0 ? 0 : 1;  // (distance 0 itself may lie in a later bucket than the keys ahead)
   auto uniform = [](float x) {  // (the product, not its factor: a scalar register has no product of its own, and the backward no vector register for it)
     asm volatile("" : "+v"(x));
     return __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(x)));

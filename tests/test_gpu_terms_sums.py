@@ -1,11 +1,12 @@
 """Gradients of a relative bias's table bucket by bucket: what a bucket gets is the sum over its own pairs, whatever the others hold."""
-import math
+import struct
 
 import pytest
 import torch
 
 import ring_attention as ra
 from oracle import terms_oracle as T
+from ring_attention import _lib, ring as rr
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,28 @@ def test_buckets_of_little_weight_are_their_own_sums(device, kw):
     grad, (want, off) = c.gradient().double(), c.want()
     for u in small:
         assert ((grad[u] - want[u]).abs() <= off[u] + 2.0 ** -24 * want[u].abs()).all(), (u, grad[u], want[u], off[u])
+
+
+@pytest.mark.parametrize("two", [False, True])
+@pytest.mark.parametrize("starts", [(0, 0, 0, 3), (0, 0, 7, 40), (0, 1, 1, 1)])
+def test_buckets_that_start_where_the_next_one_does(device, starts, two):
+    """Starts as the C interface takes them: a bucket that begins with the next one is empty, but for bucket 0 of a one-sided bias, which holds the keys ahead."""
+    B, Sq, Sk, H, q_off = 1, 150, 200, 2, 1
+    g = torch.Generator().manual_seed(5)
+    q, k, v, do = (torch.randn(B, S, H, 64, generator=g).to(device, torch.bfloat16) for S in (Sq, Sk, Sk, Sq))
+    table = _table(8 if two else 4, H).to(device).requires_grad_(True)
+    at = torch.arange(Sk, device=device)[None] - q_off - torch.arange(Sq, device=device)[:, None]
+    n = at.abs() if two else -at
+    bucket = (n[..., None] >= torch.tensor(starts, device=device)).sum(-1).clamp(min=1) - 1
+    bucket = bucket + (4 * (at > 0) if two else 0)
+    w = T.Attention(q, k, v, do=do, bias=table.detach().double()[bucket].permute(2, 0, 1))
+    plan = rr._RingPlan(q, k, 1, ra.relative_bias(table, bidirectional=two), {"q_positions": q_off}, None).single()
+    out, _ = _lib.host().attend_terms(q, k, v, plan.native(q), 0.125, torch.bfloat16, torch.bfloat16, q_off, 0, table, two,
+                                      struct.pack("4i", *starts), 0, None)
+    assert ((out.detach().double() - w.out).abs() <= w.out_off).all()
+    grad, = torch.autograd.grad(out, table, do)
+    want, off = w.table_gradient(bucket, table.shape[0], 2.0 ** -23)
+    assert ((grad.double() - want).abs() <= off).all()
+    empty = torch.ones(table.shape[0], dtype=torch.bool, device=device)
+    empty[bucket.unique()] = False
+    assert (grad[empty] == 0).all()
