@@ -124,8 +124,8 @@ class Attention:
         self.dv, self.dv_off = grad(W.transpose(2, 3) @ do, (e + n32q) * (W.transpose(2, 3) @ do.abs()))
         self.dS, self.dS_off32 = dS, off
 
-    def table_gradient(self, bucket, num_buckets, eps):
-        """[num_buckets, h] sums of dS, and their bounds: a bucket may be taken as minus the others' sum."""
+    def table_gradient(self, bucket, num_buckets, eps, own=False):
+        """[num_buckets, h] sums of dS, and their bounds: of all pairs together, or of a bucket's own."""
         n = self.dS.shape[2] * self.dS.shape[3] * self.dS.shape[0]
         e_sum = 2.0 ** -24 * (math.log2(n) + 64)  # sums of sums, at most so deep each
         got, off = [], []
@@ -134,4 +134,4 @@ class Attention:
             got.append(self.dS[:, :, at].sum((0, 2)))
             off.append((self.dS_off32 + 64 * e_sum * self.dS.abs())[:, :, at].sum((0, 2)))
         got, off = torch.stack(got), torch.stack(off)
-        return got, off.sum(0, keepdim=True) + eps / 2 * got.abs() + 1e-30
+        return got, (off if own else off.sum(0, keepdim=True)) + eps / 2 * got.abs() + (1e-36 if own else 1e-30)

@@ -7,6 +7,7 @@ import torch
 import ring_attention as ra
 from oracle import terms_oracle as T
 from ring_attention import _lib, ring as rr
+from test_gpu_terms import MASKS, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -54,14 +55,7 @@ class Call:
         """[buckets, H] in 64 bits, and how far off a sum over a bucket's own pairs in 32 bits may be."""
         bias = self.table.double()[self.bucket].permute(2, 0, 1)
         w = T.Attention(self.q, self.k, self.v, do=self.do, live=self.live, bias=bias, keep=self.keep, threshold=self.threshold, eps=self.eps)
-        got, off = [], []
-        for u in range(self.buckets):
-            at = self.bucket == u
-            got.append(w.dS[:, :, at].sum((0, 2)))
-            # a pair's part in 32 bits; every sum on the way (of 16 of a lane, its blocks, a wave, workgroups, diagonals: fewer than 256 one
-            # after the other) is of this bucket's pairs, half a step of 32 bits each
-            off.append((w.dS_off32 + 256 * 2.0 ** -24 * w.dS.abs())[:, :, at].sum((0, 2)))
-        return torch.stack(got), torch.stack(off) + 1e-36
+        return w.table_gradient(self.bucket, self.buckets, 2.0 ** -23, own=True)
 
 
 def _documents(B, S, n):
@@ -98,7 +92,42 @@ def test_buckets_of_little_weight_are_their_own_sums(device, kw):
     c = Call(device, table, **kw)
     grad, (want, off) = c.gradient().double(), c.want()
     for u in small:
-        assert ((grad[u] - want[u]).abs() <= off[u] + 2.0 ** -24 * want[u].abs()).all(), (u, grad[u], want[u], off[u])
+        assert ((grad[u] - want[u]).abs() <= off[u]).all(), (u, grad[u], want[u], off[u])
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("kw", [dict(relative="both", Sq=333, distance=100), dict(relative="one", Sq=290, p=0.25, D=128, dtype=torch.float16),
+                                dict(relative="both", Sq=200, Sk=450, buckets=128, distance=300)])
+def test_every_bucket_by_its_own_pairs(device, mask, kw):
+    """Many of a call's buckets hold a few pairs beside one that holds most."""
+    c = Case(device, B=2, H=2, mask=mask, table_dtype=torch.float32, **kw)
+    want, off = c.want().table_gradient(c.bucket, c.buckets, 2.0 ** -23, own=True)
+    assert ((c.grads()[2][3].double() - want).abs() <= off).all()
+
+
+def test_two_layers_with_a_table_each_and_with_one(device):
+    """The table's gradient of either of two layers, and of a table that both take (whose gradient goes through the first layer's output too)."""
+    g = torch.Generator().manual_seed(6)
+    B, S, H = 2, 256, 4
+    table = torch.randn(32, H, generator=g).to(device)
+    x, do = (torch.randn(B, S, H, 64, generator=g).to(device, torch.bfloat16) for _ in range(2))
+    bucket = T.bucket_of(torch.arange(S, device=device)[None] - torch.arange(S, device=device)[:, None], 32, 128, False)
+    bias, live = table.double()[bucket].permute(2, 0, 1), T.scores_mask(S, S, causal=True, device=device)
+
+    def layer(x, table):
+        return ra.ring_attention(x, x, x, 1, ra.causal_bias() + ra.relative_bias(table, bidirectional=False))
+
+    leaves = [table.clone().requires_grad_(True) for _ in range(2)]
+    y = layer(x, leaves[0])
+    z = layer(y, leaves[1])
+    gy, g1, g2 = torch.autograd.grad(z, (y, *leaves), do)
+    for got, at, grad in ((g2, y.detach(), do), (g1, x, gy)):
+        w = T.Attention(at, at, at, do=grad, live=live, bias=bias)
+        want, off = w.table_gradient(bucket, 32, 2.0 ** -23, own=True)
+        assert ((got.double() - want).abs() <= off).all()
+    one = table.clone().requires_grad_(True)
+    both, = torch.autograd.grad(layer(layer(x, one), one), one, do)
+    assert ((both - (g1 + g2)).abs() <= 2.0 ** -23 * (g1.abs() + g2.abs())).all()
 
 
 @pytest.mark.parametrize("two", [False, True])
@@ -119,7 +148,7 @@ def test_buckets_that_start_where_the_next_one_does(device, starts, two):
                                       struct.pack("4i", *starts), 0, None)
     assert ((out.detach().double() - w.out).abs() <= w.out_off).all()
     grad, = torch.autograd.grad(out, table, do)
-    want, off = w.table_gradient(bucket, table.shape[0], 2.0 ** -23)
+    want, off = w.table_gradient(bucket, table.shape[0], 2.0 ** -23, own=True)
     assert ((grad.double() - want).abs() <= off).all()
     empty = torch.ones(table.shape[0], dtype=torch.bool, device=device)
     empty[bucket.unique()] = False
