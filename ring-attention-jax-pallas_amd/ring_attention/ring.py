@@ -386,7 +386,7 @@ class _RingPlan:
             raise ValueError(f"sequence lengths ({Sq}, {Sk}) must be divisible by the ring size {n}")
         self.Lq, self.Lk = Sq // n, Sk // n
         self.fn = fn
-        self.callable = None
+        self.callable = self.positional = None  # positional: the terms that a callable of explicit positions stands for
         self.device = dev = q.device
         q_kwargs = dict(q_kwargs or {})
         kv_kwargs = dict(kv_kwargs or {})
@@ -402,8 +402,7 @@ class _RingPlan:
                     raise ValueError(f"bias kwarg {name!r} must be a tensor [b, {S}, ...]")
             self.callable = fn
             self.fn = None
-            self.q_kw = {a: t.to(dev) for a, t in q_kwargs.items()}
-            self.kv_kw = {a: t.to(dev) for a, t in kv_kwargs.items()}
+            self._lay(q_kwargs, kv_kwargs)
             return
         known_q = {"q_segment_ids", "q_positions", "q_prefix_mask"}
         known_kv = {"kv_segment_ids", "kv_positions", "kv_prefix_mask"}
@@ -414,26 +413,13 @@ class _RingPlan:
         if fn is None and any(v is not None for v in list(q_kwargs.values()) + list(kv_kwargs.values())):
             raise ValueError("bias kwargs were given without a bias_fn")
 
-        def ids(t, S, name):
-            if t is None:
-                return None
-            if tuple(t.shape) != (self.B, S):
-                raise ValueError(f"{name} must have shape {(self.B, S)}, got {tuple(t.shape)}")
-            return t.to(device=dev, dtype=torch.int32).contiguous()
-
-        self.q_seg = self.kv_seg = self.q_pre = self.kv_pre = None
+        self._lay(q_kwargs, kv_kwargs)
         if fn is not None:
             fn.validate()
-            if fn.segments:
-                self.q_seg = ids(q_kwargs.get("q_segment_ids"), Sq, "q_segment_ids")
-                self.kv_seg = ids(kv_kwargs.get("kv_segment_ids"), Sk, "kv_segment_ids")
-                if self.q_seg is None or self.kv_seg is None:
-                    raise ValueError("segment bias needs q_segment_ids and kv_segment_ids")
-            if fn.prefix:
-                self.q_pre = ids(q_kwargs.get("q_prefix_mask"), Sq, "q_prefix_mask")
-                self.kv_pre = ids(kv_kwargs.get("kv_prefix_mask"), Sk, "kv_prefix_mask")
-                if self.q_pre is None or self.kv_pre is None:
-                    raise ValueError("prefix bias needs q_prefix_mask and kv_prefix_mask")
+            if fn.segments and (self.q_seg is None or self.kv_seg is None):
+                raise ValueError("segment bias needs q_segment_ids and kv_segment_ids")
+            if fn.prefix and (self.q_pre is None or self.kv_pre is None):
+                raise ValueError("prefix bias needs q_prefix_mask and kv_prefix_mask")
             if fn.alibi_slopes is not None:
                 if fn.alibi_slopes.numel() != self.H:
                     raise ValueError("alibi slopes must have one entry per head")
@@ -448,22 +434,69 @@ class _RingPlan:
                     # by element, ring.py:396): the kernels take one offset per shard, so the terms
                     # are materialised per ring step from the position arrays and streamed as a
                     # dense block, like a callable bias_fn.
-                    def full(t, S):
-                        if t is None or isinstance(t, int):
-                            t = (torch.arange(S, device=dev) + (t or 0))[None].expand(self.B, S)
-                        return t.to(device=dev, dtype=torch.int64)
-                    self.callable = _positional_bias_callable(fn)
+                    self.callable, self.positional = _positional_bias_callable(fn), fn
+                    self._lay(q_kwargs, kv_kwargs)
                     self.fn = None
-                    self.q_kw = {"q_positions": full(qp, Sq)}
-                    self.kv_kw = {"kv_positions": full(kp, Sk)}
-                    for kw, name, t in ((self.q_kw, "q_segment_ids", self.q_seg), (self.kv_kw, "kv_segment_ids", self.kv_seg),
-                                        (self.q_kw, "q_prefix_mask", self.q_pre), (self.kv_kw, "kv_prefix_mask", self.kv_pre)):
-                        if t is not None:
-                            kw[name] = t
                     return
                 self.q_off, self.kv_off = q_off, kv_off
             if fn.relative is not None:
                 self.fn = replace(self.fn, relative=None)  # (a call brings its own table: ``attend_terms``)
+
+    def _lay(self, q_kwargs, kv_kwargs, before=None) -> None:
+        """The bias arrays as the kernels, or a callable, take them.  ``made``: some of them are copies of device arrays, that hold what those held when they
+        were made.  ``before``: a plan of the same arrays, whose copies of host arrays are taken over."""
+        Sq, Sk, dev = self.n * self.Lq, self.n * self.Lk, self.device
+        self.made = False
+
+        def laid(t, make, kept):
+            if before is not None and t.device != dev:
+                return kept()
+            x = make(t)
+            self.made = self.made or (t.device == dev and x.data_ptr() != t.data_ptr())
+            return x
+
+        if self.fn is None and self.callable is not None:
+            self.q_kw = {a: laid(t, lambda t: t.to(dev), lambda: before.q_kw[a]) for a, t in q_kwargs.items()}
+            self.kv_kw = {a: laid(t, lambda t: t.to(dev), lambda: before.kv_kw[a]) for a, t in kv_kwargs.items()}
+            return
+
+        def ids(kw, S, name, attr):
+            t = kw.get(name)
+            if t is None:
+                return None
+            if tuple(t.shape) != (self.B, S):
+                raise ValueError(f"{name} must have shape {(self.B, S)}, got {tuple(t.shape)}")
+            return laid(t, lambda t: t.to(device=dev, dtype=torch.int32).contiguous(), lambda: getattr(before, attr))
+
+        self.q_seg = self.kv_seg = self.q_pre = self.kv_pre = None
+        if self.fn is not None and self.fn.segments:
+            self.q_seg, self.kv_seg = ids(q_kwargs, Sq, "q_segment_ids", "q_seg"), ids(kv_kwargs, Sk, "kv_segment_ids", "kv_seg")
+        if self.fn is not None and self.fn.prefix:
+            self.q_pre, self.kv_pre = ids(q_kwargs, Sq, "q_prefix_mask", "q_pre"), ids(kv_kwargs, Sk, "kv_prefix_mask", "kv_pre")
+        if self.callable is None:
+            return
+
+        def full(t, S, kept):
+            if t is None or isinstance(t, int):
+                t = (torch.arange(S) + (t or 0))[None].expand(self.B, S)
+            return laid(t, lambda t: t.to(device=dev, dtype=torch.int64), kept)
+
+        self.q_kw = {"q_positions": full(q_kwargs.get("q_positions"), Sq, lambda: before.q_kw["q_positions"])}
+        self.kv_kw = {"kv_positions": full(kv_kwargs.get("kv_positions"), Sk, lambda: before.kv_kw["kv_positions"])}
+        for kw, name, t in ((self.q_kw, "q_segment_ids", self.q_seg), (self.kv_kw, "kv_segment_ids", self.kv_seg),
+                            (self.q_kw, "q_prefix_mask", self.q_pre), (self.kv_kw, "kv_prefix_mask", self.kv_pre)):
+            if t is not None:
+                kw[name] = t
+
+    def laid_again(self, q_kwargs, kv_kwargs) -> "_RingPlan":
+        """This plan with its copies of device arrays made anew, by work that the current capture records."""
+        plan = object.__new__(_RingPlan)
+        plan.__dict__.update({a: x for a, x in self.__dict__.items() if not a.startswith("_")})
+        if plan.positional is not None:
+            plan.fn = plan.positional
+        plan._lay(dict(q_kwargs or {}), dict(kv_kwargs or {}), self)
+        plan.fn = self.fn
+        return plan
 
     def _offsets(self, pos, S, L, name):
         """One position offset per shard if the positions are consecutive inside every shard and
@@ -688,13 +721,19 @@ def clear_plan_cache() -> None:
     _PLAN_CACHE.clear()
 
 
+def _capturing(t) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def _plan_for(q, k, n, bias_fn, q_kwargs, kv_kwargs) -> "_RingPlan":
     """The ``_RingPlan`` of a call, from a small cache: a plan (shard offsets read back from the
     position arrays, id arrays converted to int32, the parameter blocks of the whole-ring
     launches) depends on shapes, the ring size and the bias arrays only, so a caller who repeats a
     call - a training loop - pays for it once.  A bias array is identified by the tensor object and
     its version counter; the cache entry keeps the object alive, so its identity cannot be taken
-    over by another tensor, and an in-place change gives a new version and a new plan."""
+    over by another tensor, and an in-place change gives a new version and a new plan.  A call that is captured into a graph keeps nothing that was
+    made of the arrays (other dtypes, gathered rows): the graph makes it again in every replay, from what they hold then.  (What a replay itself writes
+    into an array changes no version: such an array has to be one that the kernels read in place, int32 and contiguous.)"""
     def ident(t):
         return (id(t), t._version) if isinstance(t, torch.Tensor) else ("v", t)
 
@@ -709,8 +748,12 @@ def _plan_for(q, k, n, bias_fn, q_kwargs, kv_kwargs) -> "_RingPlan":
     hit = _PLAN_CACHE.get(key)
     if hit is not None:
         _PLAN_CACHE.move_to_end(key)
+        if hit[0].made and _capturing(q):
+            return hit[0].laid_again(q_kwargs, kv_kwargs)
         return hit[0]
     plan = _RingPlan(q, k, n, bias_fn, q_kwargs, kv_kwargs)
+    if plan.made and _capturing(q):
+        return plan
     _PLAN_CACHE[key] = (plan, bias_fn, dict(q_kwargs or {}), dict(kv_kwargs or {}))
     while len(_PLAN_CACHE) > _PLAN_CACHE_SIZE:
         _PLAN_CACHE.popitem(last=False)
