@@ -706,10 +706,10 @@ bool long_stretches(const ra_bias& bias, int D, int64_t wgs, int64_t total, int6
 // cost more in partial results (528 bytes per row and share) than they gain.
 constexpr int kMinChunk = 6, kMaxSplit = 64;
 // With a relative bias or dropout (`always`), where a tile takes longer and nothing else is measured against: shares down to a third of that if the rows
-// are few, or one tile of them.  Kernels of a call, us, shares of six | of two (twice that for dK and dV): a token behind 1000 keys, H=8, D=64, bias 12.8 + 4.0 | 8.8 + 3.5,
-// 5000, H=16, D=128 16.8 + 5.9 | 15.8 + 4.4, 128 of 3000, H=8, D=128 19.4 + 4.1 | 17.7 + 5.7; training, dropout, causal 512, H=4, D=64 52.5 | 36.1, both 78.8 |
-// 63.5 (H=8, D=128), 1024, H=4, D=64 72.7 | 60.5, unmasked 512, H=4 58.3 | 48.2; not even rows on 64 workgroups, unmasked 1000, H=8, D=128 78.0 | 82.2.
-// (Those with a bias: before its forward's second output product, a tile of which takes up to a third longer.)
+// are few, or one tile of them.  All kernels of a call but the statistics, us, shares of six | of two (twice that for dK and dV): a token behind 1000 keys,
+// H=8, D=64, bias 17.8 | 13.1, 5000, H=16, D=128 24.9 | 22.1, 128 of 3000, H=8, D=128 25.4 | 24.9; training, causal 512, H=4, D=64, dropout 47.6 | 31.6, H=8, D=128,
+// both 74.9 | 57.8, 1024, H=4, D=64 dropout 49.4 | 39.6, both 67.8 | 55.2, unmasked 512, H=4, D=64 dropout 37.6 | 31.2, bias 46.1 | 39.3.  Even rows on 33 to 64
+// workgroups gain or lose: both, 2 x 8 heads of 450, D=64 69 | 60, 8 of 1000, D=128 97 | 94, 16 of 512, D=128 81 | 90 (dropout 59 | 64, bias 68 | 77).
 int min_chunk(bool always, bool even, int64_t rows, int64_t wgs, int most, int tiles) {
   return always && (rows == 1 || wgs <= (even ? 32 : 64)) && most > tiles ? tiles / 3 : tiles;
 }
@@ -736,8 +736,8 @@ bool one_by_one(const ra_bias& b, int64_t total, int most, int64_t rows) {
 // places as many shares as places, and beyond that long rows of the forward by the count (documents of 3000 in 10000, H=5, D=64, 253
 // | 184; short ones lose: documents of 1500 in 4096, H=12, 107 | 121, and so does the backward: prefix 20000, H=3, 1103 | 1202).
 // uneven_most: workgroups of long rows of different lengths that are shared.  With dropout, whose forward takes 1.25 times as long a tile, as many as there are
-// places: not shared | shared, us, forward, causal: 16 heads of 4096, D=128 155 | 136 + 9, with a relative bias (before its second output product) 172 | 154 + 10, D=64 125 | 109 + 6 (bias alone 141 | 135 + 9;
-// the backward, 296 | 320 + 16).
+// places: not shared | shared, us, forward, causal, 16 heads of 4096: D=128 157 | 143 + 9, with a relative bias 184 | 173 + 9, D=64 124 | 107 + 6, with a bias 146 |
+// 130 + 6 (bias alone D=128 139 | 137 + 9, D=64 99 | 95 + 6; the backward, D=128, dropout 315 | 337 + 17, bias 270 | 290 + 17, D=64, dropout 245 | 234 + 10).
 void plan_split(PairPlan& r, int64_t heads, int64_t rows, int64_t total, int most, int min_chunk, int64_t share, const ra_bias& bias,
                 bool beside, int uneven_most = kPairSlots * 3 / 4) {
   const int64_t wgs = heads * rows;

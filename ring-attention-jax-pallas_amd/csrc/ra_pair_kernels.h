@@ -589,7 +589,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void fwd_pair_kernel(const FwdArgs
   // the weights themselves.  The table's gradient needs it: most of a bucket's sum cancels (over a row, sum of P (dP - delta) = 0), and a delta = out . dO of
   // rounded weights is off by their roundings, which cancel in no bucket: 2e-3 of the gradient of 16 buckets (672 x 672, bf16), as much as the
   // result's own rounding.  Twice the matrix instructions for the output: forward, 16 heads of 2 x 4096, D=64 109 | 142 us, 16 of 4096, D=128, with dropout
-  // 144 | 165.
+  // 144 | 165.  (Calls without gradients too: their output has the bits of one with gradients.)
   constexpr bool FINE = REL;
   using T = std::conditional_t<HALF, _Float16, bf16_t>;
   using X8 = vec_of<T, 8>;

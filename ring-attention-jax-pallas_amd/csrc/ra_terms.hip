@@ -5,7 +5,7 @@ namespace ra {
 
 // The relative bias's gradient from the workgroups' sums: a workgroup per head, a thread per bucket and row in turn, always in the same order.
 // Bound by latency: the sums come from all over the chip.  Eight rows a thread are on their way at once (one after the other: 9.2 us at 2 x 32 tiles, 32
-// buckets, H=16; now 6.1 to 6.7, of which the 0.5 MB would be 0.1 at a large copy's rate).
+// buckets, H=16; now 5.2, of which the 0.5 MB would be 0.1 at a large copy's rate).
 constexpr int kGradThreads = 512, kGradAhead = 8;
 __global__ __launch_bounds__(kGradThreads) void table_grad_kernel(const TermArgs t, const int* part_n, int B, int H, int tiles, int n_split) {
   __shared__ float s_sum[kGradThreads];

@@ -18,7 +18,7 @@ Public names follow the reference (``ring.py:246`` ``ring_attention``, ``ring.py
   [b, h | 1, lq, lk]`` (ring.py:107), whose dense block is materialised per ring step and
   streamed by the kernels.
 * Compute is bf16 on the matrix cores with fp32 carries; other input dtypes are cast on
-  entry and the result is cast back.  Head dims are zero-padded to 64 or 128, on whole sequences
+  entry and the result is cast back (fp16 stays fp16 under a relative bias or dropout).  Head dims are zero-padded to 64 or 128, on whole sequences
   (``_RingPlan._whole``) to the next multiple of 32.
 
 Everything runs through ``libringattn_hip.so``; if it is missing the import of this module
@@ -1084,7 +1084,7 @@ _NO_TABLE = RelativeBias(None)
 
 def _terms_call(q, k, v, n, fn: Optional[BiasFn], q_kwargs, kv_kwargs, sm_scale, out_dtype, final_dtype, drop: int, seed):
     """A call with a relative bias or dropout: one launch over the whole sequence (``attend_terms`` of ``csrc/ra_host.cc``).  The table, the seed and
-    positions that are given as an int are the call's own, so that a plan serves every step of a training or decoding loop."""
+    positions that are given as an int are the call's own, so that one plan serves all calls of the same lengths and id arrays."""
     if torch._C._get_tracing_state() is not None:
         raise RuntimeError("a relative bias and dropout cannot be traced")
     relative = q_off = kv_off = None
@@ -1195,7 +1195,7 @@ def ring_attention(q, k, v, axis_name, bias_fn: Union[BiasFn, Callable, None] = 
             (launch per step) and ``"hip_fused"`` (one launch for all ring passes: the kernels walk
             the shards themselves); anything else raises ``ValueError`` as the reference does
             (ring.py:312).  Every value runs the same kernels on the same bf16 operands.  (A relative bias and dropout: one launch over the
-            whole sequence, whatever the value.)
+            whole sequence, whatever the value, and fp16 operands stay fp16.)
         dropout: a ``Dropout`` of the attention weights; none by default.  Not with a callable ``bias_fn``.
     Returns:
         attention output ``[b, S, h, d]``; differentiable w.r.t. q, k, v and the table of a relative bias.
