@@ -747,7 +747,10 @@ def _plan_for(q, k, n, bias_fn, q_kwargs, kv_kwargs) -> "_RingPlan":
     key = (q.shape, k.shape, q.device, n, fn_key, kw_key)
     hit = _PLAN_CACHE.get(key)
     if hit is not None:
-        _PLAN_CACHE.move_to_end(key)
+        try:
+            _PLAN_CACHE.move_to_end(key)
+        except KeyError:  # another thread's call has put it out meanwhile
+            pass
         if hit[0].made and _capturing(q):
             return hit[0].laid_again(q_kwargs, kv_kwargs)
         return hit[0]

@@ -35,9 +35,9 @@ def _near(name, got, want, dim=None):
 
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("D,mask", [(64, "none"), (128, "causal"), (96, "none")])
-@pytest.mark.parametrize("do", [2.0 ** -10, 2.0 ** -13])
+@pytest.mark.parametrize("do", [2.0 ** -10, 2.0 ** -13, 2.0 ** -17])
 def test_small_output_gradients(device, form, D, mask, do):
-    """Without loss scaling: dO of 1e-3 and 1e-4, so that dS is next to or below fp16's smallest number, and keys or queries that bring the gradient back
+    """Without loss scaling: dO of 1e-3, 1e-4 and 1e-5, so that dS is next to or below fp16's smallest number, and keys or queries that bring the gradient back
     into the range."""
     for q, k, name in ((2.0 ** -6, 64.0, "dq"), (64.0, 2.0 ** -6, "dk")):
         c = _case(device, H=2, Sq=1500, D=D, mask=mask, q=q, k=k, do=do, **form)
