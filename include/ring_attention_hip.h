@@ -402,6 +402,72 @@ int ra_bwd_terms(const ra_rows* before, int32_t n_before, const ra_bwd_step_para
                  void* dk, void* dv, int64_t dkv_stride_b, int64_t dkv_stride_h, int64_t dkv_stride_l, void* d_table,
                  void* workspace, int64_t workspace_bytes, void* stream);
 
+/* A key-value cache in pages, for generation (the reference has no counterpart: its keys and values are whole arrays, ring.py:246-325).
+ * A pool holds n_pages pages of page_size tokens, element [page, token, head, d] at ptr[page * stride_page + token * stride_token +
+ * head * stride_head + d]; row b of a table names the pages of sequence b in order.  page_size is a power of two from 16 to 65536, d a multiple of
+ * 32 up to 128, elements are RA_DTYPE_BF16 or RA_DTYPE_F16.  Numbers on the device are not trusted: lengths are cut to [0, width *
+ * page_size], and pages or slots outside of the pool take no part.  Up to RA_MAX_PAGED_ROWS sequences per call. */
+#define RA_MAX_PAGED_ROWS 4096
+typedef struct ra_pool {
+  void* ptr; /* 16-byte aligned, strides multiples of 8 elements, offsets within a page below 2^31 */
+  int64_t stride_page, stride_token, stride_head;
+} ra_pool;
+typedef struct ra_page_table {
+  int32_t* ptr; /* [B, width] */
+  int64_t stride_b;
+  int32_t width, n_pages, page_size;
+} ra_page_table;
+
+/* Sequences go from lengths[b] to new_lengths[b] tokens.  Pages come from the head of the ring of free ones (free_pages [n_pages], of which
+ * free_state[1] from place free_state[0] on are free, around its end) and are written into the table; pages beyond the new length go
+ * behind its last one; both in the order of the sequences.  Pages given back by a call are given out by later ones.  Results:
+ *  - slots [n_slots]: page * page_size + place of each new token, sequence by sequence; -1 for one without a page and beyond the last
+ *  - starts [B + 1]: where a sequence's tokens begin in slots
+ *  - granted [B]: the new lengths, cut to what there were pages for: the lengths to go on with
+ *  - free_state_out [2]: the ring's new state (none of the results may overlap an operand) */
+int ra_page_slots(const ra_page_table* table, const int32_t* lengths, const int32_t* new_lengths, int32_t B, int32_t* free_pages,
+                  const int32_t* free_state, int64_t* slots, int32_t n_slots, int32_t* starts, int32_t* granted, int32_t* free_state_out,
+                  void* stream);
+
+/* Keys and values of T tokens, [T, H, D] with strides of their own, to their slots (those outside of [0, n_pages * page_size) are left
+ * out; a slot occurs once).  Sources of any RA_DTYPE_* are rounded to the pools' type.  RA_ERR_TOO_LARGE: T * H * D / 8 of 2^31 or more. */
+int ra_write_pages(const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token, int64_t v_stride_head,
+                   int32_t src_dtype, int32_t T, int32_t H, int32_t D, const ra_pool* k_pool, const ra_pool* v_pool, int32_t dtype,
+                   int32_t n_pages, int32_t page_size, const int64_t* slots, void* stream);
+
+/* means[page, head, :] = the mean of the keys that the page holds (sums in 32 bits, rounded once), for the pages whose tokens change between
+ * lengths[b] and new_lengths[b]. */
+int ra_page_means(const ra_pool* k_pool, int32_t dtype, const ra_page_table* table, const int32_t* lengths, const int32_t* new_lengths, int32_t B,
+                  int32_t H, int32_t D, void* means, int64_t means_stride_page, int64_t means_stride_head, void* stream);
+
+/* For each sequence and head of the cache the numbers (within the sequence) of the `count` pages with the largest score, in order:
+ * (sum of the queries of the `group` heads that share it) . (the page's mean key), in 64 bits, ties from the lowest number.  The first `first`
+ * and the last `last` pages are always among them.  A sequence of no more pages than `count` has all of them, and -1 behind.
+ * q: [B, H * group, D].  pages: [B, H, count] contiguous.  workspace: ra_select_pages_workspace() bytes, 16-byte aligned. */
+int64_t ra_select_pages_workspace(const ra_page_table* table, int32_t B, int32_t H);
+int ra_select_pages(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* means, int64_t means_stride_page, int64_t means_stride_head,
+                    int32_t dtype, const ra_page_table* table, const int32_t* lengths, int32_t B, int32_t H, int32_t group, int32_t D, int32_t count,
+                    int32_t first, int32_t last, int32_t* pages, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of one token per sequence, the last of its lengths[b] tokens, whose key and value lie in the pool already:
+ * out[b, h * group + g] = softmax(sm_scale q . k + bias) v over the tokens of sequence b, lse their logsumexp.  A row without tokens is zero, its
+ * logsumexp -inf.  Several tokens of a sequence are several rows with the same pages, each with its own length. */
+typedef struct ra_paged_params {
+  int32_t B, H, group, D;  /* sequences, heads of the cache, query heads that share each, head dim */
+  int32_t dtype, window;   /* window > 0: the last `window` tokens only */
+  float sm_scale;
+  int32_t n_pages_read;    /* with `pages`: [B, H, n_pages_read] contiguous */
+  const void* q;           /* [B, H * group, D] */
+  int64_t q_stride_b, q_stride_h;
+  ra_pool k, v;
+  ra_page_table table;
+  const int32_t* lengths;
+  const int32_t* pages;    /* numbers (within the sequence) of the pages that are read, each at most once, others left out; NULL: all are */
+  const float* slopes;     /* ALiBi, [H * group]: -slope * distance added to the scores; NULL: none */
+} ra_paged_params;
+int64_t ra_paged_attention_workspace(const ra_paged_params* p);
+int ra_paged_attention(const ra_paged_params* p, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Host-only, pure: 1 if every score of the (query shard, key/value shard) pair is masked
  * by the positional terms of `bias` (CAUSAL / WINDOW), so that the whole ring step is an
  * identity on the carry and may be skipped; 0 otherwise.  The reference runs such steps and

@@ -14,14 +14,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(HERE, "ring_attention", "libringattn_hip.so")
-SOURCES = ["ra_fwd.hip", "ra_bwd.hip", "ra_pair.hip", "ra_terms.hip", "ra_terms_f16.hip", "ra_convert.hip", "ra_api.hip"]
+SOURCES = ["ra_fwd.hip", "ra_bwd.hip", "ra_pair.hip", "ra_terms.hip", "ra_terms_f16.hip", "ra_convert.hip", "ra_paged.hip",
+           "ra_paged_api.hip", "ra_api.hip"]
 # the matrix-rate probe that bench.py reports next to the roofline: a library of its own, so that
 # the block-step library exports nothing but the block-step ABI
 PROBE_LIB_PATH = os.path.join(HERE, "ring_attention", "libringattn_probe.so")
 PROBE_SOURCES = ["ra_probe.hip"]
-# the calls on whole sequences from Python: a CPython extension over torch's C++ API
+# the calls on whole sequences and on a paged cache from Python: a CPython extension over torch's C++ API
 HOST_LIB_PATH = os.path.join(HERE, "ring_attention", "_host.so")
-HOST_SOURCE = "ra_host.cc"
+HOST_SOURCES = ["ra_host.cc", "ra_paged_host.cc"]
 # the XLA FFI handlers over the C ABI (what a JAX host binds): built only where jaxlib's headers are
 FFI_LIB_PATH = os.path.join(HERE, "ring_attention", "libringattn_xla_ffi.so")
 FFI_SOURCE = "ra_xla_ffi.cc"
@@ -88,7 +89,7 @@ def build_xla_ffi(verbose: bool = False) -> str | None:
 
 
 def build_host(verbose: bool = False) -> str | None:
-    """ring_attention/_host.so from csrc/ra_host.cc; skipped (None) without a ROCm build of torch, for hosts that bind the C ABI or the
+    """ring_attention/_host.so from HOST_SOURCES; skipped (None) without a ROCm build of torch, for hosts that bind the C ABI or the
     XLA FFI handlers only."""
     import sysconfig
 
@@ -100,16 +101,24 @@ def build_host(verbose: bool = False) -> str | None:
         missing = e
     if missing:
         if verbose:
-            print(f"{HOST_SOURCE} skipped: {missing}")
+            print(f"{HOST_SOURCES[0]} skipped: {missing}")
         return None
     include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include"]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(x for p in include for x in ("-isystem", p)),
-           os.path.join(CSRC, HOST_SOURCE), "-o", HOST_LIB_PATH, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"{cmd[0]} failed on {HOST_SOURCE}:\n{res.stderr}")
+    compiler = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC"]
+    defines = ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+               *(x for p in include for x in ("-isystem", p))]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+
+    def run(cmd: list[str], what: str) -> None:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{compiler[0]} failed on {what}:\n{res.stderr}")
+
+    objs = [os.path.join(OBJ_DIR, os.path.splitext(s)[0] + ".o") for s in HOST_SOURCES]
+    with ThreadPoolExecutor(max_workers=len(objs)) as pool:
+        list(pool.map(lambda so: run([*compiler, *defines, "-c", os.path.join(CSRC, so[0]), "-o", so[1]], so[0]), zip(HOST_SOURCES, objs)))
+    run([*compiler, "-shared", *objs, "-o", HOST_LIB_PATH, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+         "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"], "_host.so")
     if verbose:
         print(f"built {HOST_LIB_PATH}")
     return HOST_LIB_PATH

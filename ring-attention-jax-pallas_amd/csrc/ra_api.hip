@@ -10,6 +10,10 @@
 
 #include "ra_launch.h"
 
+namespace ra {
+int fail_with(int code, const char* fmt, va_list ap);  // (its text is the thread's last error)
+}
+
 namespace {
 
 thread_local char g_err[512] = "";
@@ -17,7 +21,7 @@ thread_local char g_err[512] = "";
 int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  ra::fail_with(code, fmt, ap);
   va_end(ap);
   return code;
 }
@@ -25,6 +29,13 @@ int fail(int code, const char* fmt, ...) {
 int hip_fail(hipError_t e, const char* what) {
   return fail(RA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
+
+}  // namespace
+int ra::fail_with(int code, const char* fmt, va_list ap) {
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  return code;
+}
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/ring_attention_hip.h"
+#include "ra_host.h"
 
 namespace {
 
@@ -723,4 +724,14 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "Calls on whole sequence
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host(void) { return PyModule_Create(&g_module); }
+void ra_host::check(const char* what, int code) { ::check(what, code); }
+void* ra_host::stream(const at::Device& device) { return ::stream(device); }
+int ra_host::row_dtype(at::ScalarType t) { return ::row_dtype(t); }
+const at::Tensor& ra_host::tensor_of(PyObject* x) { return ::tensor_of(x); }
+PyObject* ra_host::tuple_of(std::vector<at::Tensor>&& tensors) { return ::tuple_of(std::move(tensors)); }
+
+PyMODINIT_FUNC PyInit__host(void) {
+  PyObject* module = PyModule_Create(&g_module);
+  if (module && PyModule_AddFunctions(module, ra_host::paged_methods()) < 0) Py_CLEAR(module);
+  return module;
+}

@@ -1,0 +1,96 @@
+// Argument blocks and host launchers of the paged key-value cache: page slots, writes, mean keys, page selection, attention of one
+// token per sequence.
+#pragma once
+#include "ra_common.h"
+
+namespace ra {
+
+constexpr int kMaxRows = RA_MAX_PAGED_ROWS;  // sequences of one call: their prefix sums lie in shared memory
+constexpr int kStepKeys = 128;               // keys that a workgroup of the attention kernel takes at a time, 32 a wave
+constexpr int kPartRows = 16;                // query heads of a workgroup: the columns of a matrix instruction
+
+struct PageTable {
+  const int* at;
+  long long sb;
+  int width, n_pages, shift;  // page_size = 1 << shift
+};
+
+// A pool [page, token, head, dim] of 16-bit elements: strides in elements, `dim` contiguous; offsets within a page fit 32 bits.
+struct PoolArg {
+  const unsigned short* ptr;
+  long long sp;
+  int st, sh;
+};
+
+struct SlotsArgs {
+  int* table;
+  long long table_sb;
+  int width, B, shift;
+  const int *before, *after;
+  int* ring;
+  int n_pages;
+  const int* state;
+  long long* slots;
+  int n_slots;
+  int *starts, *granted, *state_out;
+};
+hipError_t launch_slots(const SlotsArgs& a, hipStream_t stream);
+
+struct WriteArgs {
+  const void *k, *v;
+  long long k_st, k_sh, v_st, v_sh;  // of the sources, [token, head, dim]
+  PoolArg k_pool, v_pool;
+  const long long* slots;
+  int T, H, D, shift;
+  long long n_slots;  // n_pages * page_size
+};
+hipError_t launch_write(const WriteArgs& a, int src_dtype, int dtype, hipStream_t stream);
+
+struct MeansArgs {
+  PoolArg k;
+  PageTable table;
+  const int *before, *after;
+  unsigned short* means;
+  long long means_sp;
+  int means_sh, B, H, D;
+};
+hipError_t launch_means(const MeansArgs& a, int dtype, hipStream_t stream);
+
+struct SelectArgs {
+  const unsigned short* q;
+  long long q_sb;
+  int q_sh;
+  const unsigned short* means;
+  long long means_sp;
+  int means_sh;
+  PageTable table;
+  const int* lengths;
+  int B, H, G, D, count, first, last;
+  unsigned long long* keys;  // [B, H, width]
+  int* pages;                // [B, H, count]
+};
+hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream);
+
+struct PagedArgs {
+  const unsigned short* q;
+  long long q_sb;
+  int q_sh;
+  PoolArg k, v;
+  PageTable table;
+  const int* lengths;
+  const int* pages;  // [B, H, count]: the pages that are read; NULL: all
+  int count;
+  int B, H, G, tiles;  // heads of the cache, query heads for each, groups of kPartRows among them
+  int window;          // 0: none
+  const float* slopes;
+  float scale2;        // sm_scale * log2(e)
+  unsigned short* out;  // [B, H * G, D]
+  float* lse;           // [B, H * G]
+  float* part;          // [2 n_wg, kPartRows, D], then [2 n_wg, kPartRows] maxima and as many sums
+  int n_wg;
+};
+int paged_workgroups(long long most_steps);
+long long paged_part_floats(int n_wg, int D);
+hipError_t launch_paged(const PagedArgs& a, int D, int dtype, bool one_step, hipStream_t stream);
+
+}  // namespace ra

@@ -1,0 +1,805 @@
+// A key-value cache in pages: which page holds which token (slots), writing into pages, the mean keys of pages, the choice of pages by
+// those, and attention of one token per sequence over its pages.
+#include "ra_paged.h"
+
+namespace ra {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2), aligned(4))) unsigned int u32x2a;
+typedef __attribute__((ext_vector_type(3), aligned(4))) unsigned int u32x3a;
+
+struct BF16 {
+  static RA_DEV float up(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
+  static RA_DEV unsigned short down(float x) { return __builtin_bit_cast(unsigned short, (bf16_t)x); }
+  static RA_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static constexpr float kLift = 0.f;
+};
+struct F16 {
+  static RA_DEV float up(unsigned short x) { return (float)__builtin_bit_cast(_Float16, x); }
+  static RA_DEV unsigned short down(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
+  static RA_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  // Weights are rounded to fp16 as 2^15 times their value: 2^17 of them that are 2^-25 of the largest, each below fp16's least, make up 2^-8 of
+  // the output.
+  static constexpr float kLift = 15.f;
+};
+template <class T>
+RA_DEV unsigned down2(float lo, float hi) {
+  return (unsigned)T::down(lo) | (unsigned)T::down(hi) << 16;
+}
+
+RA_DEV int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
+
+// Exclusive prefix sums of `value(row)` over rows [0, B) in sums[0 .. B], their total returned; all NT threads.  `red`: a word per wave and one.
+// The sums lie in shared memory, so that whatever walks the rows' items in one line finds an item's row by halving.
+template <int NT, class F>
+RA_DEV int scan_rows(int B, F value, int* sums, int* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int before = 0;
+  for (int i0 = 0; i0 < B; i0 += NT) {
+    const int i = i0 + threadIdx.x;
+    const int x = i < B ? value(i) : 0;
+    int s = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(s, o, 64);
+      s += lane >= o ? y : 0;
+    }
+    if (lane == 63) red[wave] = s;
+    __syncthreads();
+    int ahead = before, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+      ahead += w < wave ? red[w] : 0;
+      all += red[w];
+    }
+    if (i < B) sums[i] = ahead + s - x;
+    before += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) sums[B] = before;
+  __syncthreads();
+  return before;
+}
+// The row that item i < sums[B] belongs to: the last one whose sum is <= i.
+RA_DEV int row_of(const int* sums, int B, int i) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sums[mid] <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------------------
+// slots
+// ---------------------------------------------------------------------------------------
+// Row b goes from before[b] to after[b] tokens.  Pages are taken from the head of the ring of free pages and given back behind its end, both in the
+// order of the rows, so every place follows from prefix sums over the rows: each workgroup makes those for itself, and no workgroup waits for
+// another.  What is read (the ring's free part, the rows that end) is never what is written (the part behind it, the rows
+// that grow).
+constexpr int kSlotThreads = 256;
+__global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) {
+  extern __shared__ int s_mem[];
+  __shared__ int red[kSlotThreads / 64];
+  int* s_new = s_mem;
+  int* s_take = s_new + a.B + 1;
+  int* s_give = s_take + a.B + 1;
+  const int size = 1 << a.shift, cap = a.width << a.shift, tid = threadIdx.x;
+  const int P = a.n_pages;
+  const int first = (int)((unsigned)max(a.state[0], 0) % (unsigned)P), count = min(max(a.state[1], 0), P);
+  auto old_of = [&](int b) { return min(max(a.before[b], 0), cap); };
+  auto had_of = [&](int b) { return pages_of(old_of(b), a.shift); };
+  auto wants_of = [&](int b) { return pages_of(min(max(a.after[b], 0), cap), a.shift); };
+  scan_rows<kSlotThreads>(a.B, [&](int b) { return max(a.after[b] - max(a.before[b], 0), 0); }, s_new, red);
+  const int take = scan_rows<kSlotThreads>(a.B, [&](int b) { return max(wants_of(b) - had_of(b), 0); }, s_take, red);
+  const int give = scan_rows<kSlotThreads>(a.B, [&](int b) { return max(had_of(b) - wants_of(b), 0); }, s_give, red);
+  // what row b holds from now on: no more than its pages do
+  auto granted_of = [&](int b) {
+    const int n = old_of(b), m = min(max(a.after[b], 0), cap);
+    if (m <= n) return m;
+    const int got = min(s_take[b + 1] - s_take[b], max(count - s_take[b], 0));
+    return min(m, (pages_of(n, a.shift) + got) << a.shift);
+  };
+  const int stride = gridDim.x * kSlotThreads, me = blockIdx.x * kSlotThreads + tid;
+  for (int b = me; b < a.B; b += stride) {
+    a.granted[b] = granted_of(b);
+    a.starts[b] = s_new[b];
+  }
+  if (me == 0) {
+    const int used = min(take, count);
+    a.starts[a.B] = s_new[a.B];
+    a.state_out[0] = (int)(((unsigned)first + (unsigned)used) % (unsigned)P);
+    a.state_out[1] = min(count - used + give, P);
+  }
+  auto ring_at = [&](int r) { return (int)(((unsigned)first + (unsigned)r) % (unsigned)P); };
+  for (int t = me; t < a.n_slots; t += stride) {
+    long long slot = -1;
+    if (t < s_new[a.B]) {
+      const int b = row_of(s_new, a.B, t), n = old_of(b), position = n + t - s_new[b];
+      if (position >= n && position < granted_of(b)) {
+        const int j = position >> a.shift, had = pages_of(n, a.shift);
+        const int page = j < had ? a.table[b * a.table_sb + j] : a.ring[ring_at(s_take[b] + j - had)];
+        if (page >= 0 && page < P) slot = (long long)page * size + (position & (size - 1));
+      }
+    }
+    a.slots[t] = slot;
+  }
+  for (int i = me; i < min(take, count); i += stride) {
+    const int b = row_of(s_take, a.B, i);
+    a.table[b * a.table_sb + had_of(b) + i - s_take[b]] = a.ring[ring_at(i)];
+  }
+  for (int i = me; i < give; i += stride) {
+    const int b = row_of(s_give, a.B, i);
+    a.ring[(int)(((unsigned)ring_at(count) + (unsigned)i) % (unsigned)P)] = a.table[b * a.table_sb + wants_of(b) + i - s_give[b]];
+  }
+}
+
+hipError_t launch_slots(const SlotsArgs& a, hipStream_t stream) {
+  const int items = a.n_slots > a.B ? a.n_slots : a.B;
+  const int wgs = items <= kSlotThreads ? 1 : (items + 2 * kSlotThreads - 1) / (2 * kSlotThreads);
+  hipLaunchKernelGGL(slots_kernel, dim3(wgs < 256 ? wgs : 256), dim3(kSlotThreads), 3 * (a.B + 1) * sizeof(int), stream, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------
+// writes
+// ---------------------------------------------------------------------------------------
+// Eight elements of a token's key and of its value per thread, neighbouring threads on neighbouring chunks.  HBM bound.
+template <class S, class T>
+RA_DEV u32x4 load8(const void* base, long long at) {
+  if constexpr (__is_same(S, float)) {
+    const f32x4 x = *(const f32x4*)((const float*)base + at), y = *(const f32x4*)((const float*)base + at + 4);
+    return (u32x4){down2<T>(x[0], x[1]), down2<T>(x[2], x[3]), down2<T>(y[0], y[1]), down2<T>(y[2], y[3])};
+  } else {
+    const u32x4 x = *(const u32x4*)((const unsigned short*)base + at);
+    if constexpr (__is_same(S, T)) return x;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = down2<T>(S::up((unsigned short)x[i]), S::up((unsigned short)(x[i] >> 16)));
+    return r;
+  }
+}
+template <class S, class T>
+__global__ __launch_bounds__(256) void write_kernel(const WriteArgs a) {
+  const unsigned cpr = (unsigned)a.D / 8, line = cpr * (unsigned)a.H;
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  const long long t = i / line;
+  if (t >= a.T) return;
+  const long long slot = a.slots[t];
+  if (slot < 0 || slot >= a.n_slots) return;
+  const unsigned in_line = i - (unsigned)t * line, h = in_line / cpr, d = 8 * (in_line - h * cpr);
+  const long long page = slot >> a.shift;
+  const int off = (int)(slot & ((1 << a.shift) - 1));
+  const u32x4 k = load8<S, T>(a.k, t * a.k_st + h * a.k_sh + d), v = load8<S, T>(a.v, t * a.v_st + h * a.v_sh + d);
+  *(u32x4*)const_cast<unsigned short*>(a.k_pool.ptr + page * a.k_pool.sp + (off * a.k_pool.st + (int)h * a.k_pool.sh + (int)d)) = k;
+  *(u32x4*)const_cast<unsigned short*>(a.v_pool.ptr + page * a.v_pool.sp + (off * a.v_pool.st + (int)h * a.v_pool.sh + (int)d)) = v;
+}
+
+hipError_t launch_write(const WriteArgs& a, int src_dtype, int dtype, hipStream_t stream) {
+  const long long chunks = (long long)a.T * a.H * (a.D / 8);
+  const dim3 grid((unsigned)((chunks + 255) / 256));
+  const bool half = dtype == RA_DTYPE_F16;
+  void (*kernel)(WriteArgs) = half ? write_kernel<BF16, F16> : write_kernel<BF16, BF16>;
+  if (src_dtype == RA_DTYPE_F32) kernel = half ? write_kernel<float, F16> : write_kernel<float, BF16>;
+  else if (src_dtype == RA_DTYPE_F16) kernel = half ? write_kernel<F16, F16> : write_kernel<F16, BF16>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------
+// mean keys
+// ---------------------------------------------------------------------------------------
+// The mean over the tokens that a page holds, for each page whose tokens change between before[b] and after[b]: a workgroup per page and 64 chunks
+// of eight elements, its threads on neighbouring chunks and, beyond those, on different tokens.  HBM bound.
+constexpr int kMeanThreads = 256;
+template <class T>
+__global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) {
+  extern __shared__ int s_first[];
+  __shared__ int red[kMeanThreads / 64];
+  __shared__ float s_sum[kMeanThreads][9];  // (nine words apart: no two of a wave's rows in one bank)
+  const int size = 1 << a.table.shift, cap = a.table.width << a.table.shift, tid = threadIdx.x;
+  auto low = [&](int b) { return min(max(min(a.before[b], a.after[b]), 0), cap) >> a.table.shift; };
+  auto pages = [&](int b) {
+    return a.before[b] == a.after[b] ? 0 : max(pages_of(min(max(a.after[b], 0), cap), a.table.shift) - low(b), 0);
+  };
+  const int total = scan_rows<kMeanThreads>(a.B, pages, s_first, red);
+  const int cpr = a.D / 8, line = cpr * a.H;
+  int cols = 8;
+  while (cols < 64 && cols < line) cols *= 2;
+  const int chunk = blockIdx.y * 64 + tid % cols, step = kMeanThreads / cols, r0 = tid / cols;
+  const int h = chunk / cpr, d = 8 * (chunk % cpr);
+  for (int i = blockIdx.x; i < total; i += gridDim.x) {
+    const int b = row_of(s_first, a.B, i), j = low(b) + i - s_first[b];
+    const int n = min(size, min(max(a.after[b], 0), cap) - (j << a.table.shift));
+    const int page = a.table.at[b * a.table.sb + j];
+    const bool there = page >= 0 && page < a.table.n_pages;
+    float sum[8] = {};
+    if (there && chunk < line) {
+      const unsigned short* at = a.k.ptr + page * a.k.sp + (h * a.k.sh + d);
+#pragma unroll 4
+      for (int r = r0; r < n; r += step) {
+        const u32x4 x = *(const u32x4*)(at + r * a.k.st);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum[2 * e] += T::up((unsigned short)x[e]);
+          sum[2 * e + 1] += T::up((unsigned short)(x[e] >> 16));
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_sum[tid][e] = sum[e];
+    __syncthreads();
+    if (r0 == 0 && there && chunk < line) {
+      for (int g = 1; g < step; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += s_sum[tid + g * cols][e];
+      const float count = (float)n;
+      *(u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + d)) =
+          (u32x4){down2<T>(sum[0] / count, sum[1] / count), down2<T>(sum[2] / count, sum[3] / count), down2<T>(sum[4] / count, sum[5] / count),
+                  down2<T>(sum[6] / count, sum[7] / count)};
+    }
+    __syncthreads();
+  }
+}
+
+hipError_t launch_means(const MeansArgs& a, int dtype, hipStream_t stream) {
+  const int line = a.H * a.D / 8;
+  const int wgs = a.B < 256 ? 256 : (a.B < 1024 ? a.B : 1024);
+  void (*kernel)(MeansArgs) = dtype == RA_DTYPE_F16 ? means_kernel<F16> : means_kernel<BF16>;
+  hipLaunchKernelGGL(kernel, dim3(wgs, (line + 63) / 64), dim3(kMeanThreads),
+                     (a.B + 1) * sizeof(int), stream, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------
+// choice of pages
+// ---------------------------------------------------------------------------------------
+// Scores: (sum of the group's queries) . (mean key), in 64 bits: products of 16-bit floats are exact there, and so are their sums but for
+// extreme ranges, so that the order of pages does not depend on the order of a sum.  A score becomes a whole number of the same order.
+// Sixteen lanes (eight, four for narrow heads) read a page's mean in one go, a wave 64 pages; their partial sums are exchanged so that each
+// lane ends with the sums of its own pages.
+constexpr int kScorePages = 256;  // of a workgroup, 64 a wave
+constexpr unsigned long long kForced = ~0ull;
+RA_DEV unsigned long long ordered(double x) {
+  if (x != x) return kForced - 1;  // (not a number: before every number, as sorting has it)
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, x + 0.0);  // (-0 and 0 are equal)
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+RA_DEV double shfl_xor(double x, int o) { return __shfl_xor(x, o, 64); }
+
+template <class T, int D>
+__global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
+  constexpr int LPR = D == 32 ? 4 : (D == 64 ? 8 : 16);  // lanes of a row
+  constexpr int RPI = 64 / LPR, ITERS = 64 / RPI;        // rows a load, loads for 64 pages (= LPR)
+  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63;
+  const int n = pages_of(min(max(a.lengths[b], 0), a.table.width << a.table.shift), a.table.shift);
+  const int p0 = blockIdx.x * kScorePages + (threadIdx.x >> 6) * 64;
+  if (p0 >= n || n <= a.count) return;  // (few pages: all of them, whatever their scores)
+  const int c = lane % LPR, sub = lane / LPR;
+  const bool in_row = c * 8 < D;
+  const int mine = p0 + lane < n ? a.table.at[b * a.table.sb + p0 + lane] : -1;
+  u32x4 m[ITERS];
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    const int page = __shfl(mine, i * RPI + sub, 64);
+    m[i] = (u32x4){0, 0, 0, 0};
+    if (in_row && page >= 0 && page < a.table.n_pages) m[i] = *(const u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + c * 8));
+  }
+  double q[8] = {};
+  if (in_row)
+    for (int g = 0; g < a.G; ++g) {
+      const u32x4 x = *(const u32x4*)(a.q + b * a.q_sb + ((long long)h * a.G + g) * a.q_sh + c * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        q[2 * e] += (double)T::up((unsigned short)x[e]);
+        q[2 * e + 1] += (double)T::up((unsigned short)(x[e] >> 16));
+      }
+    }
+  double s[ITERS];
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    s[i] = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[i] = __builtin_fma(q[2 * e], (double)T::up((unsigned short)m[i][e]), s[i]);
+      s[i] = __builtin_fma(q[2 * e + 1], (double)T::up((unsigned short)(m[i][e] >> 16)), s[i]);
+    }
+  }
+  // lane c of a row's lanes keeps the loads whose number is c
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) {
+    const bool up = c & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const double keep = up ? s[i + o] : s[i], send = up ? s[i] : s[i + o];
+      s[i] = keep + shfl_xor(send, o);
+    }
+  }
+  const int p = p0 + c * RPI + sub;
+  if (p < n) a.keys[((long long)b * a.H + h) * a.table.width + p] = p < a.first || p >= n - a.last ? kForced : ordered(s[0]);
+}
+
+// The `count` largest of a row's numbers, ties from the lowest index, their indexes in order: the threshold by its digits from the first in which
+// the numbers differ, eight bits at a time, until all that share its digits are taken; then every wave places what it takes of
+// its part of the row.
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
+  __shared__ int s_hist[256], s_pick[2], s_above[kSelectWaves], s_equal[kSelectWaves];
+  __shared__ unsigned long long s_or[kSelectWaves], s_and[kSelectWaves];
+  const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = pages_of(min(max(a.lengths[b], 0), a.table.width << a.table.shift), a.table.shift);
+  int* out = a.pages + ((long long)b * a.H + h) * a.count;
+  if (n <= a.count) {
+    for (int i = tid; i < a.count; i += kSelectThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const unsigned long long* keys = a.keys + ((long long)b * a.H + h) * a.table.width;
+  unsigned long long any = 0, every = ~0ull;
+  for (int i = tid; i < n; i += kSelectThreads) {
+    any |= keys[i];
+    every &= keys[i];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    any |= __shfl_xor(any, o, 64);
+    every &= __shfl_xor(every, o, 64);
+  }
+  if (lane == 0) {
+    s_or[wave] = any;
+    s_and[wave] = every;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    any |= s_or[w];
+    every &= s_and[w];
+  }
+  const unsigned long long differ = any ^ every;
+  // `known` bits from the top are those of the threshold; `need` of the numbers that have them are to be taken
+  int known = differ ? __builtin_clzll(differ) : 64, need = a.count, sharing = n;
+  unsigned long long top = known == 0 ? 0 : (known == 64 ? any : any >> (64 - known) << (64 - known));
+  while (known < 64 && need < sharing) {
+    const int bits = min(8, 64 - known), down = 64 - known - bits;
+    for (int i = tid; i < 256; i += kSelectThreads) s_hist[i] = 0;
+    __syncthreads();
+    const unsigned long long mask = known == 0 ? 0 : ~0ull << (64 - known);
+    for (int i = tid; i < n; i += kSelectThreads) {
+      const unsigned long long x = keys[i];
+      if ((x & mask) == top) atomicAdd(&s_hist[(int)(x >> down) & ((1 << bits) - 1)], 1);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // four digits a lane, from the highest: lane 0 has 255 .. 252
+      int c[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[e] = s_hist[255 - 4 * lane - e];
+        sum += c[e];
+      }
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o, 64);
+        upto += lane >= o ? y : 0;
+      }
+      int above = upto - sum;
+      if (above < need && upto >= need)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (above < need && above + c[e] >= need) {
+            s_pick[0] = 255 - 4 * lane - e;
+            s_pick[1] = above;
+          }
+          above += c[e];
+        }
+    }
+    __syncthreads();
+    const int digit = s_pick[0];
+    need -= s_pick[1];
+    sharing = s_hist[digit];
+    top |= (unsigned long long)digit << down;
+    known += bits;
+    __syncthreads();
+  }
+  const unsigned long long mask = known == 0 ? 0 : ~0ull << (64 - known);
+  const int part = ((n + kSelectThreads - 1) / kSelectThreads) * 64, from = wave * part, to = min(from + part, n);
+  int above = 0, equal = 0;
+  for (int i = from + lane; i - lane < to; i += 64) {
+    const unsigned long long x = i < to ? keys[i] & mask : 0;
+    above += __popcll(__ballot(i < to && x > top));
+    equal += __popcll(__ballot(i < to && x == top));
+  }
+  if (lane == 0) {
+    s_above[wave] = above;
+    s_equal[wave] = equal;
+  }
+  __syncthreads();
+  above = equal = 0;
+  for (int w = 0; w < wave; ++w) {
+    above += s_above[w];
+    equal += s_equal[w];
+  }
+  const unsigned long long below = (1ull << lane) - 1;
+  for (int i = from + lane; i - lane < to; i += 64) {
+    const unsigned long long x = i < to ? keys[i] & mask : 0;
+    const bool gt = i < to && x > top, eq = i < to && x == top;
+    const unsigned long long gts = __ballot(gt), eqs = __ballot(eq);
+    const int my_gt = above + __popcll(gts & below), my_eq = equal + __popcll(eqs & below);
+    if (gt || (eq && my_eq < need)) out[my_gt + min(my_eq, need)] = i;
+    above += __popcll(gts);
+    equal += __popcll(eqs);
+  }
+}
+
+template <class T>
+static void launch_score(const SelectArgs& a, hipStream_t stream) {
+  const dim3 grid((a.table.width + kScorePages - 1) / kScorePages, a.H, a.B);
+  void (*kernel)(SelectArgs) = a.D == 32 ? score_kernel<T, 32> : a.D == 64 ? score_kernel<T, 64> : a.D == 96 ? score_kernel<T, 96> : score_kernel<T, 128>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
+}
+hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
+  if (a.table.width > a.count) {  // (else every row has few pages)
+    if (dtype == RA_DTYPE_F16) launch_score<F16>(a, stream);
+    else launch_score<BF16>(a, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(select_kernel, dim3(a.H, a.B), dim3(kSelectThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------
+// attention of one token per sequence
+// ---------------------------------------------------------------------------------------
+// The work of a call is one line of steps of 128 keys: row by row of the batch, head by head of the cache, along the sequence.  Every workgroup
+// takes an equal stretch of it, so that rows of any lengths load the chip evenly; lengths are on the device, and each workgroup makes the
+// line's prefix sums for itself.  A stretch that holds a (row, head) whole stores its output; parts of one go to memory as (maximum, sum,
+// unnormalised output) in 32 bits and are joined by a second kernel.
+struct Line {
+  int steps_b;     // steps of a row, of each of its heads
+  unsigned whole, rest;  // steps of a workgroup: whole + 1 for the first `rest`, whole for the others
+};
+RA_DEV int first_key(const PagedArgs& a, int len) { return a.window > 0 ? max(len - a.window, 0) & ~31 : 0; }
+RA_DEV int row_length(const PagedArgs& a, int b) { return min(max(a.lengths[b], 0), a.table.width << a.table.shift); }
+RA_DEV int row_steps(const PagedArgs& a, int b) {
+  if (a.pages != nullptr) return ((a.count << a.table.shift) + kStepKeys - 1) / kStepKeys;
+  const int len = row_length(a, b);
+  return max((len - first_key(a, len) + kStepKeys - 1) / kStepKeys, 1);  // (one for an empty row: its output is stored too)
+}
+RA_DEV unsigned start_of(unsigned wg, unsigned whole, unsigned rest) { return wg * whole + min(wg, rest); }
+RA_DEV unsigned holder_of(unsigned step, unsigned whole, unsigned rest) {
+  const unsigned ahead = rest * (whole + 1);
+  return step < ahead ? step / (whole + 1) : rest + (step - ahead) / whole;
+}
+
+// (a maximum of -inf beside a sum: all scores that count are not numbers)
+template <class T>
+RA_DEV float logsumexp_of(float top, float sum) {
+  return ((top == RA_NEG_INF ? 0.f : top) - T::kLift + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// A wave's 32 keys and values on their way.  Keys are the matrix instruction's first operand: lane l holds key l % 16 of each half, eight
+// elements from 8 (l / 16) of every 32.  Of values lane l holds, of D / 16 elements from (l % 16) D / 16, the eight keys whose weights it gets from the scores'
+// product: 4 (l / 16) + 0 .. 3 of each half; a row is read whole by sixteen lanes.
+template <int D>
+struct KeyTile {
+  u32x4 k[2][D / 32];
+  unsigned v[8][D / 32];
+};
+
+template <int D>
+RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
+  if constexpr (D == 128) {
+    const u32x4 x = *(const u32x4*)at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x[i];
+  } else if constexpr (D == 96) {
+    const u32x3a x = *(const u32x3a*)at;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[i] = x[i];
+  } else if constexpr (D == 64) {
+    const u32x2a x = *(const u32x2a*)at;
+    v[0] = x[0];
+    v[1] = x[1];
+  } else {
+    v[0] = *(const unsigned*)at;
+  }
+}
+
+constexpr int kPagedThreads = 256, kPagedWaves = 4, kEntries = 1024;
+constexpr int kNowhere = 0x3fffffff;  // (a position behind every sequence)
+
+template <class T, int D, bool ALIBI>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs a) {
+  constexpr int KS = D / 32;  // matrix instructions of a score, words of a lane's value row
+  constexpr int DPL = D / 16;  // elements of a lane's value row
+  extern __shared__ int s_first[];
+  __shared__ int red[kPagedWaves];
+  __shared__ int s_page[kEntries], s_pos[kEntries];
+  __shared__ float s_m[kPagedWaves][16], s_l[kPagedWaves][16];
+  __shared__ float s_o[kPagedWaves][16][D + 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int units = a.H * a.tiles;  // of a row
+  const unsigned total = (unsigned)scan_rows<kPagedThreads>(a.B, [&](int b) { return row_steps(a, b); }, s_first, red) * (unsigned)units;
+  const unsigned whole = total / (unsigned)a.n_wg, rest = total % (unsigned)a.n_wg;
+  const unsigned begin = start_of(blockIdx.x, whole, rest), end = start_of(blockIdx.x + 1, whole, rest);
+  unsigned at = begin;
+  const int size = 1 << a.table.shift;
+  while (at < end) {
+    // the (row, head) that the stretch is in, and which of its steps
+    int b = row_of(s_first, a.B, (int)(at / (unsigned)units));
+    b = __builtin_amdgcn_readfirstlane(b);
+    const unsigned row0 = (unsigned)s_first[b] * units, steps = (unsigned)__builtin_amdgcn_readfirstlane(s_first[b + 1] - s_first[b]);
+    const unsigned unit = __builtin_amdgcn_readfirstlane((at - row0) / steps);
+    const unsigned unit0 = row0 + unit * steps, upto = min(end, unit0 + steps);
+    const int h = (int)unit / a.tiles, tile = (int)unit % a.tiles;
+    const int heads = min(a.G - tile * 16, 16);  // query heads of this unit
+    const long long head0 = (long long)b * a.H * a.G + h * a.G + tile * 16;
+    const int len = row_length(a, b), low = a.window > 0 ? max(len - a.window, 0) : 0, key0 = a.pages != nullptr ? 0 : first_key(a, len);
+    u32x4 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      q[s] = col < heads ? *(const u32x4*)(a.q + b * a.q_sb + (long long)(h * a.G + tile * 16 + col) * a.q_sh + s * 32 + grp * 8) : (u32x4){0, 0, 0, 0};
+    float slope = 0.f;
+    if constexpr (ALIBI) slope = col < heads ? a.slopes[h * a.G + tile * 16 + col] * kLog2e : 0.f;
+    float m = RA_NEG_INF, l = 0.f;
+    f32x4 o[DPL];
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const int n_entries = a.pages != nullptr ? a.count : pages_of(len, a.table.shift);
+    // kEntries pages at a time; a step's keys lie in the entries of one such chunk (both are powers of two and key0 is cut off below)
+    unsigned step = at - unit0;
+    const unsigned step_end = upto - unit0;
+    while (step < step_end) {
+      const int from_key = key0 + (int)step * kStepKeys, entry0 = from_key >> a.table.shift;
+      const unsigned fit = (unsigned)(((entry0 + kEntries) << a.table.shift) - from_key) / kStepKeys;
+      const unsigned chunk_end = min(step_end, step + fit);
+      const int n_here = min(((key0 + (int)chunk_end * kStepKeys - 1) >> a.table.shift) - entry0 + 1, kEntries);
+      __syncthreads();  // (the entries of the chunk before have been read)
+      for (int i = tid; i < n_here; i += kPagedThreads) {
+        const int e = entry0 + i;
+        int logical = e < n_entries ? e : -1;
+        if (a.pages != nullptr && logical >= 0) logical = a.pages[((long long)b * a.H + h) * a.count + e];
+        int page = logical >= 0 && logical < a.table.width ? a.table.at[b * a.table.sb + logical] : -1;
+        const bool there = page >= 0 && page < a.table.n_pages;
+        s_page[i] = there ? page : 0;
+        s_pos[i] = there ? logical << a.table.shift : kNowhere;
+      }
+      __syncthreads();
+      KeyTile<D> tiles[2];
+      int pos[2][2];
+      auto load = [&](KeyTile<D>& x, int (&p)[2], unsigned s) {
+        const int key = key0 + (int)s * kStepKeys + wave * 32;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int kt = key + 16 * t, e = (kt >> a.table.shift) - entry0, off = kt & (size - 1);
+          const int page = __builtin_amdgcn_readfirstlane(s_page[e]);
+          p[t] = __builtin_amdgcn_readfirstlane(s_pos[e]) + off;
+          const unsigned short* kp = a.k.ptr + page * a.k.sp + (off * a.k.st + h * a.k.sh);
+          const unsigned short* vp = a.v.ptr + page * a.v.sp + (off * a.v.st + h * a.v.sh);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) x.k[t][i] = *(const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) load_values<D>(x.v[4 * t + j], vp + ((4 * grp + j) * a.v.st + col * DPL));
+        }
+      };
+      auto use = [&](KeyTile<D>& x, const int (&p)[2]) {
+        const bool live = (p[0] < len && p[0] + 16 > low) || (p[1] < len && p[1] + 16 > low);
+        if (!live) return;
+        const bool inside = p[0] >= low && p[0] + 16 <= len && p[1] >= low && p[1] + 16 <= len;
+        float w[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < KS; ++i) c = T::mfma(x.k[t][i], q[i], c);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            w[4 * t + r] = c[r] * a.scale2;
+            if constexpr (ALIBI) w[4 * t + r] -= slope * (float)(len - 1 - p[t] - 4 * grp - r);
+          }
+        }
+        if (!inside) {
+          // What is masked may hold anything: its score is replaced, and its value too (0 times infinity is not 0).
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int at_key = p[j >> 2] + 4 * grp + (j & 3);
+            const bool on = at_key >= low && at_key < len;
+            w[j] = on ? w[j] : RA_NEG_INF;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) x.v[j][i] = on ? x.v[j][i] : 0u;
+          }
+        }
+        float top = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = half_max(top);
+        if (__any(top > m)) {
+          const float next = fmaxf(m, top), keep = next == RA_NEG_INF ? 1.f : __builtin_amdgcn_exp2f(m - next);
+          m = next;
+          l *= keep;
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) o[i] *= keep;
+        }
+        const float base = m == RA_NEG_INF ? 0.f : m - T::kLift;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          w[j] = __builtin_amdgcn_exp2f(w[j] - base);
+          l += w[j];
+        }
+        const u32x4 wb = {down2<T>(w[0], w[1]), down2<T>(w[2], w[3]), down2<T>(w[4], w[5]), down2<T>(w[6], w[7])};
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) {
+          const unsigned pick = i & 1 ? 0x07060302u : 0x05040100u;
+          u32x4 vt;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vt[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i >> 1], x.v[2 * j][i >> 1], pick);
+          o[i] = T::mfma(vt, wb, o[i]);
+        }
+      };
+      load(tiles[0], pos[0], step);
+      for (; step < chunk_end; step += 2) {
+        if (step + 1 < chunk_end) load(tiles[1], pos[1], step + 1);
+        use(tiles[0], pos[0]);
+        if (step + 1 >= chunk_end) break;
+        if (step + 2 < chunk_end) load(tiles[0], pos[0], step + 2);
+        use(tiles[1], pos[1]);
+      }
+      step = chunk_end;
+    }
+
+    // the four waves' parts
+    l += __shfl_xor(l, 16, 64);
+    l = half_sum(l);
+    __syncthreads();  // (the sums of the unit before have been read)
+    if (grp == 0) {
+      s_m[wave][col] = m;
+      s_l[wave][col] = l;
+    }
+    __syncthreads();
+    float most = RA_NEG_INF;
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) most = fmaxf(most, s_m[w][col]);
+    const float mine = m == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(m - most);
+    if (col < heads) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) s_o[wave][col][(4 * grp + r) * DPL + i] = o[i][r] * mine;
+    }
+    __syncthreads();
+    const bool complete = at == unit0 && upto == unit0 + steps;
+    const long long slot = 2ll * blockIdx.x + (at != begin);
+    for (int i = tid; i < heads * (D / 2); i += kPagedThreads) {
+      const int r = i / (D / 2), d = 2 * (i % (D / 2));
+      float top = RA_NEG_INF, sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < kPagedWaves; ++w) {
+        sum += s_l[w][r] * (s_m[w][r] == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+        x += s_o[w][r][d];
+        y += s_o[w][r][d + 1];
+      }
+      if (complete) {
+        // (a row without a key has a sum of 0; scores that are not numbers are in no maximum, but in the sum)
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *(unsigned*)(a.out + (head0 + r) * D + d) = down2<T>(x * inv, y * inv);
+        if (d == 0) a.lse[head0 + r] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
+      } else {
+        float* p = a.part + (slot * kPartRows + r) * D + d;
+        p[0] = x;
+        p[1] = y;
+        if (d == 0) {
+          float* stats = a.part + 2ll * a.n_wg * kPartRows * D;
+          stats[slot * kPartRows + r] = top;
+          stats[2ll * a.n_wg * kPartRows + slot * kPartRows + r] = sum;
+        }
+      }
+    }
+    at = upto;
+  }
+}
+
+// The parts of a (row, query head): a workgroup each, threads on neighbouring elements and on different parts.
+template <class T, int D>
+__global__ __launch_bounds__(256) void join_kernel(const PagedArgs a) {
+  constexpr int COLS = D / 4, GROUPS = 256 / COLS;
+  extern __shared__ int s_mem[];
+  __shared__ int red[4];
+  __shared__ float s_red[4], s_sum[GROUPS][D];
+  int* s_first = s_mem;
+  float* s_w = (float*)(s_mem + a.B + 1);  // a weight a part
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int units = a.H * a.tiles;
+  const unsigned total = (unsigned)scan_rows<256>(a.B, [&](int b) { return row_steps(a, b); }, s_first, red) * (unsigned)units;
+  const unsigned whole = total / (unsigned)a.n_wg, rest = total % (unsigned)a.n_wg;
+  const int b = blockIdx.y, head = blockIdx.x, h = head / a.G, g = head % a.G, r = g % 16;
+  const unsigned steps = (unsigned)(s_first[b + 1] - s_first[b]);
+  const unsigned unit0 = (unsigned)s_first[b] * units + (unsigned)(h * a.tiles + g / 16) * steps;
+  const unsigned w0 = holder_of(unit0, whole, rest), w1 = holder_of(unit0 + steps - 1, whole, rest);
+  if (w0 == w1) return;
+  const int parts = (int)(w1 - w0) + 1;
+  // a workgroup's first unit has its first place
+  const long long slot0 = 2ll * w0 + (start_of(w0, whole, rest) < unit0);
+  auto slot_of = [&](int i) { return i == 0 ? slot0 : 2ll * (w0 + i); };
+  const float* maxima = a.part + 2ll * a.n_wg * kPartRows * D;
+  const float* sums = maxima + 2ll * a.n_wg * kPartRows;
+  float top = RA_NEG_INF;
+  for (int i = tid; i < parts; i += 256) {
+    const float x = maxima[slot_of(i) * kPartRows + r];
+    s_w[i] = x;
+    top = fmaxf(top, x);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if (lane == 0) s_red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  float sum = 0.f;
+  for (int i = tid; i < parts; i += 256) {
+    const float w = s_w[i] == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_w[i] - top);
+    s_w[i] = w;
+    sum += w * sums[slot_of(i) * kPartRows + r];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  __syncthreads();
+  if (lane == 0) s_red[wave] = sum;
+  __syncthreads();
+  sum = s_red[0] + s_red[1] + s_red[2] + s_red[3];
+  const int c = tid % COLS, p0 = tid / COLS;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (p0 < GROUPS) {
+#pragma unroll 8
+    for (int i = p0; i < parts; i += GROUPS) x += s_w[i] * *(const f32x4*)(a.part + (slot_of(i) * kPartRows + r) * D + 4 * c);
+    *(f32x4*)&s_sum[p0][4 * c] = x;
+  }
+  __syncthreads();
+  const long long at = (long long)b * a.H * a.G + head;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (tid < D / 2) {
+    float y = 0.f, z = 0.f;
+#pragma unroll
+    for (int p = 0; p < GROUPS; ++p) {
+      y += s_sum[p][2 * tid];
+      z += s_sum[p][2 * tid + 1];
+    }
+    *(unsigned*)(a.out + at * D + 2 * tid) = down2<T>(y * inv, z * inv);
+  }
+  if (tid == 0) a.lse[at] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
+}
+
+int paged_workgroups(long long most_steps) { return (int)(most_steps < 512 ? most_steps : 512); }
+long long paged_part_floats(int n_wg, int D) { return 2ll * n_wg * kPartRows * (D + 2); }
+
+template <class T, int D>
+static hipError_t launch_paged_of(const PagedArgs& a, bool one_step, hipStream_t stream) {
+  const size_t shared = (a.B + 1) * sizeof(int);
+  if (a.slopes != nullptr) hipLaunchKernelGGL((paged_kernel<T, D, true>), dim3(a.n_wg), dim3(kPagedThreads), shared, stream, a);
+  else hipLaunchKernelGGL((paged_kernel<T, D, false>), dim3(a.n_wg), dim3(kPagedThreads), shared, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || one_step) return e;
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3(a.H * a.G, a.B), dim3(256), shared + a.n_wg * sizeof(float), stream, a);
+  return hipGetLastError();
+}
+template <class T>
+static hipError_t launch_paged_type(const PagedArgs& a, int D, bool one_step, hipStream_t stream) {
+  switch (D) {
+    case 32: return launch_paged_of<T, 32>(a, one_step, stream);
+    case 64: return launch_paged_of<T, 64>(a, one_step, stream);
+    case 96: return launch_paged_of<T, 96>(a, one_step, stream);
+    default: return launch_paged_of<T, 128>(a, one_step, stream);
+  }
+}
+hipError_t launch_paged(const PagedArgs& a, int D, int dtype, bool one_step, hipStream_t stream) {
+  return dtype == RA_DTYPE_F16 ? launch_paged_type<F16>(a, D, one_step, stream) : launch_paged_type<BF16>(a, D, one_step, stream);
+}
+
+}  // namespace ra

@@ -85,6 +85,25 @@ class RaTerms(C.Structure):  # (filled by csrc/ra_host.cc in the package's own c
     ]
 
 
+RA_MAX_PAGED_ROWS = 4096  # sequences of one call on a paged cache
+
+
+class RaPool(C.Structure):  # (these three filled by csrc/ra_paged_host.cc in the package's own calls)
+    _fields_ = [("ptr", C.c_void_p), ("stride_page", C.c_int64), ("stride_token", C.c_int64), ("stride_head", C.c_int64)]
+
+
+class RaPageTable(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_b", C.c_int64), ("width", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32)]
+
+
+class RaPagedParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("group", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32), ("window", C.c_int32),
+        ("sm_scale", C.c_float), ("n_pages_read", C.c_int32), ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64),
+        ("k", RaPool), ("v", RaPool), ("table", RaPageTable), ("lengths", C.c_void_p), ("pages", C.c_void_p), ("slopes", C.c_void_p),
+    ]
+
+
 EXPORTS = {
     "ra_version": (C.c_int, []),
     "ra_last_error": (C.c_char_p, []),
@@ -152,6 +171,18 @@ EXPORTS = {
     "ra_dense_map_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "ra_dense_map": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32,
                                C.c_int32, C.c_void_p, C.c_void_p]),
+    "ra_page_slots": (C.c_int, [C.POINTER(RaPageTable), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
+                                C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ra_write_pages": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                 C.POINTER(RaPool), C.POINTER(RaPool), C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+    "ra_page_means": (C.c_int, [C.POINTER(RaPool), C.c_int32, C.POINTER(RaPageTable), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+                                C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
+    "ra_select_pages_workspace": (C.c_int64, [C.POINTER(RaPageTable), C.c_int32, C.c_int32]),
+    "ra_select_pages": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.POINTER(RaPageTable), C.c_void_p,
+                                  C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64,
+                                  C.c_void_p]),
+    "ra_paged_attention_workspace": (C.c_int64, [C.POINTER(RaPagedParams)]),
+    "ra_paged_attention": (C.c_int, [C.POINTER(RaPagedParams), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "ra_step_is_skippable": (C.c_int, [C.POINTER(RaBias), C.c_int32, C.c_int32]),
     "ra_fwd_step_check": (C.c_int, [C.POINTER(RaFwdStepParams)]),
     "ra_bwd_step_check": (C.c_int, [C.POINTER(RaBwdStepParams)]),
@@ -190,7 +221,7 @@ _host = None
 
 
 def host():
-    """The module of ``csrc/ra_host.cc``, on the library that is loaded."""
+    """The module of ``csrc/ra_host.cc`` and ``csrc/ra_paged_host.cc``, on the library that is loaded."""
     global _host
     if _host is None:
         try:
@@ -203,6 +234,9 @@ def host():
                                                                  lib.ra_convert)), check)
         module.init_terms(*(C.cast(f, C.c_void_p).value for f in (lib.ra_fwd_terms, lib.ra_bwd_terms, lib.ra_fwd_terms_workspace,
                                                                        lib.ra_bwd_terms_workspace)))
+        module.init_paged(*(C.cast(f, C.c_void_p).value for f in (lib.ra_page_slots, lib.ra_write_pages, lib.ra_page_means, lib.ra_select_pages,
+                                                                       lib.ra_select_pages_workspace, lib.ra_paged_attention,
+                                                                       lib.ra_paged_attention_workspace)))
         _host = module
     return _host
 
