@@ -7,6 +7,8 @@ namespace ra {
 
 constexpr int kMaxRows = RA_MAX_PAGED_ROWS;  // sequences of one call: their prefix sums lie in shared memory
 constexpr int kStepKeys = 128;               // keys that a workgroup of the attention kernel takes at a time, 32 a wave
+constexpr int kWholeKeys = 1024;             // rows of up to so many keys (by the table) are not shared between workgroups
+constexpr int kPagedWorkgroups = 2048, kFewWorkgroups = 512, kStepsEach = 4;
 constexpr int kPartRows = 16;                // query heads of a workgroup: the columns of a matrix instruction
 
 struct PageTable {
@@ -53,6 +55,7 @@ struct MeansArgs {
   unsigned short* means;
   long long means_sp;
   int means_sh, B, H, D;
+  int cols;  // chunks of a workgroup (set by the launch)
 };
 hipError_t launch_means(const MeansArgs& a, int dtype, hipStream_t stream);
 
@@ -86,11 +89,19 @@ struct PagedArgs {
   float scale2;        // sm_scale * log2(e)
   unsigned short* out;  // [B, H * G, D]
   float* lse;           // [B, H * G]
-  float* part;          // [2 n_wg, kPartRows, D], then [2 n_wg, kPartRows] maxima and as many sums
+  // parts (of the workspace): [2 n_wg, kPartRows, D] and, of each, (maximum, sum); for each (row, head) the first one's place and their number
+  float* part;
+  float2* stats;
+  int2* where;
   int n_wg;
 };
-int paged_workgroups(long long most_steps);
-long long paged_part_floats(int n_wg, int D);
-hipError_t launch_paged(const PagedArgs& a, int D, int dtype, bool one_step, hipStream_t stream);
+struct PagedShape {
+  int workgroups;
+  bool whole;  // each takes a (row, head) whole
+  long long workspace;
+};
+// For rows of up to `keys` keys and so many (row, head)s.
+PagedShape paged_shape(long long keys, long long units, int D);
+hipError_t launch_paged(PagedArgs& a, int D, int dtype, const PagedShape& shape, void* workspace, hipStream_t stream);
 
 }  // namespace ra

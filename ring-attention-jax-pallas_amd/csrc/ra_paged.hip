@@ -33,36 +33,51 @@ RA_DEV unsigned down2(float lo, float hi) {
 
 RA_DEV int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
 
-// Exclusive prefix sums of `value(row)` over rows [0, B) in sums[0 .. B], their total returned; all NT threads.  `red`: a word per wave and one.
-// The sums lie in shared memory, so that whatever walks the rows' items in one line finds an item's row by halving.
-template <int NT, class F>
-RA_DEV int scan_rows(int B, F value, int* sums, int* red) {
+// Exclusive prefix sums of N values of each row, sums[n][0 .. B] in shared memory, so that whatever walks the rows' items in one line finds an
+// item's row by halving; all NT threads, neighbouring rows in a thread.  `values(row, x)` is called twice where B > NT.
+template <int NT, int N, class F>
+RA_DEV void scan_rows(int B, F values, int* const (&sums)[N], int (&red)[NT / 64][N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int before = 0;
-  for (int i0 = 0; i0 < B; i0 += NT) {
-    const int i = i0 + threadIdx.x;
-    const int x = i < B ? value(i) : 0;
-    int s = x;
+  const int per = (B + NT - 1) / NT, from = threadIdx.x * per, to = min(from + per, B);
+  int x[N], mine[N], s[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) mine[n] = 0;
+  for (int i = from; i < to; ++i) {
+    values(i, x);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mine[n] += x[n];
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    s[n] = mine[n];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(s, o, 64);
-      s += lane >= o ? y : 0;
+      const int y = __shfl_up(s[n], o, 64);
+      s[n] += lane >= o ? y : 0;
     }
-    if (lane == 63) red[wave] = s;
-    __syncthreads();
-    int ahead = before, all = 0;
+    if (lane == 63) red[wave][n] = s[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int all = 0;
+    s[n] -= mine[n];
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) {
-      ahead += w < wave ? red[w] : 0;
-      all += red[w];
+      s[n] += w < wave ? red[w][n] : 0;
+      all += red[w][n];
     }
-    if (i < B) sums[i] = ahead + s - x;
-    before += all;
-    __syncthreads();
+    if (threadIdx.x == 0) sums[n][B] = all;
   }
-  if (threadIdx.x == 0) sums[B] = before;
+  for (int i = from; i < to; ++i) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) sums[n][i] = s[n];
+    if (per == 1) break;
+    values(i, x);
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] += x[n];
+  }
   __syncthreads();
-  return before;
 }
 // The row that item i < sums[B] belongs to: the last one whose sum is <= i.
 RA_DEV int row_of(const int* sums, int B, int i) {
@@ -85,7 +100,7 @@ RA_DEV int row_of(const int* sums, int B, int i) {
 constexpr int kSlotThreads = 256;
 __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) {
   extern __shared__ int s_mem[];
-  __shared__ int red[kSlotThreads / 64];
+  __shared__ int red[kSlotThreads / 64][3];
   int* s_new = s_mem;
   int* s_take = s_new + a.B + 1;
   int* s_give = s_take + a.B + 1;
@@ -95,9 +110,17 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
   auto old_of = [&](int b) { return min(max(a.before[b], 0), cap); };
   auto had_of = [&](int b) { return pages_of(old_of(b), a.shift); };
   auto wants_of = [&](int b) { return pages_of(min(max(a.after[b], 0), cap), a.shift); };
-  scan_rows<kSlotThreads>(a.B, [&](int b) { return max(a.after[b] - max(a.before[b], 0), 0); }, s_new, red);
-  const int take = scan_rows<kSlotThreads>(a.B, [&](int b) { return max(wants_of(b) - had_of(b), 0); }, s_take, red);
-  const int give = scan_rows<kSlotThreads>(a.B, [&](int b) { return max(had_of(b) - wants_of(b), 0); }, s_give, red);
+  scan_rows<kSlotThreads, 3>(
+      a.B,
+      [&](int b, int (&x)[3]) {
+        const int n = a.before[b], m = a.after[b];
+        const int pages = pages_of(min(max(m, 0), cap), a.shift) - pages_of(min(max(n, 0), cap), a.shift);
+        x[0] = max(m - max(n, 0), 0);
+        x[1] = max(pages, 0);
+        x[2] = max(-pages, 0);
+      },
+      {s_new, s_take, s_give}, red);
+  const int take = s_take[a.B], give = s_give[a.B];
   // what row b holds from now on: no more than its pages do
   auto granted_of = [&](int b) {
     const int n = old_of(b), m = min(max(a.after[b], 0), cap);
@@ -194,24 +217,25 @@ hipError_t launch_write(const WriteArgs& a, int src_dtype, int dtype, hipStream_
 // ---------------------------------------------------------------------------------------
 // mean keys
 // ---------------------------------------------------------------------------------------
-// The mean over the tokens that a page holds, for each page whose tokens change between before[b] and after[b]: a workgroup per page and 64 chunks
+// The mean over the tokens that a page holds, for each page whose tokens change between before[b] and after[b]: a workgroup per page and up to 64 chunks
 // of eight elements, its threads on neighbouring chunks and, beyond those, on different tokens.  HBM bound.
 constexpr int kMeanThreads = 256;
 template <class T>
 __global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) {
   extern __shared__ int s_first[];
-  __shared__ int red[kMeanThreads / 64];
+  __shared__ int red[kMeanThreads / 64][1];
   __shared__ float s_sum[kMeanThreads][9];  // (nine words apart: no two of a wave's rows in one bank)
   const int size = 1 << a.table.shift, cap = a.table.width << a.table.shift, tid = threadIdx.x;
   auto low = [&](int b) { return min(max(min(a.before[b], a.after[b]), 0), cap) >> a.table.shift; };
-  auto pages = [&](int b) {
-    return a.before[b] == a.after[b] ? 0 : max(pages_of(min(max(a.after[b], 0), cap), a.table.shift) - low(b), 0);
-  };
-  const int total = scan_rows<kMeanThreads>(a.B, pages, s_first, red);
-  const int cpr = a.D / 8, line = cpr * a.H;
-  int cols = 8;
-  while (cols < 64 && cols < line) cols *= 2;
-  const int chunk = blockIdx.y * 64 + tid % cols, step = kMeanThreads / cols, r0 = tid / cols;
+  scan_rows<kMeanThreads, 1>(
+      a.B,
+      [&](int b, int (&x)[1]) {
+        x[0] = a.before[b] == a.after[b] ? 0 : max(pages_of(min(max(a.after[b], 0), cap), a.table.shift) - low(b), 0);
+      },
+      {s_first}, red);
+  const int total = s_first[a.B];
+  const int cpr = a.D / 8, line = cpr * a.H, cols = a.cols;
+  const int chunk = blockIdx.y * cols + tid % cols, step = kMeanThreads / cols, r0 = tid / cols;
   const int h = chunk / cpr, d = 8 * (chunk % cpr);
   for (int i = blockIdx.x; i < total; i += gridDim.x) {
     const int b = row_of(s_first, a.B, i), j = low(b) + i - s_first[b];
@@ -221,7 +245,7 @@ __global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) 
     float sum[8] = {};
     if (there && chunk < line) {
       const unsigned short* at = a.k.ptr + page * a.k.sp + (h * a.k.sh + d);
-#pragma unroll 4
+#pragma unroll 8
       for (int r = r0; r < n; r += step) {
         const u32x4 x = *(const u32x4*)(at + r * a.k.st);
 #pragma unroll
@@ -247,12 +271,15 @@ __global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) 
   }
 }
 
-hipError_t launch_means(const MeansArgs& a, int dtype, hipStream_t stream) {
+hipError_t launch_means(const MeansArgs& args, int dtype, hipStream_t stream) {
+  MeansArgs a = args;
   const int line = a.H * a.D / 8;
-  const int wgs = a.B < 256 ? 256 : (a.B < 1024 ? a.B : 1024);
+  // neighbouring threads on as many chunks as leave less than half of the last workgroup's without one
+  a.cols = 64;
+  while (a.cols > 8 && line % a.cols != 0 && line % a.cols <= a.cols / 2) a.cols /= 2;
+  const int wgs = a.B < 512 ? 512 : (a.B < 1024 ? a.B : 1024);
   void (*kernel)(MeansArgs) = dtype == RA_DTYPE_F16 ? means_kernel<F16> : means_kernel<BF16>;
-  hipLaunchKernelGGL(kernel, dim3(wgs, (line + 63) / 64), dim3(kMeanThreads),
-                     (a.B + 1) * sizeof(int), stream, a);
+  hipLaunchKernelGGL(kernel, dim3(wgs, (line + a.cols - 1) / a.cols), dim3(kMeanThreads), (a.B + 1) * sizeof(int), stream, a);
   return hipGetLastError();
 }
 
@@ -270,36 +297,58 @@ RA_DEV unsigned long long ordered(double x) {
   const unsigned long long u = __builtin_bit_cast(unsigned long long, x + 0.0);  // (-0 and 0 are equal)
   return u >> 63 ? ~u : u | 1ull << 63;
 }
-RA_DEV double shfl_xor(double x, int o) { return __shfl_xor(x, o, 64); }
+// Sums s[0 .. 2 O) over 2 O lanes, each of which keeps the one whose number is its own: half of them go to the partner, lane by lane bit.
+template <int O, int N>
+RA_DEV void exchange(double (&s)[N], int lane) {
+  if constexpr (O > 0) {
+    const bool up = lane & O;
+#pragma unroll
+    for (int i = 0; i < O; ++i) {
+      const double keep = up ? s[i + O] : s[i], send = up ? s[i] : s[i + O];
+      s[i] = keep + __shfl_xor(send, O, 64);
+    }
+    exchange<O / 2>(s, lane);
+  }
+}
 
 template <class T, int D>
 __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   constexpr int LPR = D == 32 ? 4 : (D == 64 ? 8 : 16);  // lanes of a row
   constexpr int RPI = 64 / LPR, ITERS = 64 / RPI;        // rows a load, loads for 64 pages (= LPR)
   const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63;
-  const int n = pages_of(min(max(a.lengths[b], 0), a.table.width << a.table.shift), a.table.shift);
   const int p0 = blockIdx.x * kScorePages + (threadIdx.x >> 6) * 64;
-  if (p0 >= n || n <= a.count) return;  // (few pages: all of them, whatever their scores)
   const int c = lane % LPR, sub = lane / LPR;
   const bool in_row = c * 8 < D;
-  const int mine = p0 + lane < n ? a.table.at[b * a.table.sb + p0 + lane] : -1;
+  // the length, the pages and the queries are on their way together
+  const int mine = a.table.at[b * a.table.sb + min(p0 + lane, a.table.width - 1)];
+  const int length = a.lengths[b];
+  const unsigned short* q_at = a.q + b * a.q_sb + (long long)h * a.G * a.q_sh + (in_row ? c * 8 : 0);
+  u32x4 x[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) x[g] = *(const u32x4*)(q_at + (long long)min(g, a.G - 1) * a.q_sh);
+  const int n = pages_of(min(max(length, 0), a.table.width << a.table.shift), a.table.shift);
+  if (p0 >= n || n <= a.count) return;  // (few pages: all of them, whatever their scores)
   u32x4 m[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    const int page = __shfl(mine, i * RPI + sub, 64);
-    m[i] = (u32x4){0, 0, 0, 0};
-    if (in_row && page >= 0 && page < a.table.n_pages) m[i] = *(const u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + c * 8));
+    const int page = min(max(__shfl(mine, i * RPI + sub, 64), 0), a.table.n_pages - 1);
+    m[i] = *(const u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + (in_row ? c * 8 : 0)));
+    if constexpr (D == 96) m[i] = in_row ? m[i] : (u32x4){0, 0, 0, 0};
   }
   double q[8] = {};
-  if (in_row)
-    for (int g = 0; g < a.G; ++g) {
-      const u32x4 x = *(const u32x4*)(a.q + b * a.q_sb + ((long long)h * a.G + g) * a.q_sh + c * 8);
+  for (int g0 = 0; g0 < a.G; g0 += 4) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        q[2 * e] += (double)T::up((unsigned short)x[e]);
-        q[2 * e + 1] += (double)T::up((unsigned short)(x[e] >> 16));
+        const unsigned y = g0 + g < a.G && in_row ? x[g][e] : 0u;
+        q[2 * e] += (double)T::up((unsigned short)y);
+        q[2 * e + 1] += (double)T::up((unsigned short)(y >> 16));
       }
-    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (g0 + 4 < a.G) x[g] = *(const u32x4*)(q_at + (long long)min(g0 + 4 + g, a.G - 1) * a.q_sh);
+  }
   double s[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
@@ -310,27 +359,19 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
       s[i] = __builtin_fma(q[2 * e + 1], (double)T::up((unsigned short)(m[i][e] >> 16)), s[i]);
     }
   }
-  // lane c of a row's lanes keeps the loads whose number is c
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) {
-    const bool up = c & o;
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const double keep = up ? s[i + o] : s[i], send = up ? s[i] : s[i + o];
-      s[i] = keep + shfl_xor(send, o);
-    }
-  }
-  const int p = p0 + c * RPI + sub;
+  exchange<LPR / 2>(s, c);  // (lane c of a row's lanes: the rows of load c)
+  const int p = p0 + c * RPI + sub, page = __shfl(mine, c * RPI + sub, 64);
+  if (page < 0 || page >= a.table.n_pages) s[0] = 0.0;
   if (p < n) a.keys[((long long)b * a.H + h) * a.table.width + p] = p < a.first || p >= n - a.last ? kForced : ordered(s[0]);
 }
 
-// The `count` largest of a row's numbers, ties from the lowest index, their indexes in order: the threshold by its digits from the first in which
-// the numbers differ, eight bits at a time, until all that share its digits are taken; then every wave places what it takes of
-// its part of the row.
-constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+// The `count` largest of a row's numbers, ties from the lowest index, their indexes in order: the threshold by its digits of twelve bits from the
+// top, until all that share the digits found so far are taken; then every wave places what it takes of its part of the row.  Twelve bits: the
+// first digit is a double's sign and exponent, and the second mostly settles it.  HELD: the row's numbers stay in registers, kHeld of a thread.
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kHeld = 8, kDigitBits = 12, kDigits = 1 << kDigitBits;
+template <bool HELD>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
-  __shared__ int s_hist[256], s_pick[2], s_above[kSelectWaves], s_equal[kSelectWaves];
-  __shared__ unsigned long long s_or[kSelectWaves], s_and[kSelectWaves];
+  __shared__ int s_hist[kDigits], s_pick[3], s_above[kSelectWaves], s_equal[kSelectWaves];
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = pages_of(min(max(a.lengths[b], 0), a.table.width << a.table.shift), a.table.shift);
   int* out = a.pages + ((long long)b * a.H + h) * a.count;
@@ -339,101 +380,95 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
     return;
   }
   const unsigned long long* keys = a.keys + ((long long)b * a.H + h) * a.table.width;
-  unsigned long long any = 0, every = ~0ull;
-  for (int i = tid; i < n; i += kSelectThreads) {
-    any |= keys[i];
-    every &= keys[i];
-  }
+  const int rounds = (n + kSelectThreads - 1) / kSelectThreads, part = rounds * 64, from = wave * part + lane, to = min(wave * part + part, n);
+  unsigned long long held[kHeld];
+  if constexpr (HELD) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    any |= __shfl_xor(any, o, 64);
-    every &= __shfl_xor(every, o, 64);
+    for (int r = 0; r < kHeld; ++r) held[r] = r < rounds && from + 64 * r < to ? keys[from + 64 * r] : 0;
   }
-  if (lane == 0) {
-    s_or[wave] = any;
-    s_and[wave] = every;
-  }
-  __syncthreads();
+  // every number of this thread: place, number
+  auto each = [&](auto&& use) {
+    if constexpr (HELD) {
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) {
-    any |= s_or[w];
-    every &= s_and[w];
-  }
-  const unsigned long long differ = any ^ every;
+      for (int r = 0; r < kHeld; ++r)
+        if (r < rounds) use(from + 64 * r, held[r]);
+    } else {
+      for (int r = 0; r < rounds; ++r) use(from + 64 * r, from + 64 * r < to ? keys[from + 64 * r] : 0ull);
+    }
+  };
   // `known` bits from the top are those of the threshold; `need` of the numbers that have them are to be taken
-  int known = differ ? __builtin_clzll(differ) : 64, need = a.count, sharing = n;
-  unsigned long long top = known == 0 ? 0 : (known == 64 ? any : any >> (64 - known) << (64 - known));
+  int known = 0, need = a.count, sharing = n;
+  unsigned long long top = 0, mask = 0;
   while (known < 64 && need < sharing) {
-    const int bits = min(8, 64 - known), down = 64 - known - bits;
-    for (int i = tid; i < 256; i += kSelectThreads) s_hist[i] = 0;
+    const int bits = min(kDigitBits, 64 - known), down = 64 - known - bits;
+#pragma unroll
+    for (int i = 0; i < kDigits / kSelectThreads; ++i) s_hist[tid + i * kSelectThreads] = 0;
     __syncthreads();
-    const unsigned long long mask = known == 0 ? 0 : ~0ull << (64 - known);
-    for (int i = tid; i < n; i += kSelectThreads) {
-      const unsigned long long x = keys[i];
-      if ((x & mask) == top) atomicAdd(&s_hist[(int)(x >> down) & ((1 << bits) - 1)], 1);
+    each([&](int i, unsigned long long x) {
+      if (i < to && (x & mask) == top) atomicAdd(&s_hist[(int)(x >> down) & ((1 << bits) - 1)], 1);
+    });
+    __syncthreads();
+    // four digits a thread, from the highest; sums within a wave, then over the waves before it
+    constexpr int DPT = kDigits / kSelectThreads;
+    int c[DPT], sum = 0;
+#pragma unroll
+    for (int e = 0; e < DPT; ++e) {
+      c[e] = s_hist[kDigits - 1 - DPT * tid - e];
+      sum += c[e];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o, 64);
+      upto += lane >= o ? y : 0;
+    }
+    if (lane == 63) s_above[wave] = upto;
+    __syncthreads();
+    int above = upto - sum;
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; ++w) above += w < wave ? s_above[w] : 0;
+#pragma unroll
+    for (int e = 0; e < DPT; ++e) {
+      if (above < need && above + c[e] >= need) {
+        s_pick[0] = kDigits - 1 - DPT * tid - e;
+        s_pick[1] = above;
+        s_pick[2] = c[e];
+      }
+      above += c[e];
     }
     __syncthreads();
-    if (wave == 0) {
-      // four digits a lane, from the highest: lane 0 has 255 .. 252
-      int c[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[e] = s_hist[255 - 4 * lane - e];
-        sum += c[e];
-      }
-      int upto = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o, 64);
-        upto += lane >= o ? y : 0;
-      }
-      int above = upto - sum;
-      if (above < need && upto >= need)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (above < need && above + c[e] >= need) {
-            s_pick[0] = 255 - 4 * lane - e;
-            s_pick[1] = above;
-          }
-          above += c[e];
-        }
-    }
-    __syncthreads();
-    const int digit = s_pick[0];
     need -= s_pick[1];
-    sharing = s_hist[digit];
-    top |= (unsigned long long)digit << down;
+    sharing = s_pick[2];
+    top |= (unsigned long long)s_pick[0] << down;
     known += bits;
-    __syncthreads();
+    mask = ~0ull << (64 - known);
   }
-  const unsigned long long mask = known == 0 ? 0 : ~0ull << (64 - known);
-  const int part = ((n + kSelectThreads - 1) / kSelectThreads) * 64, from = wave * part, to = min(from + part, n);
   int above = 0, equal = 0;
-  for (int i = from + lane; i - lane < to; i += 64) {
-    const unsigned long long x = i < to ? keys[i] & mask : 0;
-    above += __popcll(__ballot(i < to && x > top));
-    equal += __popcll(__ballot(i < to && x == top));
-  }
+  each([&](int i, unsigned long long x) {
+    above += __popcll(__ballot(i < to && (x & mask) > top));
+    equal += __popcll(__ballot(i < to && (x & mask) == top));
+  });
+  __syncthreads();
   if (lane == 0) {
     s_above[wave] = above;
     s_equal[wave] = equal;
   }
   __syncthreads();
   above = equal = 0;
-  for (int w = 0; w < wave; ++w) {
-    above += s_above[w];
-    equal += s_equal[w];
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    above += w < wave ? s_above[w] : 0;
+    equal += w < wave ? s_equal[w] : 0;
   }
   const unsigned long long below = (1ull << lane) - 1;
-  for (int i = from + lane; i - lane < to; i += 64) {
-    const unsigned long long x = i < to ? keys[i] & mask : 0;
-    const bool gt = i < to && x > top, eq = i < to && x == top;
+  each([&](int i, unsigned long long x) {
+    const bool gt = i < to && (x & mask) > top, eq = i < to && (x & mask) == top;
     const unsigned long long gts = __ballot(gt), eqs = __ballot(eq);
     const int my_gt = above + __popcll(gts & below), my_eq = equal + __popcll(eqs & below);
     if (gt || (eq && my_eq < need)) out[my_gt + min(my_eq, need)] = i;
     above += __popcll(gts);
     equal += __popcll(eqs);
-  }
+  });
 }
 
 template <class T>
@@ -449,7 +484,8 @@ hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(select_kernel, dim3(a.H, a.B), dim3(kSelectThreads), 0, stream, a);
+  void (*kernel)(SelectArgs) = a.table.width <= kHeld * kSelectThreads ? select_kernel<true> : select_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(a.H, a.B), dim3(kSelectThreads), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -459,17 +495,14 @@ hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
 // The work of a call is one line of steps of 128 keys: row by row of the batch, head by head of the cache, along the sequence.  Every workgroup
 // takes an equal stretch of it, so that rows of any lengths load the chip evenly; lengths are on the device, and each workgroup makes the
 // line's prefix sums for itself.  A stretch that holds a (row, head) whole stores its output; parts of one go to memory as (maximum, sum,
-// unnormalised output) in 32 bits and are joined by a second kernel.
-struct Line {
-  int steps_b;     // steps of a row, of each of its heads
-  unsigned whole, rest;  // steps of a workgroup: whole + 1 for the first `rest`, whole for the others
-};
+// unnormalised output) in 32 bits and are joined by a second kernel.  Where no row is longer than kWholeKeys (by the table), a workgroup of eight
+// waves takes each (row, head) whole, and that is all.
 RA_DEV int first_key(const PagedArgs& a, int len) { return a.window > 0 ? max(len - a.window, 0) & ~31 : 0; }
 RA_DEV int row_length(const PagedArgs& a, int b) { return min(max(a.lengths[b], 0), a.table.width << a.table.shift); }
-RA_DEV int row_steps(const PagedArgs& a, int b) {
-  if (a.pages != nullptr) return ((a.count << a.table.shift) + kStepKeys - 1) / kStepKeys;
-  const int len = row_length(a, b);
-  return max((len - first_key(a, len) + kStepKeys - 1) / kStepKeys, 1);  // (one for an empty row: its output is stored too)
+template <int STEP>
+RA_DEV int row_steps(const PagedArgs& a, int len) {
+  if (a.pages != nullptr) return ((a.count << a.table.shift) + STEP - 1) / STEP;
+  return max((len - first_key(a, len) + STEP - 1) / STEP, 1);  // (one for an empty row: its output is stored too)
 }
 RA_DEV unsigned start_of(unsigned wg, unsigned whole, unsigned rest) { return wg * whole + min(wg, rest); }
 RA_DEV unsigned holder_of(unsigned step, unsigned whole, unsigned rest) {
@@ -495,53 +528,75 @@ struct KeyTile {
 template <int D>
 RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
   if constexpr (D == 128) {
-    const u32x4 x = *(const u32x4*)at;
+    const u32x4 x = __builtin_nontemporal_load((const u32x4*)at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = x[i];
   } else if constexpr (D == 96) {
-    const u32x3a x = *(const u32x3a*)at;
+    const u32x3a x = __builtin_nontemporal_load((const u32x3a*)at);
 #pragma unroll
     for (int i = 0; i < 3; ++i) v[i] = x[i];
   } else if constexpr (D == 64) {
-    const u32x2a x = *(const u32x2a*)at;
+    const u32x2a x = __builtin_nontemporal_load((const u32x2a*)at);
     v[0] = x[0];
     v[1] = x[1];
   } else {
-    v[0] = *(const unsigned*)at;
+    v[0] = __builtin_nontemporal_load((const unsigned*)at);
   }
 }
 
-constexpr int kPagedThreads = 256, kPagedWaves = 4, kEntries = 1024;
+constexpr int kEntries = 1024;
 constexpr int kNowhere = 0x3fffffff;  // (a position behind every sequence)
 
-template <class T, int D, bool ALIBI>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs a) {
+template <class T, int D, bool ALIBI, bool WHOLE>
+__global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const PagedArgs a) {
+  constexpr int WAVES = WHOLE ? 8 : 4, THREADS = 64 * WAVES, STEP = 32 * WAVES;
   constexpr int KS = D / 32;  // matrix instructions of a score, words of a lane's value row
   constexpr int DPL = D / 16;  // elements of a lane's value row
   extern __shared__ int s_first[];
-  __shared__ int red[kPagedWaves];
+  __shared__ int red[WAVES][1];
   __shared__ int s_page[kEntries], s_pos[kEntries];
-  __shared__ float s_m[kPagedWaves][16], s_l[kPagedWaves][16];
-  __shared__ float s_o[kPagedWaves][16][D + 4];
+  __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+  __shared__ float s_o[4][16][D + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int units = a.H * a.tiles;  // of a row
-  const unsigned total = (unsigned)scan_rows<kPagedThreads>(a.B, [&](int b) { return row_steps(a, b); }, s_first, red) * (unsigned)units;
-  const unsigned whole = total / (unsigned)a.n_wg, rest = total % (unsigned)a.n_wg;
-  const unsigned begin = start_of(blockIdx.x, whole, rest), end = start_of(blockIdx.x + 1, whole, rest);
+  unsigned whole = 0, rest = 0, begin = 0, end = 1;
+  if constexpr (!WHOLE) {
+    scan_rows<THREADS, 1>(a.B, [&](int b, int (&x)[1]) { x[0] = row_steps<STEP>(a, row_length(a, b)); }, {s_first}, red);
+    const unsigned total = (unsigned)s_first[a.B] * (unsigned)units;
+    const unsigned n_wg = min((unsigned)a.n_wg, max(total / kStepsEach, (unsigned)kFewWorkgroups));
+    whole = total / n_wg;
+    rest = total % n_wg;
+    if (blockIdx.x >= n_wg) return;
+    begin = start_of(blockIdx.x, whole, rest);
+    end = start_of(blockIdx.x + 1, whole, rest);
+  }
   unsigned at = begin;
   const int size = 1 << a.table.shift;
   while (at < end) {
     // the (row, head) that the stretch is in, and which of its steps
-    int b = row_of(s_first, a.B, (int)(at / (unsigned)units));
-    b = __builtin_amdgcn_readfirstlane(b);
-    const unsigned row0 = (unsigned)s_first[b] * units, steps = (unsigned)__builtin_amdgcn_readfirstlane(s_first[b + 1] - s_first[b]);
-    const unsigned unit = __builtin_amdgcn_readfirstlane((at - row0) / steps);
-    const unsigned unit0 = row0 + unit * steps, upto = min(end, unit0 + steps);
+    int b, len;
+    unsigned unit, unit0, steps, upto;
+    if constexpr (WHOLE) {
+      b = blockIdx.x / units;
+      unit = blockIdx.x % units;
+      len = row_length(a, b);
+      steps = row_steps<STEP>(a, len);
+      unit0 = 0;
+      upto = steps;
+    } else {
+      b = __builtin_amdgcn_readfirstlane(row_of(s_first, a.B, (int)(at / (unsigned)units)));
+      len = row_length(a, b);
+      const unsigned row0 = (unsigned)s_first[b] * units;
+      steps = (unsigned)__builtin_amdgcn_readfirstlane(s_first[b + 1] - s_first[b]);
+      unit = __builtin_amdgcn_readfirstlane((at - row0) / steps);
+      unit0 = row0 + unit * steps;
+      upto = min(end, unit0 + steps);
+    }
     const int h = (int)unit / a.tiles, tile = (int)unit % a.tiles;
     const int heads = min(a.G - tile * 16, 16);  // query heads of this unit
     const long long head0 = (long long)b * a.H * a.G + h * a.G + tile * 16;
-    const int len = row_length(a, b), low = a.window > 0 ? max(len - a.window, 0) : 0, key0 = a.pages != nullptr ? 0 : first_key(a, len);
+    const int low = a.window > 0 ? max(len - a.window, 0) : 0, key0 = a.pages != nullptr ? 0 : first_key(a, len);
     u32x4 q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -554,16 +609,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs
     for (int i = 0; i < DPL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
     const int n_entries = a.pages != nullptr ? a.count : pages_of(len, a.table.shift);
-    // kEntries pages at a time; a step's keys lie in the entries of one such chunk (both are powers of two and key0 is cut off below)
+    // kEntries pages at a time
     unsigned step = at - unit0;
     const unsigned step_end = upto - unit0;
     while (step < step_end) {
-      const int from_key = key0 + (int)step * kStepKeys, entry0 = from_key >> a.table.shift;
-      const unsigned fit = (unsigned)(((entry0 + kEntries) << a.table.shift) - from_key) / kStepKeys;
+      const int from_key = key0 + (int)step * STEP, entry0 = from_key >> a.table.shift;
+      const unsigned fit = (unsigned)(((entry0 + kEntries) << a.table.shift) - from_key) / STEP;
       const unsigned chunk_end = min(step_end, step + fit);
-      const int n_here = min(((key0 + (int)chunk_end * kStepKeys - 1) >> a.table.shift) - entry0 + 1, kEntries);
+      const int n_here = min(((key0 + (int)chunk_end * STEP - 1) >> a.table.shift) - entry0 + 1, kEntries);
       __syncthreads();  // (the entries of the chunk before have been read)
-      for (int i = tid; i < n_here; i += kPagedThreads) {
+      for (int i = tid; i < n_here; i += THREADS) {
         const int e = entry0 + i;
         int logical = e < n_entries ? e : -1;
         if (a.pages != nullptr && logical >= 0) logical = a.pages[((long long)b * a.H + h) * a.count + e];
@@ -576,7 +631,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs
       KeyTile<D> tiles[2];
       int pos[2][2];
       auto load = [&](KeyTile<D>& x, int (&p)[2], unsigned s) {
-        const int key = key0 + (int)s * kStepKeys + wave * 32;
+        const int key = key0 + (int)s * STEP + wave * 32;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int kt = key + 16 * t, e = (kt >> a.table.shift) - entry0, off = kt & (size - 1);
@@ -585,7 +640,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs
           const unsigned short* kp = a.k.ptr + page * a.k.sp + (off * a.k.st + h * a.k.sh);
           const unsigned short* vp = a.v.ptr + page * a.v.sp + (off * a.v.st + h * a.v.sh);
 #pragma unroll
-          for (int i = 0; i < KS; ++i) x.k[t][i] = *(const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8));
+          for (int i = 0; i < KS; ++i) x.k[t][i] = __builtin_nontemporal_load((const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8)));
 #pragma unroll
           for (int j = 0; j < 4; ++j) load_values<D>(x.v[4 * t + j], vp + ((4 * grp + j) * a.v.st + col * DPL));
         }
@@ -654,7 +709,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs
       step = chunk_end;
     }
 
-    // the four waves' parts
+    // the waves' parts
     l += __shfl_xor(l, 16, 64);
     l = half_sum(l);
     __syncthreads();  // (the sums of the unit before have been read)
@@ -665,29 +720,45 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs
     __syncthreads();
     float most = RA_NEG_INF;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) most = fmaxf(most, s_m[w][col]);
+    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, s_m[w][col]);
     const float mine = m == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(m - most);
-    if (col < heads) {
+    float* my_o = &s_o[wave & 3][col][4 * grp * DPL];
+    if (wave < 4 && col < heads) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < DPL; ++i) s_o[wave][col][(4 * grp + r) * DPL + i] = o[i][r] * mine;
+        for (int i = 0; i < DPL; ++i) my_o[r * DPL + i] = o[i][r] * mine;
     }
     __syncthreads();
+    if constexpr (WAVES > 4) {
+      if (wave >= 4 && col < heads) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) my_o[r * DPL + i] += o[i][r] * mine;
+      }
+      __syncthreads();
+    }
     const bool complete = at == unit0 && upto == unit0 + steps;
     const long long slot = 2ll * blockIdx.x + (at != begin);
-    for (int i = tid; i < heads * (D / 2); i += kPagedThreads) {
+    if (!WHOLE && at == unit0 && tid == 0) {
+      // where the join finds the parts: a workgroup's first unit has its first place, so all but the first part lie in even ones
+      const unsigned last = complete ? blockIdx.x : holder_of(unit0 + steps - 1, whole, rest);
+      a.where[b * units + (int)unit] = make_int2((int)slot, (int)(last - blockIdx.x) + 1);
+    }
+    for (int i = tid; i < heads * (D / 2); i += THREADS) {
       const int r = i / (D / 2), d = 2 * (i % (D / 2));
       float top = RA_NEG_INF, sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, s_m[w][r]);
+      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, s_m[w][r]);
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w) {
-        sum += s_l[w][r] * (s_m[w][r] == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+      for (int w = 0; w < WAVES; ++w) sum += s_l[w][r] * (s_m[w][r] == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
         x += s_o[w][r][d];
         y += s_o[w][r][d + 1];
       }
-      if (complete) {
+      if (WHOLE || complete) {
         // (a row without a key has a sum of 0; scores that are not numbers are in no maximum, but in the sum)
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         *(unsigned*)(a.out + (head0 + r) * D + d) = down2<T>(x * inv, y * inv);
@@ -696,71 +767,55 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(const PagedArgs
         float* p = a.part + (slot * kPartRows + r) * D + d;
         p[0] = x;
         p[1] = y;
-        if (d == 0) {
-          float* stats = a.part + 2ll * a.n_wg * kPartRows * D;
-          stats[slot * kPartRows + r] = top;
-          stats[2ll * a.n_wg * kPartRows + slot * kPartRows + r] = sum;
-        }
+        if (d == 0) a.stats[slot * kPartRows + r] = make_float2(top, sum);
       }
     }
-    at = upto;
+    at = WHOLE ? end : upto;
   }
 }
 
-// The parts of a (row, query head): a workgroup each, threads on neighbouring elements and on different parts.
+// The parts of a (row, query head): a workgroup each, threads on neighbouring elements and on different parts.  Latency bound: a part's statistics and
+// its elements are on their way together, for 64 parts at a time.
 template <class T, int D>
 __global__ __launch_bounds__(256) void join_kernel(const PagedArgs a) {
-  constexpr int COLS = D / 4, GROUPS = 256 / COLS;
-  extern __shared__ int s_mem[];
-  __shared__ int red[4];
-  __shared__ float s_red[4], s_sum[GROUPS][D];
-  int* s_first = s_mem;
-  float* s_w = (float*)(s_mem + a.B + 1);  // a weight a part
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int units = a.H * a.tiles;
-  const unsigned total = (unsigned)scan_rows<256>(a.B, [&](int b) { return row_steps(a, b); }, s_first, red) * (unsigned)units;
-  const unsigned whole = total / (unsigned)a.n_wg, rest = total % (unsigned)a.n_wg;
+  constexpr int COLS = D / 4, GROUPS = 256 / COLS, MOST = (64 + GROUPS - 1) / GROUPS;
+  __shared__ float s_sum[GROUPS][D];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.y, head = blockIdx.x, h = head / a.G, g = head % a.G, r = g % 16;
-  const unsigned steps = (unsigned)(s_first[b + 1] - s_first[b]);
-  const unsigned unit0 = (unsigned)s_first[b] * units + (unsigned)(h * a.tiles + g / 16) * steps;
-  const unsigned w0 = holder_of(unit0, whole, rest), w1 = holder_of(unit0 + steps - 1, whole, rest);
-  if (w0 == w1) return;
-  const int parts = (int)(w1 - w0) + 1;
-  // a workgroup's first unit has its first place
-  const long long slot0 = 2ll * w0 + (start_of(w0, whole, rest) < unit0);
-  auto slot_of = [&](int i) { return i == 0 ? slot0 : 2ll * (w0 + i); };
-  const float* maxima = a.part + 2ll * a.n_wg * kPartRows * D;
-  const float* sums = maxima + 2ll * a.n_wg * kPartRows;
-  float top = RA_NEG_INF;
-  for (int i = tid; i < parts; i += 256) {
-    const float x = maxima[slot_of(i) * kPartRows + r];
-    s_w[i] = x;
-    top = fmaxf(top, x);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  if (lane == 0) s_red[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  float sum = 0.f;
-  for (int i = tid; i < parts; i += 256) {
-    const float w = s_w[i] == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_w[i] - top);
-    s_w[i] = w;
-    sum += w * sums[slot_of(i) * kPartRows + r];
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  __syncthreads();
-  if (lane == 0) s_red[wave] = sum;
-  __syncthreads();
-  sum = s_red[0] + s_red[1] + s_red[2] + s_red[3];
+  const int2 where = a.where[b * a.H * a.tiles + h * a.tiles + g / 16];
+  const int parts = where.y;
+  if (parts <= 1) return;
+  auto place = [&](int i) { return (long long)(i == 0 ? where.x : (where.x & ~1) + 2 * i) * kPartRows + r; };
   const int c = tid % COLS, p0 = tid / COLS;
+  float top = RA_NEG_INF, sum = 0.f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  if (p0 < GROUPS) {
-#pragma unroll 8
-    for (int i = p0; i < parts; i += GROUPS) x += s_w[i] * *(const f32x4*)(a.part + (slot_of(i) * kPartRows + r) * D + 4 * c);
-    *(f32x4*)&s_sum[p0][4 * c] = x;
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    const int n = min(parts - i0, 64);
+    const float2 st = a.stats[place(i0 + min(lane, n - 1))];
+    f32x4 y[MOST];
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) {
+      const int i = p0 + j * GROUPS;
+      y[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (p0 < GROUPS && i < n) y[j] = *(const f32x4*)(a.part + place(i0 + i) * D + 4 * c);
+    }
+    float next = lane < n ? st.x : RA_NEG_INF;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) next = fmaxf(next, __shfl_xor(next, o, 64));
+    next = fmaxf(next, top);
+    const float keep = top == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(top - next);
+    const float w = lane < n && st.x != RA_NEG_INF ? __builtin_amdgcn_exp2f(st.x - next) : 0.f;
+    float s = lane < n ? w * st.y : 0.f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    // (what is not a number stays so under a weight of 0)
+    sum = sum * keep + s;
+    x *= keep;
+    top = next;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) x += __shfl(w, (p0 + j * GROUPS) & 63, 64) * y[j];
   }
+  if (p0 < GROUPS) *(f32x4*)&s_sum[p0][4 * c] = x;
   __syncthreads();
   const long long at = (long long)b * a.H * a.G + head;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -776,30 +831,44 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedArgs a) {
   if (tid == 0) a.lse[at] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
 }
 
-int paged_workgroups(long long most_steps) { return (int)(most_steps < 512 ? most_steps : 512); }
-long long paged_part_floats(int n_wg, int D) { return 2ll * n_wg * kPartRows * (D + 2); }
+// The workspace: parts, their statistics, and where those of each (row, head) are.
+static long long part_bytes(int n_wg, int D) { return 2ll * n_wg * kPartRows * D * (long long)sizeof(float); }
+static long long stat_bytes(int n_wg) { return 2ll * n_wg * kPartRows * (long long)sizeof(float2); }
+PagedShape paged_shape(long long keys, long long units, int D) {
+  const long long steps = (keys + kStepKeys - 1) / kStepKeys, most = steps * units;
+  if (keys <= kWholeKeys) return {(int)units, true, 0};
+  const int n_wg = (int)(most < kPagedWorkgroups ? most : kPagedWorkgroups);
+  return {n_wg, false, part_bytes(n_wg, D) + stat_bytes(n_wg) + units * (long long)sizeof(int2)};
+}
 
-template <class T, int D>
-static hipError_t launch_paged_of(const PagedArgs& a, bool one_step, hipStream_t stream) {
-  const size_t shared = (a.B + 1) * sizeof(int);
-  if (a.slopes != nullptr) hipLaunchKernelGGL((paged_kernel<T, D, true>), dim3(a.n_wg), dim3(kPagedThreads), shared, stream, a);
-  else hipLaunchKernelGGL((paged_kernel<T, D, false>), dim3(a.n_wg), dim3(kPagedThreads), shared, stream, a);
+template <class T, int D, bool ALIBI>
+static hipError_t launch_paged_of(PagedArgs& a, const PagedShape& shape, void* workspace, hipStream_t stream) {
+  a.n_wg = shape.workgroups;
+  if (shape.whole) {
+    hipLaunchKernelGGL((paged_kernel<T, D, ALIBI, true>), dim3(a.n_wg), dim3(512), 0, stream, a);
+    return hipGetLastError();
+  }
+  a.part = static_cast<float*>(workspace);
+  a.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + part_bytes(a.n_wg, D));
+  a.where = reinterpret_cast<int2*>(static_cast<char*>(workspace) + part_bytes(a.n_wg, D) + stat_bytes(a.n_wg));
+  hipLaunchKernelGGL((paged_kernel<T, D, ALIBI, false>), dim3(a.n_wg), dim3(256), (a.B + 1) * sizeof(int), stream, a);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || one_step) return e;
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3(a.H * a.G, a.B), dim3(256), shared + a.n_wg * sizeof(float), stream, a);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3(a.H * a.G, a.B), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 template <class T>
-static hipError_t launch_paged_type(const PagedArgs& a, int D, bool one_step, hipStream_t stream) {
+static hipError_t launch_paged_type(PagedArgs& a, int D, const PagedShape& shape, void* workspace, hipStream_t stream) {
+  const bool alibi = a.slopes != nullptr;
   switch (D) {
-    case 32: return launch_paged_of<T, 32>(a, one_step, stream);
-    case 64: return launch_paged_of<T, 64>(a, one_step, stream);
-    case 96: return launch_paged_of<T, 96>(a, one_step, stream);
-    default: return launch_paged_of<T, 128>(a, one_step, stream);
+    case 32: return alibi ? launch_paged_of<T, 32, true>(a, shape, workspace, stream) : launch_paged_of<T, 32, false>(a, shape, workspace, stream);
+    case 64: return alibi ? launch_paged_of<T, 64, true>(a, shape, workspace, stream) : launch_paged_of<T, 64, false>(a, shape, workspace, stream);
+    case 96: return alibi ? launch_paged_of<T, 96, true>(a, shape, workspace, stream) : launch_paged_of<T, 96, false>(a, shape, workspace, stream);
+    default: return alibi ? launch_paged_of<T, 128, true>(a, shape, workspace, stream) : launch_paged_of<T, 128, false>(a, shape, workspace, stream);
   }
 }
-hipError_t launch_paged(const PagedArgs& a, int D, int dtype, bool one_step, hipStream_t stream) {
-  return dtype == RA_DTYPE_F16 ? launch_paged_type<F16>(a, D, one_step, stream) : launch_paged_type<BF16>(a, D, one_step, stream);
+hipError_t launch_paged(PagedArgs& a, int D, int dtype, const PagedShape& shape, void* workspace, hipStream_t stream) {
+  return dtype == RA_DTYPE_F16 ? launch_paged_type<F16>(a, D, shape, workspace, stream) : launch_paged_type<BF16>(a, D, shape, workspace, stream);
 }
 
 }  // namespace ra

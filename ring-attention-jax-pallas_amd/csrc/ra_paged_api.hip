@@ -77,7 +77,7 @@ int check_lengths(const int32_t* a, const int32_t* b) {
   return misaligned(a, 4) || misaligned(b, 4) ? fail(RA_ERR_ALIGN, "the lengths are not aligned to their elements") : RA_OK;
 }
 
-int paged_args(const ra_paged_params* p, PagedArgs& a, bool& one_step) {
+int paged_args(const ra_paged_params* p, PagedArgs& a, PagedShape& shape) {
   if (!p) return fail(RA_ERR_NULL, "the parameters are NULL");
   if (int e = check_type(p->dtype)) return e;
   if (int e = check_rows(p->B, p->H, p->D)) return e;
@@ -110,8 +110,7 @@ int paged_args(const ra_paged_params* p, PagedArgs& a, bool& one_step) {
   if (!p->pages && p->window > 0 && p->window + 31ll < keys) keys = p->window + 31ll;
   const int64_t steps = (keys + kStepKeys - 1) / kStepKeys, most = steps * p->B * p->H * a.tiles;
   if (most > kMost32) return fail(RA_ERR_TOO_LARGE, "%lld steps of %d keys are too many for one call", (long long)most, kStepKeys);
-  one_step = steps == 1;
-  a.n_wg = paged_workgroups(most);
+  shape = paged_shape(keys, (int64_t)p->B * p->H * a.tiles, p->D);
   return RA_OK;
 }
 
@@ -233,25 +232,22 @@ int ra_select_pages(const void* q, int64_t q_stride_b, int64_t q_stride_h, const
 
 int64_t ra_paged_attention_workspace(const ra_paged_params* p) {
   PagedArgs a;
-  bool one_step;
-  if (paged_args(p, a, one_step) != RA_OK) return 0;  // (the call itself says what is wrong)
-  return one_step ? 0 : paged_part_floats(a.n_wg, p->D) * (int64_t)sizeof(float);
+  PagedShape shape;
+  return paged_args(p, a, shape) == RA_OK ? shape.workspace : 0;  // (the call itself says what is wrong)
 }
 int ra_paged_attention(const ra_paged_params* p, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   PagedArgs a;
-  bool one_step;
-  if (int e = paged_args(p, a, one_step)) return e;
+  PagedShape shape;
+  if (int e = paged_args(p, a, shape)) return e;
   if (!out || !lse) return fail(RA_ERR_NULL, "out or lse is NULL");
   if (misaligned(out, 16) || misaligned(lse, 4)) return fail(RA_ERR_ALIGN, "out must be 16-byte aligned, lse to its elements");
-  if (!one_step) {
-    const int64_t need = paged_part_floats(a.n_wg, p->D) * (int64_t)sizeof(float);
-    if (!workspace || workspace_bytes < need) return fail(RA_ERR_NULL, "a workspace of %lld bytes is needed", (long long)need);
+  if (shape.workspace > 0) {
+    if (!workspace || workspace_bytes < shape.workspace) return fail(RA_ERR_NULL, "a workspace of %lld bytes is needed", shape.workspace);
     if (misaligned(workspace, 16)) return fail(RA_ERR_ALIGN, "the workspace must be 16-byte aligned");
   }
   a.out = static_cast<unsigned short*>(out);
   a.lse = lse;
-  a.part = static_cast<float*>(workspace);
-  return done(launch_paged(a, p->D, p->dtype, one_step, static_cast<hipStream_t>(stream)), "ra_paged_attention");
+  return done(launch_paged(a, p->D, p->dtype, shape, workspace, static_cast<hipStream_t>(stream)), "ra_paged_attention");
 }
 
 }  // extern "C"

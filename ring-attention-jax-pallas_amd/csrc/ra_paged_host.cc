@@ -2,8 +2,10 @@
 // way.  Such calls are small: the slots of a step are 5 us of kernel.
 #include "ra_host.h"
 
+#include <ATen/EmptyTensor.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -37,9 +39,18 @@ PyObject* init(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, const at::Device& device) {
-  return at::empty(shape, at::TensorOptions().dtype(dtype).device(device));
+// Memory of the current device and stream, for a call's results and its workspace; without the dispatcher, which takes as long again (a tensor 1.3 us).
+c10::Allocator* allocator() { return c10::hip::HIPCachingAllocatorMasqueradingAsCUDA::get(); }
+Tensor empty(at::IntArrayRef shape, at::ScalarType dtype) {
+  return at::detail::empty_generic(shape, allocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), dtype, c10::nullopt);
 }
+struct Workspace {
+  c10::DataPtr held;
+  explicit Workspace(int64_t bytes) {
+    if (bytes > 0) held = allocator()->allocate((size_t)bytes);
+  }
+  void* at() const { return held.get(); }
+};
 
 int64_t number_of(PyObject* x, const char* name, int64_t most = INT32_MAX) {
   const int64_t n = THPVariable_Check(x) ? -1 : PyLong_AsLongLong(x);
@@ -142,7 +153,7 @@ PyObject* page_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const ra_page_table t = table_of(c, table, ring.size(0), page_size);
     const int64_t B = table.size(0);
     const Tensor x = ints(c, before, "lengths", B), y = ints(c, after, "new_lengths", B), s = ints(c, state, "free_state", 2);
-    got = {empty({tokens}, at::kLong, c.device), empty({B + 1}, at::kInt, c.device), empty({B}, at::kInt, c.device), empty({2}, at::kInt, c.device)};
+    got = {empty({tokens}, at::kLong), empty({B + 1}, at::kInt), empty({B}, at::kInt), empty({2}, at::kInt)};
     check("ra_page_slots", g_lib.page_slots(&t, x.data_ptr<int32_t>(), y.data_ptr<int32_t>(), (int32_t)B, ring.data_ptr<int32_t>(), s.data_ptr<int32_t>(),
                                             tokens ? got[0].data_ptr<int64_t>() : nullptr, (int32_t)tokens, got[1].data_ptr<int32_t>(),
                                             got[2].data_ptr<int32_t>(), got[3].data_ptr<int32_t>(), stream(c.device)));
@@ -253,14 +264,13 @@ PyObject* select_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     // (the call's own checks come before anything is allocated)
     TORCH_CHECK_VALUE(count > 0 && first + last <= count, "count must be positive and hold the first and last pages (got ", count, ", ", first, ", ", last, ")");
     TORCH_CHECK_VALUE(B * H * count <= INT32_MAX, "too many pages to choose: ", B, " x ", H, " x ", count);
-    pages = empty({B, H, count}, at::kInt, c.device);
+    pages = empty({B, H, count}, at::kInt);
     const int64_t bytes = t.width > count ? g_lib.select_workspace(&t, (int32_t)B, int32_of(H, "heads")) : 0;
-    Tensor work;
-    if (bytes) work = empty({bytes}, at::kByte, c.device);
+    const Workspace work(bytes);
     check("ra_select_pages", g_lib.select_pages(x.data_ptr(), stride_of(x, 0), stride_of(x, 1), means.data_ptr(), stride_of(means, 0), stride_of(means, 1),
                                                 row_dtype(means.scalar_type()), &t, y.data_ptr<int32_t>(), int32_of(B, "block_table"), int32_of(H, "heads"),
                                                 int32_of(x.size(1) / H, "q"), int32_of(x.size(2), "d"), (int32_t)count, (int32_t)first, (int32_t)last,
-                                                pages.data_ptr<int32_t>(), bytes ? work.data_ptr() : nullptr, bytes, stream(c.device)));
+                                                pages.data_ptr<int32_t>(), work.at(), bytes, stream(c.device)));
   }
   return THPVariable_Wrap(std::move(pages));
   END_HANDLE_TH_ERRORS
@@ -316,10 +326,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     p.q_stride_h = stride_of(x, 1);
     p.lengths = y.data_ptr<int32_t>();
     const int64_t bytes = g_lib.attention_workspace(&p);
-    got = {empty({B, x.size(1), D}, type, c.device), empty({B, x.size(1)}, at::kFloat, c.device)};
-    Tensor work;
-    if (bytes) work = empty({bytes}, at::kByte, c.device);
-    check("ra_paged_attention", g_lib.attention(&p, got[0].data_ptr(), got[1].data_ptr<float>(), bytes ? work.data_ptr() : nullptr, bytes, stream(c.device)));
+    got = {empty({B, x.size(1), D}, type), empty({B, x.size(1)}, at::kFloat)};
+    const Workspace work(bytes);
+    check("ra_paged_attention", g_lib.attention(&p, got[0].data_ptr(), got[1].data_ptr<float>(), work.at(), bytes, stream(c.device)));
   }
   return tuple_of(std::move(got));
   END_HANDLE_TH_ERRORS

@@ -76,13 +76,14 @@ def test_attention_rejects_bad_parameters(lib, change, code):
 
 def test_attention_rejects_bad_results_and_workspaces(lib):
     p = _params()
+    p.table.width = p.table.stride_b = 65  # 1040 tokens: shared between workgroups
     need = lib.ra_paged_attention_workspace(C.byref(p))
     assert need > 0
     for args, code in (((None, 0x7000, WORK, need), -1), ((0x6000, None, WORK, need), -1), ((0x6002, 0x7000, WORK, need), -4),
                        ((0x6000, 0x7002, WORK, need), -4), ((0x6000, 0x7000, None, need), -1), ((0x6000, 0x7000, WORK, need - 1), -1),
                        ((0x6000, 0x7000, WORK + 4, need), -4)):
         assert lib.ra_paged_attention(C.byref(p), *args, None) == code
-    p.table.width = p.table.stride_b = 8  # 128 tokens: one step, nothing to join
+    p.table.width = p.table.stride_b = 64  # 1024 tokens are not, and nothing is joined
     assert lib.ra_paged_attention_workspace(C.byref(p)) == 0
     assert lib.ra_paged_attention(None, 0x6000, 0x7000, None, 0, None) == -1
 
