@@ -69,6 +69,7 @@ struct SelectArgs {
   PageTable table;
   const int* lengths;
   int B, H, G, D, count, first, last;
+  int heads;  // of a page in one load (set by the launch)
   unsigned long long* keys;  // [B, H, width]
   int* pages;                // [B, H, count]
 };

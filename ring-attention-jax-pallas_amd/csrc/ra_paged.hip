@@ -33,6 +33,52 @@ RA_DEV unsigned down2(float lo, float hi) {
 
 RA_DEV int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
 
+// A lane's value from the lanes before it, `id` where there is none: 1, 2, 4, 8 lanes back within a row of sixteen, then the last lane of the row
+// and of the half before.  These moves are part of an addition; a shuffle goes through shared memory, ten times as long.
+template <int CTRL, int ROWS = 0xf>
+RA_DEV int lane_before(int id, int x) { return __builtin_amdgcn_update_dpp(id, x, CTRL, ROWS, 0xf, false); }
+RA_DEV int scan_sum(int x) {
+  x += lane_before<0x111>(0, x);
+  x += lane_before<0x112>(0, x);
+  x += lane_before<0x114>(0, x);
+  x += lane_before<0x118>(0, x);
+  x += lane_before<0x142, 0xa>(0, x);
+  x += lane_before<0x143, 0xc>(0, x);
+  return x;
+}
+template <int CTRL, int ROWS = 0xf>
+RA_DEV float float_before(float id, float x) { return __int_as_float(lane_before<CTRL, ROWS>(__float_as_int(id), __float_as_int(x))); }
+RA_DEV float last_lane(float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63)); }
+RA_DEV float sum_of_wave(float x) {
+  x += float_before<0x111>(0.f, x);
+  x += float_before<0x112>(0.f, x);
+  x += float_before<0x114>(0.f, x);
+  x += float_before<0x118>(0.f, x);
+  x += float_before<0x142, 0xa>(0.f, x);
+  x += float_before<0x143, 0xc>(0.f, x);
+  return last_lane(x);
+}
+RA_DEV float max_of_wave(float x) {
+  x = fmaxf(x, float_before<0x111>(RA_NEG_INF, x));
+  x = fmaxf(x, float_before<0x112>(RA_NEG_INF, x));
+  x = fmaxf(x, float_before<0x114>(RA_NEG_INF, x));
+  x = fmaxf(x, float_before<0x118>(RA_NEG_INF, x));
+  x = fmaxf(x, float_before<0x142, 0xa>(RA_NEG_INF, x));
+  x = fmaxf(x, float_before<0x143, 0xc>(RA_NEG_INF, x));
+  return last_lane(x);
+}
+// ... of the four lanes l, l ^ 16, l ^ 32, l ^ 48, in each of them.
+RA_DEV float max_of_rows(float x) {
+  const unsigned u = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+RA_DEV float sum_of_rows(float x) {
+  const unsigned u = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 // Exclusive prefix sums of N values of each row, sums[n][0 .. B] in shared memory, so that whatever walks the rows' items in one line finds an
 // item's row by halving; all NT threads, neighbouring rows in a thread.  `values(row, x)` is called twice where B > NT.
 template <int NT, int N, class F>
@@ -49,12 +95,7 @@ RA_DEV void scan_rows(int B, F values, int* const (&sums)[N], int (&red)[NT / 64
   }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    s[n] = mine[n];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(s[n], o, 64);
-      s[n] += lane >= o ? y : 0;
-    }
+    s[n] = scan_sum(mine[n]);
     if (lane == 63) red[wave][n] = s[n];
   }
   __syncthreads();
@@ -152,20 +193,21 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
     }
     a.slots[t] = slot;
   }
-  for (int i = me; i < min(take, count); i += stride) {
+  // (the rest from other workgroups on: the first one has had the rows)
+  auto from = [&](int third) { return (int)((blockIdx.x + gridDim.x * third / 3) % gridDim.x) * kSlotThreads + tid; };
+  for (int i = from(1); i < min(take, count); i += stride) {
     const int b = row_of(s_take, a.B, i);
     a.table[b * a.table_sb + had_of(b) + i - s_take[b]] = a.ring[ring_at(i)];
   }
-  for (int i = me; i < give; i += stride) {
+  for (int i = from(2); i < give; i += stride) {
     const int b = row_of(s_give, a.B, i);
     a.ring[(int)(((unsigned)ring_at(count) + (unsigned)i) % (unsigned)P)] = a.table[b * a.table_sb + wants_of(b) + i - s_give[b]];
   }
 }
 
 hipError_t launch_slots(const SlotsArgs& a, hipStream_t stream) {
-  const int items = a.n_slots > a.B ? a.n_slots : a.B;
-  const int wgs = items <= kSlotThreads ? 1 : (items + 2 * kSlotThreads - 1) / (2 * kSlotThreads);
-  hipLaunchKernelGGL(slots_kernel, dim3(wgs < 256 ? wgs : 256), dim3(kSlotThreads), 3 * (a.B + 1) * sizeof(int), stream, a);
+  const int items = a.n_slots > a.B ? a.n_slots : a.B, wgs = (items + kSlotThreads - 1) / kSlotThreads;
+  hipLaunchKernelGGL(slots_kernel, dim3(wgs < 512 ? wgs : 512), dim3(kSlotThreads), 3 * (a.B + 1) * sizeof(int), stream, a);
   return hipGetLastError();
 }
 
@@ -290,7 +332,7 @@ hipError_t launch_means(const MeansArgs& args, int dtype, hipStream_t stream) {
 // extreme ranges, so that the order of pages does not depend on the order of a sum.  A score becomes a whole number of the same order.
 // Sixteen lanes (eight, four for narrow heads) read a page's mean in one go, a wave 64 pages; their partial sums are exchanged so that each
 // lane ends with the sums of its own pages.
-constexpr int kScorePages = 256;  // of a workgroup, 64 a wave
+constexpr int kScoreRows = 256;  // (page, head)s of a workgroup, 64 a wave
 constexpr unsigned long long kForced = ~0ull;
 RA_DEV unsigned long long ordered(double x) {
   if (x != x) return kForced - 1;  // (not a number: before every number, as sorting has it)
@@ -315,9 +357,11 @@ template <class T, int D>
 __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   constexpr int LPR = D == 32 ? 4 : (D == 64 ? 8 : 16);  // lanes of a row
   constexpr int RPI = 64 / LPR, ITERS = 64 / RPI;        // rows a load, loads for 64 pages (= LPR)
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63;
-  const int p0 = blockIdx.x * kScorePages + (threadIdx.x >> 6) * 64;
-  const int c = lane % LPR, sub = lane / LPR;
+  // the rows of one load: `hs` heads of a page beside each other, then the next page
+  const int hs = a.heads, pages_i = RPI / hs, pages_w = 64 / hs;
+  const int lane = threadIdx.x & 63, c = lane % LPR, sub = lane / LPR;
+  const int b = blockIdx.z, h = blockIdx.y * hs + sub % hs, sub_page = sub / hs;
+  const int p0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * pages_w;
   const bool in_row = c * 8 < D;
   // the length, the pages and the queries are on their way together
   const int mine = a.table.at[b * a.table.sb + min(p0 + lane, a.table.width - 1)];
@@ -331,20 +375,22 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   u32x4 m[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    const int page = min(max(__shfl(mine, i * RPI + sub, 64), 0), a.table.n_pages - 1);
+    const int page = min(max(__shfl(mine, i * pages_i + sub_page, 64), 0), a.table.n_pages - 1);
     m[i] = *(const u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + (in_row ? c * 8 : 0)));
     if constexpr (D == 96) m[i] = in_row ? m[i] : (u32x4){0, 0, 0, 0};
   }
   double q[8] = {};
   for (int g0 = 0; g0 < a.G; g0 += 4) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < 4; ++g) {
+      if (g0 + g >= a.G) break;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned y = g0 + g < a.G && in_row ? x[g][e] : 0u;
+        const unsigned y = in_row ? x[g][e] : 0u;
         q[2 * e] += (double)T::up((unsigned short)y);
         q[2 * e + 1] += (double)T::up((unsigned short)(y >> 16));
       }
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       if (g0 + 4 < a.G) x[g] = *(const u32x4*)(q_at + (long long)min(g0 + 4 + g, a.G - 1) * a.q_sh);
@@ -360,40 +406,45 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
     }
   }
   exchange<LPR / 2>(s, c);  // (lane c of a row's lanes: the rows of load c)
-  const int p = p0 + c * RPI + sub, page = __shfl(mine, c * RPI + sub, 64);
+  const int in_wave = c * pages_i + sub_page, p = p0 + in_wave, page = __shfl(mine, in_wave, 64);
   if (page < 0 || page >= a.table.n_pages) s[0] = 0.0;
   if (p < n) a.keys[((long long)b * a.H + h) * a.table.width + p] = p < a.first || p >= n - a.last ? kForced : ordered(s[0]);
 }
 
-// The `count` largest of a row's numbers, ties from the lowest index, their indexes in order: the threshold by its digits of twelve bits from the
-// top, until all that share the digits found so far are taken; then every wave places what it takes of its part of the row.  Twelve bits: the
-// first digit is a double's sign and exponent, and the second mostly settles it.  HELD: the row's numbers stay in registers, kHeld of a thread.
-constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kHeld = 8, kDigitBits = 12, kDigits = 1 << kDigitBits;
-template <bool HELD>
-__global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
-  __shared__ int s_hist[kDigits], s_pick[3], s_above[kSelectWaves], s_equal[kSelectWaves];
+// The `count` largest of a row's numbers, ties from the lowest place, their places in order: the threshold by its digits of twelve bits (ten
+// for few numbers) from the top, until all that share the digits found so far are taken; then every wave places what it takes of its part of the
+// row.  Twelve bits: the first digit is a double's sign and exponent, and the second mostly settles it.  Bound by latency: some ten
+// barriers, and few numbers between them.  HELD: the row's numbers stay in registers, kHeld of a thread.
+constexpr int kHeld = 8;
+template <int NT, bool HELD>
+__global__ __launch_bounds__(NT) void select_kernel(const SelectArgs a) {
+  constexpr int WAVES = NT / 64, kDigitBits = NT > 256 ? 12 : 10, kDigits = 1 << kDigitBits, DPT = kDigits / NT;
+  __shared__ int s_hist[kDigits], s_pick[3], s_above[WAVES], s_equal[WAVES];
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = pages_of(min(max(a.lengths[b], 0), a.table.width << a.table.shift), a.table.shift);
-  int* out = a.pages + ((long long)b * a.H + h) * a.count;
-  if (n <= a.count) {
-    for (int i = tid; i < a.count; i += kSelectThreads) out[i] = i < n ? i : -1;
-    return;
-  }
-  const unsigned long long* keys = a.keys + ((long long)b * a.H + h) * a.table.width;
-  const int rounds = (n + kSelectThreads - 1) / kSelectThreads, part = rounds * 64, from = wave * part + lane, to = min(wave * part + part, n);
+  const int width = a.table.width;
+  const unsigned long long* keys = a.keys + ((long long)b * a.H + h) * width;
+  // a wave's part of the table's width: its numbers are on their way together with the length
+  const int rounds = (width + NT - 1) / NT, part = rounds * 64, from = wave * part + lane;
   unsigned long long held[kHeld];
   if constexpr (HELD) {
 #pragma unroll
-    for (int r = 0; r < kHeld; ++r) held[r] = r < rounds && from + 64 * r < to ? keys[from + 64 * r] : 0;
+    for (int r = 0; r < kHeld; ++r) held[r] = width > a.count ? keys[min(from + 64 * r, width - 1)] : 0;  // (else there is no workspace)
   }
-  // every number of this thread: place, number
+  const int n = pages_of(min(max(a.lengths[b], 0), width << a.table.shift), a.table.shift);
+  int* out = a.pages + ((long long)b * a.H + h) * a.count;
+  if (n <= a.count) {
+    for (int i = tid; i < a.count; i += NT) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int to = min(wave * part + part, n);
+  // every number of this thread: place, number (places from `to` on: whatever lies there)
   auto each = [&](auto&& use) {
     if constexpr (HELD) {
 #pragma unroll
       for (int r = 0; r < kHeld; ++r)
         if (r < rounds) use(from + 64 * r, held[r]);
     } else {
-      for (int r = 0; r < rounds; ++r) use(from + 64 * r, from + 64 * r < to ? keys[from + 64 * r] : 0ull);
+      for (int r = 0; r < rounds && from - lane + 64 * r < n; ++r) use(from + 64 * r, keys[min(from + 64 * r, width - 1)]);
     }
   };
   // `known` bits from the top are those of the threshold; `need` of the numbers that have them are to be taken
@@ -402,39 +453,35 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   while (known < 64 && need < sharing) {
     const int bits = min(kDigitBits, 64 - known), down = 64 - known - bits;
 #pragma unroll
-    for (int i = 0; i < kDigits / kSelectThreads; ++i) s_hist[tid + i * kSelectThreads] = 0;
+    for (int i = 0; i < DPT; ++i) s_hist[tid + i * NT] = 0;
     __syncthreads();
     each([&](int i, unsigned long long x) {
       if (i < to && (x & mask) == top) atomicAdd(&s_hist[(int)(x >> down) & ((1 << bits) - 1)], 1);
     });
     __syncthreads();
-    // four digits a thread, from the highest; sums within a wave, then over the waves before it
-    constexpr int DPT = kDigits / kSelectThreads;
+    // digits from the highest, neighbours in a thread; sums within a wave, then over the waves before it
     int c[DPT], sum = 0;
 #pragma unroll
     for (int e = 0; e < DPT; ++e) {
       c[e] = s_hist[kDigits - 1 - DPT * tid - e];
       sum += c[e];
     }
-    int upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o, 64);
-      upto += lane >= o ? y : 0;
-    }
+    const int upto = scan_sum(sum);
     if (lane == 63) s_above[wave] = upto;
     __syncthreads();
     int above = upto - sum;
 #pragma unroll
-    for (int w = 0; w < kSelectWaves; ++w) above += w < wave ? s_above[w] : 0;
+    for (int w = 0; w < WAVES; ++w) above += w < wave ? s_above[w] : 0;
+    if (above < need && above + sum >= need) {
 #pragma unroll
-    for (int e = 0; e < DPT; ++e) {
-      if (above < need && above + c[e] >= need) {
-        s_pick[0] = kDigits - 1 - DPT * tid - e;
-        s_pick[1] = above;
-        s_pick[2] = c[e];
+      for (int e = 0; e < DPT; ++e) {
+        if (above < need && above + c[e] >= need) {
+          s_pick[0] = kDigits - 1 - DPT * tid - e;
+          s_pick[1] = above;
+          s_pick[2] = c[e];
+        }
+        above += c[e];
       }
-      above += c[e];
     }
     __syncthreads();
     need -= s_pick[1];
@@ -456,7 +503,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   __syncthreads();
   above = equal = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     above += w < wave ? s_above[w] : 0;
     equal += w < wave ? s_equal[w] : 0;
   }
@@ -472,8 +519,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
 }
 
 template <class T>
-static void launch_score(const SelectArgs& a, hipStream_t stream) {
-  const dim3 grid((a.table.width + kScorePages - 1) / kScorePages, a.H, a.B);
+static void launch_score(const SelectArgs& args, hipStream_t stream) {
+  SelectArgs a = args;
+  // as many heads of a page in one load as its rows hold and as divide the heads (means of neighbouring heads mostly lie side by side)
+  a.heads = a.D == 32 ? 16 : (a.D == 64 ? 8 : 4);
+  while (a.H % a.heads != 0) a.heads /= 2;
+  const int pages = kScoreRows / a.heads;
+  const dim3 grid((a.table.width + pages - 1) / pages, a.H / a.heads, a.B);
   void (*kernel)(SelectArgs) = a.D == 32 ? score_kernel<T, 32> : a.D == 64 ? score_kernel<T, 64> : a.D == 96 ? score_kernel<T, 96> : score_kernel<T, 128>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
 }
@@ -484,8 +536,11 @@ hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  void (*kernel)(SelectArgs) = a.table.width <= kHeld * kSelectThreads ? select_kernel<true> : select_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3(a.H, a.B), dim3(kSelectThreads), 0, stream, a);
+  // (four waves pass a barrier sooner than sixteen)
+  if (a.table.width <= kHeld * 256) hipLaunchKernelGGL((select_kernel<256, true>), dim3(a.H, a.B), dim3(256), 0, stream, a);
+  else if (a.table.width <= kHeld * 512) hipLaunchKernelGGL((select_kernel<512, true>), dim3(a.H, a.B), dim3(512), 0, stream, a);
+  else if (a.table.width <= kHeld * 1024) hipLaunchKernelGGL((select_kernel<1024, true>), dim3(a.H, a.B), dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL((select_kernel<1024, false>), dim3(a.H, a.B), dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -495,8 +550,8 @@ hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
 // The work of a call is one line of steps of 128 keys: row by row of the batch, head by head of the cache, along the sequence.  Every workgroup
 // takes an equal stretch of it, so that rows of any lengths load the chip evenly; lengths are on the device, and each workgroup makes the
 // line's prefix sums for itself.  A stretch that holds a (row, head) whole stores its output; parts of one go to memory as (maximum, sum,
-// unnormalised output) in 32 bits and are joined by a second kernel.  Where no row is longer than kWholeKeys (by the table), a workgroup of eight
-// waves takes each (row, head) whole, and that is all.
+// unnormalised output) in 32 bits and are joined by a second kernel.  Where no row is longer than kWholeKeys (by the table), a workgroup of
+// eight waves takes each (row, head) whole, and that is all.
 RA_DEV int first_key(const PagedArgs& a, int len) { return a.window > 0 ? max(len - a.window, 0) & ~31 : 0; }
 RA_DEV int row_length(const PagedArgs& a, int b) { return min(max(a.lengths[b], 0), a.table.width << a.table.shift); }
 template <int STEP>
@@ -556,7 +611,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
   __shared__ int red[WAVES][1];
   __shared__ int s_page[kEntries], s_pos[kEntries];
   __shared__ float s_m[WAVES][16], s_l[WAVES][16];
-  __shared__ float s_o[4][16][D + 4];
+  __shared__ float s_o[WAVES][16][D + 4];  // elements in the order of the lanes' registers: 16 i + m is element m D / 16 + i
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int units = a.H * a.tiles;  // of a row
@@ -578,8 +633,8 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
     int b, len;
     unsigned unit, unit0, steps, upto;
     if constexpr (WHOLE) {
-      b = blockIdx.x / units;
-      unit = blockIdx.x % units;
+      b = blockIdx.y;
+      unit = blockIdx.x;
       len = row_length(a, b);
       steps = row_steps<STEP>(a, len);
       unit0 = 0;
@@ -593,7 +648,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
       unit0 = row0 + unit * steps;
       upto = min(end, unit0 + steps);
     }
-    const int h = (int)unit / a.tiles, tile = (int)unit % a.tiles;
+    const int h = a.tiles == 1 ? (int)unit : (int)unit / a.tiles, tile = (int)unit - h * a.tiles;
     const int heads = min(a.G - tile * 16, 16);  // query heads of this unit
     const long long head0 = (long long)b * a.H * a.G + h * a.G + tile * 16;
     const int low = a.window > 0 ? max(len - a.window, 0) : 0, key0 = a.pages != nullptr ? 0 : first_key(a, len);
@@ -628,27 +683,35 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
         s_pos[i] = there ? logical << a.table.shift : kNowhere;
       }
       __syncthreads();
-      KeyTile<D> tiles[2];
-      int pos[2][2];
-      auto load = [&](KeyTile<D>& x, int (&p)[2], unsigned s) {
+      // A step's keys are replaced by the next one's as soon as the scores are made, its values after the product with the weights: one is
+      // always on its way while the other is used, in the registers of a single step.
+      KeyTile<D> x;
+      int p[2];
+      auto load = [&](unsigned s, bool values) {
         const int key = key0 + (int)s * STEP + wave * 32;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int kt = key + 16 * t, e = (kt >> a.table.shift) - entry0, off = kt & (size - 1);
-          const int page = __builtin_amdgcn_readfirstlane(s_page[e]);
-          p[t] = __builtin_amdgcn_readfirstlane(s_pos[e]) + off;
-          const unsigned short* kp = a.k.ptr + page * a.k.sp + (off * a.k.st + h * a.k.sh);
-          const unsigned short* vp = a.v.ptr + page * a.v.sp + (off * a.v.st + h * a.v.sh);
+          const int kt = key + 16 * t, off = kt & (size - 1);
+          const long long page = __builtin_amdgcn_readfirstlane(s_page[(kt >> a.table.shift) - entry0]);
+          if (values) {
+            const unsigned short* vp = a.v.ptr + page * a.v.sp + (off * a.v.st + h * a.v.sh);
 #pragma unroll
-          for (int i = 0; i < KS; ++i) x.k[t][i] = __builtin_nontemporal_load((const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8)));
+            for (int j = 0; j < 4; ++j) load_values<D>(x.v[4 * t + j], vp + ((4 * grp + j) * a.v.st + col * DPL));
+          } else {
+            const unsigned short* kp = a.k.ptr + page * a.k.sp + (off * a.k.st + h * a.k.sh);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) load_values<D>(x.v[4 * t + j], vp + ((4 * grp + j) * a.v.st + col * DPL));
+            for (int i = 0; i < KS; ++i) x.k[t][i] = __builtin_nontemporal_load((const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8)));
+          }
         }
       };
-      auto use = [&](KeyTile<D>& x, const int (&p)[2]) {
-        const bool live = (p[0] < len && p[0] + 16 > low) || (p[1] < len && p[1] + 16 > low);
-        if (!live) return;
-        const bool inside = p[0] >= low && p[0] + 16 <= len && p[1] >= low && p[1] + 16 <= len;
+      load(step, false);
+      load(step, true);
+      for (; step < chunk_end; ++step) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int kt = key0 + (int)step * STEP + wave * 32 + 16 * t;
+          p[t] = __builtin_amdgcn_readfirstlane(s_pos[(kt >> a.table.shift) - entry0]) + (kt & (size - 1));
+        }
         float w[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -661,6 +724,8 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
             if constexpr (ALIBI) w[4 * t + r] -= slope * (float)(len - 1 - p[t] - 4 * grp - r);
           }
         }
+        if (step + 1 < chunk_end) load(step + 1, false);
+        const bool inside = p[0] >= low && p[0] + 16 <= len && p[1] >= low && p[1] + 16 <= len;
         if (!inside) {
           // What is masked may hold anything: its score is replaced, and its value too (0 times infinity is not 0).
 #pragma unroll
@@ -673,8 +738,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           }
         }
         float top = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = half_max(top);
+        top = max_of_rows(top);
         if (__any(top > m)) {
           const float next = fmaxf(m, top), keep = next == RA_NEG_INF ? 1.f : __builtin_amdgcn_exp2f(m - next);
           m = next;
@@ -689,56 +753,34 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           l += w[j];
         }
         const u32x4 wb = {down2<T>(w[0], w[1]), down2<T>(w[2], w[3]), down2<T>(w[4], w[5]), down2<T>(w[6], w[7])};
+        // What the rounded weights lack of theirs goes through the matrix unit as well, which has the time: the output is off by its own rounding.
+        u32x4 wr;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wr[j] = down2<T>(w[2 * j] - T::up((unsigned short)wb[j]), w[2 * j + 1] - T::up((unsigned short)(wb[j] >> 16)));
 #pragma unroll
         for (int i = 0; i < DPL; ++i) {
           const unsigned pick = i & 1 ? 0x07060302u : 0x05040100u;
           u32x4 vt;
 #pragma unroll
           for (int j = 0; j < 4; ++j) vt[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i >> 1], x.v[2 * j][i >> 1], pick);
-          o[i] = T::mfma(vt, wb, o[i]);
+          o[i] = T::mfma(vt, wr, T::mfma(vt, wb, o[i]));
         }
-      };
-      load(tiles[0], pos[0], step);
-      for (; step < chunk_end; step += 2) {
-        if (step + 1 < chunk_end) load(tiles[1], pos[1], step + 1);
-        use(tiles[0], pos[0]);
-        if (step + 1 >= chunk_end) break;
-        if (step + 2 < chunk_end) load(tiles[0], pos[0], step + 2);
-        use(tiles[1], pos[1]);
+        if (step + 1 < chunk_end) load(step + 1, true);
       }
-      step = chunk_end;
     }
 
-    // the waves' parts
-    l += __shfl_xor(l, 16, 64);
-    l = half_sum(l);
+    // The waves' parts.  What runs once is short: its instructions come from memory, and take longer than what they do.
+    l = sum_of_rows(l);
     __syncthreads();  // (the sums of the unit before have been read)
     if (grp == 0) {
       s_m[wave][col] = m;
       s_l[wave][col] = l;
     }
-    __syncthreads();
-    float most = RA_NEG_INF;
+    if (col < heads) {
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, s_m[w][col]);
-    const float mine = m == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(m - most);
-    float* my_o = &s_o[wave & 3][col][4 * grp * DPL];
-    if (wave < 4 && col < heads) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < DPL; ++i) my_o[r * DPL + i] = o[i][r] * mine;
+      for (int i = 0; i < DPL; ++i) *(f32x4*)&s_o[wave][col][16 * i + 4 * grp] = o[i];
     }
     __syncthreads();
-    if constexpr (WAVES > 4) {
-      if (wave >= 4 && col < heads) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int i = 0; i < DPL; ++i) my_o[r * DPL + i] += o[i][r] * mine;
-      }
-      __syncthreads();
-    }
     const bool complete = at == unit0 && upto == unit0 + steps;
     const long long slot = 2ll * blockIdx.x + (at != begin);
     if (!WHOLE && at == unit0 && tid == 0) {
@@ -748,15 +790,17 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
     }
     for (int i = tid; i < heads * (D / 2); i += THREADS) {
       const int r = i / (D / 2), d = 2 * (i % (D / 2));
+      const int e = (d % DPL) * 16 + d / DPL;
       float top = RA_NEG_INF, sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
+#pragma unroll 4
       for (int w = 0; w < WAVES; ++w) top = fmaxf(top, s_m[w][r]);
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) sum += s_l[w][r] * (s_m[w][r] == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        x += s_o[w][r][d];
-        y += s_o[w][r][d + 1];
+      const float base = top == RA_NEG_INF ? 0.f : top;  // (a wave without a score has a maximum of -inf, and a weight of 0)
+#pragma unroll 4
+      for (int w = 0; w < WAVES; ++w) {
+        const float part = __builtin_amdgcn_exp2f(s_m[w][r] - base);
+        sum += s_l[w][r] * part;
+        x += s_o[w][r][e] * part;
+        y += s_o[w][r][e + 16] * part;
       }
       if (WHOLE || complete) {
         // (a row without a key has a sum of 0; scores that are not numbers are in no maximum, but in the sum)
@@ -799,15 +843,10 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedArgs a) {
       y[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
       if (p0 < GROUPS && i < n) y[j] = *(const f32x4*)(a.part + place(i0 + i) * D + 4 * c);
     }
-    float next = lane < n ? st.x : RA_NEG_INF;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) next = fmaxf(next, __shfl_xor(next, o, 64));
-    next = fmaxf(next, top);
+    const float next = fmaxf(max_of_wave(lane < n ? st.x : RA_NEG_INF), top);
     const float keep = top == RA_NEG_INF ? 0.f : __builtin_amdgcn_exp2f(top - next);
     const float w = lane < n && st.x != RA_NEG_INF ? __builtin_amdgcn_exp2f(st.x - next) : 0.f;
-    float s = lane < n ? w * st.y : 0.f;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    const float s = sum_of_wave(lane < n ? w * st.y : 0.f);
     // (what is not a number stays so under a weight of 0)
     sum = sum * keep + s;
     x *= keep;
@@ -845,7 +884,7 @@ template <class T, int D, bool ALIBI>
 static hipError_t launch_paged_of(PagedArgs& a, const PagedShape& shape, void* workspace, hipStream_t stream) {
   a.n_wg = shape.workgroups;
   if (shape.whole) {
-    hipLaunchKernelGGL((paged_kernel<T, D, ALIBI, true>), dim3(a.n_wg), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((paged_kernel<T, D, ALIBI, true>), dim3(a.H * a.tiles, a.B), dim3(512), 0, stream, a);
     return hipGetLastError();
   }
   a.part = static_cast<float*>(workspace);
