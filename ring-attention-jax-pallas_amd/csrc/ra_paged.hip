@@ -580,22 +580,29 @@ struct KeyTile {
   unsigned v[8][D / 32];
 };
 
-template <int D>
+// STREAM: the caches are not to keep it, as they cannot keep what a large call reads once (64 x 8 heads, 2.06 GB: 341 us against 367); a small one's
+// keys may be there from the step before (1000 x 8 heads: 9.4 us either way from caches, 13.3 with the hint where they would have been in them).
+template <bool STREAM, class V>
+RA_DEV V load_row(const V* at) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(at);
+  return *at;
+}
+template <int D, bool STREAM>
 RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
   if constexpr (D == 128) {
-    const u32x4 x = __builtin_nontemporal_load((const u32x4*)at);
+    const u32x4 x = load_row<STREAM>((const u32x4*)at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = x[i];
   } else if constexpr (D == 96) {
-    const u32x3a x = __builtin_nontemporal_load((const u32x3a*)at);
+    const u32x3a x = load_row<STREAM>((const u32x3a*)at);
 #pragma unroll
     for (int i = 0; i < 3; ++i) v[i] = x[i];
   } else if constexpr (D == 64) {
-    const u32x2a x = __builtin_nontemporal_load((const u32x2a*)at);
+    const u32x2a x = load_row<STREAM>((const u32x2a*)at);
     v[0] = x[0];
     v[1] = x[1];
   } else {
-    v[0] = __builtin_nontemporal_load((const unsigned*)at);
+    v[0] = load_row<STREAM>((const unsigned*)at);
   }
 }
 
@@ -696,11 +703,11 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           if (values) {
             const unsigned short* vp = a.v.ptr + page * a.v.sp + (off * a.v.st + h * a.v.sh);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) load_values<D>(x.v[4 * t + j], vp + ((4 * grp + j) * a.v.st + col * DPL));
+            for (int j = 0; j < 4; ++j) load_values<D, !WHOLE>(x.v[4 * t + j], vp + ((4 * grp + j) * a.v.st + col * DPL));
           } else {
             const unsigned short* kp = a.k.ptr + page * a.k.sp + (off * a.k.st + h * a.k.sh);
 #pragma unroll
-            for (int i = 0; i < KS; ++i) x.k[t][i] = __builtin_nontemporal_load((const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8)));
+            for (int i = 0; i < KS; ++i) x.k[t][i] = load_row<!WHOLE>((const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8)));
           }
         }
       };

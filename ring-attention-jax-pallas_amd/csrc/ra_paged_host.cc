@@ -9,6 +9,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/ring_attention_hip.h"
@@ -80,6 +81,7 @@ struct Call {
   c10::DeviceGuard on;
   explicit Call(const Tensor& t, const char* name) : device(require(t, name)), on(device) {}
   static at::Device require(const Tensor& t, const char* name) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "calls on a paged cache cannot be traced");
     TORCH_CHECK(t.is_cuda(), "a paged cache is on the GPU only: ", name, " must live on a HIP device (there is no CPU fallback)");
     return t.device();
   }

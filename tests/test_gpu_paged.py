@@ -87,9 +87,11 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 1
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("d", [32, 64, 96, 128])
 @pytest.mark.parametrize("heads,group", [(1, 1), (2, 3), (4, 1), (1, 16), (2, 17), (1, 40)])
-def test_attention_at_every_edge(dtype, d, heads, group):
+@pytest.mark.parametrize("columns", [0, 20])
+def test_attention_at_every_edge(dtype, d, heads, group, columns):
+    """Tables of up to 1024 tokens, whose rows a workgroup takes whole, and wider ones, whose rows are shared."""
     size = {1: 16, 2: 64, 4: 128}[heads]
-    c = Cache(EDGES, heads, d, size, dtype, seed=d + group)
+    c = Cache(EDGES, heads, d, size, dtype, seed=d + group, extra_width=columns)
     q = c.queries(heads * group)
     scale = 1 / math.sqrt(d)
     _check_attention(q, c, ra.paged_attention_with_lse(q, c.k, c.v, c.table, c.n), scale)
@@ -432,6 +434,8 @@ def test_refusals():
         attend(q=q.clone().requires_grad_())
     with torch.no_grad():
         attend(q=q.clone().requires_grad_())
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda x: ra.paged_attention(x, c.k, c.v, c.table, c.n), (q,))
     for call in (lambda: ra.write_pages(q[:, :2], q[:, 2:], c.k, c.v.float(), c.n.long()), lambda: ra.write_pages(q[:, :2], q[:1, 2:], c.k, c.v, c.n.long()),
                  lambda: ra.write_pages(q[:, :2], q[:, 2:].float(), c.k, c.v, c.n.long()), lambda: ra.write_pages(q[:, :2], q[:, 2:], c.k, c.v, c.n),
                  lambda: ra.write_pages(q[:, :2], q[:, 2:], c.k[:1].expand(3, -1, -1, -1), c.v[:1].expand(3, -1, -1, -1), c.n.long()),
