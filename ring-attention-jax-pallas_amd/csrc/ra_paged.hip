@@ -606,7 +606,7 @@ RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
   }
 }
 
-constexpr int kEntries = 1024;
+constexpr int kEntries = 1024, kNearRows = 1024;  // of a stretch's pages, of the rows' lengths in shared memory
 constexpr int kNowhere = 0x3fffffff;  // (a position behind every sequence)
 
 template <class T, int D, bool ALIBI, bool WHOLE>
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
   constexpr int DPL = D / 16;  // elements of a lane's value row
   extern __shared__ int s_first[];
   __shared__ int red[WAVES][1];
-  __shared__ int s_page[kEntries], s_pos[kEntries];
+  __shared__ int s_page[kEntries], s_pos[kEntries], s_len[WHOLE ? 1 : kNearRows];
   __shared__ float s_m[WAVES][16], s_l[WAVES][16];
   __shared__ float s_o[WAVES][16][D + 4];  // elements in the order of the lanes' registers: 16 i + m is element m D / 16 + i
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -624,7 +624,14 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
   const int units = a.H * a.tiles;  // of a row
   unsigned whole = 0, rest = 0, begin = 0, end = 1;
   if constexpr (!WHOLE) {
-    scan_rows<THREADS, 1>(a.B, [&](int b, int (&x)[1]) { x[0] = row_steps<STEP>(a, row_length(a, b)); }, {s_first}, red);
+    scan_rows<THREADS, 1>(
+        a.B,
+        [&](int b, int (&x)[1]) {
+          const int len = row_length(a, b);
+          if (b < kNearRows) s_len[b] = len;
+          x[0] = row_steps<STEP>(a, len);
+        },
+        {s_first}, red);
     const unsigned total = (unsigned)s_first[a.B] * (unsigned)units;
     const unsigned n_wg = min((unsigned)a.n_wg, max(total / kStepsEach, (unsigned)kFewWorkgroups));
     whole = total / n_wg;
@@ -648,7 +655,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
       upto = steps;
     } else {
       b = __builtin_amdgcn_readfirstlane(row_of(s_first, a.B, (int)(at / (unsigned)units)));
-      len = row_length(a, b);
+      len = __builtin_amdgcn_readfirstlane(b < kNearRows ? s_len[b] : row_length(a, b));
       const unsigned row0 = (unsigned)s_first[b] * units;
       steps = (unsigned)__builtin_amdgcn_readfirstlane(s_first[b + 1] - s_first[b]);
       unit = __builtin_amdgcn_readfirstlane((at - row0) / steps);
@@ -883,7 +890,9 @@ static long long stat_bytes(int n_wg) { return 2ll * n_wg * kPartRows * (long lo
 PagedShape paged_shape(long long keys, long long units, int D) {
   const long long steps = (keys + kStepKeys - 1) / kStepKeys, most = steps * units;
   if (keys <= kWholeKeys) return {(int)units, true, 0};
-  const int n_wg = (int)(most < kPagedWorkgroups ? most : kPagedWorkgroups);
+  // (as the kernel has it, of the steps that there are at most)
+  const long long wanted = most / kStepsEach > kFewWorkgroups ? most / kStepsEach : kFewWorkgroups, cap = most < kPagedWorkgroups ? most : kPagedWorkgroups;
+  const int n_wg = (int)(wanted < cap ? wanted : cap);
   return {n_wg, false, part_bytes(n_wg, D) + stat_bytes(n_wg) + units * (long long)sizeof(int2)};
 }
 
