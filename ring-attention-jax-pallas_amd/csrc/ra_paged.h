@@ -73,6 +73,8 @@ struct SelectArgs {
   unsigned long long* keys;  // [B, H, width]
   int* pages;                // [B, H, count]
 };
+constexpr int kFewPages = 512;  // by the table: so many scores and the choice among them are one kernel's
+long long select_workspace(int width, long long rows);
 hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream);
 
 struct PagedArgs {

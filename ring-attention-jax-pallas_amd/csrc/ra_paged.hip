@@ -354,61 +354,89 @@ RA_DEV void exchange(double (&s)[N], int lane) {
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
-  constexpr int LPR = D == 32 ? 4 : (D == 64 ? 8 : 16);  // lanes of a row
-  constexpr int RPI = 64 / LPR, ITERS = 64 / RPI;        // rows a load, loads for 64 pages (= LPR)
-  // the rows of one load: `hs` heads of a page beside each other, then the next page
-  const int hs = a.heads, pages_i = RPI / hs, pages_w = 64 / hs;
-  const int lane = threadIdx.x & 63, c = lane % LPR, sub = lane / LPR;
-  const int b = blockIdx.z, h = blockIdx.y * hs + sub % hs, sub_page = sub / hs;
-  const int p0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * pages_w;
-  const bool in_row = c * 8 < D;
-  // the length, the pages and the queries are on their way together
-  const int mine = a.table.at[b * a.table.sb + min(p0 + lane, a.table.width - 1)];
-  const int length = a.lengths[b];
-  const unsigned short* q_at = a.q + b * a.q_sb + (long long)h * a.G * a.q_sh + (in_row ? c * 8 : 0);
-  u32x4 x[4];
+struct Scores {
+  static constexpr int LPR = D == 32 ? 4 : (D == 64 ? 8 : 16);  // lanes of a row
+  static constexpr int RPI = 64 / LPR, ITERS = LPR;             // rows a load, loads for 64 rows
+
+  const SelectArgs& a;
+  const int b, h, c, pages_i, sub_page;  // this lane's head, place in a row, pages a load and which of them
+  const bool in_row;
+  const unsigned short* q_at;
+  u32x4 x[4];  // four of the group's queries
+
+  // `hs` heads from `h0` on, of a page beside each other, then the next page
+  RA_DEV Scores(const SelectArgs& args, int b_, int h0, int hs)
+      : a(args), b(b_), h(h0 + lane() / LPR % hs), c(lane() % LPR), pages_i(RPI / hs), sub_page(lane() / LPR / hs), in_row(c * 8 < D),
+        q_at(args.q + b_ * args.q_sb + (long long)h * args.G * args.q_sh + (in_row ? c * 8 : 0)) {}
+  static RA_DEV int lane() { return threadIdx.x & 63; }
+  RA_DEV void load_queries() {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) x[g] = *(const u32x4*)(q_at + (long long)min(g, a.G - 1) * a.q_sh);
-  const int n = pages_of(min(max(length, 0), a.table.width << a.table.shift), a.table.shift);
-  if (p0 >= n || n <= a.count) return;  // (few pages: all of them, whatever their scores)
-  u32x4 m[ITERS];
-#pragma unroll
-  for (int i = 0; i < ITERS; ++i) {
-    const int page = min(max(__shfl(mine, i * pages_i + sub_page, 64), 0), a.table.n_pages - 1);
-    m[i] = *(const u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + (in_row ? c * 8 : 0)));
-    if constexpr (D == 96) m[i] = in_row ? m[i] : (u32x4){0, 0, 0, 0};
+    for (int g = 0; g < 4; ++g) x[g] = *(const u32x4*)(q_at + (long long)min(g, a.G - 1) * a.q_sh);
   }
-  double q[8] = {};
-  for (int g0 = 0; g0 < a.G; g0 += 4) {
+  // The queries are there from here on: loaded where they are used, each would wait for all of the means.
+  RA_DEV void have_queries() {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (g0 + g >= a.G) break;
+    for (int g = 0; g < 4; ++g) asm volatile("" : "+v"(x[g]));
+  }
+  RA_DEV int page_entry(int p0) const { return a.table.at[b * a.table.sb + min(p0 + lane(), a.table.width - 1)]; }
+
+  // The number of page p0 + in_wave() for head h, of n pages; `mine`: page_entry(p0).
+  RA_DEV int in_wave() const { return c * pages_i + sub_page; }
+  RA_DEV unsigned long long number(int mine, int p0, int n) {
+    u32x4 m[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int page = min(max(__shfl(mine, i * pages_i + sub_page, 64), 0), a.table.n_pages - 1);
+      m[i] = *(const u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + (in_row ? c * 8 : 0)));
+      if constexpr (D == 96) m[i] = in_row ? m[i] : (u32x4){0, 0, 0, 0};
+    }
+    double q[8] = {};
+    for (int g0 = 0; g0 < a.G; g0 += 4) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (g0 + g >= a.G) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned y = in_row ? x[g][e] : 0u;
+          q[2 * e] += (double)T::up((unsigned short)y);
+          q[2 * e + 1] += (double)T::up((unsigned short)(y >> 16));
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (g0 + 4 < a.G) x[g] = *(const u32x4*)(q_at + (long long)min(g0 + 4 + g, a.G - 1) * a.q_sh);
+    }
+    double s[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      s[i] = 0.0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned y = in_row ? x[g][e] : 0u;
-        q[2 * e] += (double)T::up((unsigned short)y);
-        q[2 * e + 1] += (double)T::up((unsigned short)(y >> 16));
+        s[i] = __builtin_fma(q[2 * e], (double)T::up((unsigned short)m[i][e]), s[i]);
+        s[i] = __builtin_fma(q[2 * e + 1], (double)T::up((unsigned short)(m[i][e] >> 16)), s[i]);
       }
     }
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      if (g0 + 4 < a.G) x[g] = *(const u32x4*)(q_at + (long long)min(g0 + 4 + g, a.G - 1) * a.q_sh);
+    exchange<LPR / 2>(s, c);  // (lane c of a row's lanes: the rows of load c)
+    const int p = p0 + in_wave(), page = __shfl(mine, in_wave(), 64);
+    if (page < 0 || page >= a.table.n_pages) s[0] = 0.0;
+    return p < a.first || p >= n - a.last ? kForced : ordered(s[0]);
   }
-  double s[ITERS];
-#pragma unroll
-  for (int i = 0; i < ITERS; ++i) {
-    s[i] = 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[i] = __builtin_fma(q[2 * e], (double)T::up((unsigned short)m[i][e]), s[i]);
-      s[i] = __builtin_fma(q[2 * e + 1], (double)T::up((unsigned short)(m[i][e] >> 16)), s[i]);
-    }
-  }
-  exchange<LPR / 2>(s, c);  // (lane c of a row's lanes: the rows of load c)
-  const int in_wave = c * pages_i + sub_page, p = p0 + in_wave, page = __shfl(mine, in_wave, 64);
-  if (page < 0 || page >= a.table.n_pages) s[0] = 0.0;
-  if (p < n) a.keys[((long long)b * a.H + h) * a.table.width + p] = p < a.first || p >= n - a.last ? kForced : ordered(s[0]);
+};
+RA_DEV int row_pages(const SelectArgs& a, int length) { return pages_of(min(max(length, 0), a.table.width << a.table.shift), a.table.shift); }
+
+template <class T, int D>
+__global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
+  const int hs = a.heads, b = blockIdx.z, p0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / hs);
+  Scores<T, D> scores(a, b, blockIdx.y * hs, hs);
+  // the length, the pages and the queries are on their way together
+  const int mine = scores.page_entry(p0), length = a.lengths[b];
+  scores.load_queries();
+  const int n = row_pages(a, length);
+  scores.have_queries();
+  if (p0 >= n || n <= a.count) return;  // (few pages: all of them, whatever their scores)
+  const unsigned long long x = scores.number(mine, p0, n);
+  const int p = p0 + scores.in_wave();
+  if (p < n) a.keys[((long long)b * a.H + scores.h) * a.table.width + p] = x;
 }
 
 // The `count` largest of a row's numbers, ties from the lowest place, their places in order: the threshold by its digits of twelve bits (ten
@@ -416,27 +444,16 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
 // row.  Twelve bits: the first digit is a double's sign and exponent, and the second mostly settles it.  Bound by latency: some ten
 // barriers, and few numbers between them.  HELD: the row's numbers stay in registers, kHeld of a thread.
 constexpr int kHeld = 8;
-template <int NT, bool HELD>
-__global__ __launch_bounds__(NT) void select_kernel(const SelectArgs a) {
+RA_DEV void take_all(const SelectArgs& a, int* out, int n) {
+  for (int i = threadIdx.x; i < a.count; i += blockDim.x) out[i] = i < n ? i : -1;
+}
+// Of the numbers `load(place)`, places [0, n), n > a.count; a wave has places of its own, `rounds` times 64 of them.
+template <int NT, bool HELD, class Load>
+RA_DEV void choose(const SelectArgs& a, int* out, int n, int rounds, const unsigned long long (&held)[kHeld], Load load) {
   constexpr int WAVES = NT / 64, kDigitBits = NT > 256 ? 12 : 10, kDigits = 1 << kDigitBits, DPT = kDigits / NT;
   __shared__ int s_hist[kDigits], s_pick[3], s_above[WAVES], s_equal[WAVES];
-  const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int width = a.table.width;
-  const unsigned long long* keys = a.keys + ((long long)b * a.H + h) * width;
-  // a wave's part of the table's width: its numbers are on their way together with the length
-  const int rounds = (width + NT - 1) / NT, part = rounds * 64, from = wave * part + lane;
-  unsigned long long held[kHeld];
-  if constexpr (HELD) {
-#pragma unroll
-    for (int r = 0; r < kHeld; ++r) held[r] = width > a.count ? keys[min(from + 64 * r, width - 1)] : 0;  // (else there is no workspace)
-  }
-  const int n = pages_of(min(max(a.lengths[b], 0), width << a.table.shift), a.table.shift);
-  int* out = a.pages + ((long long)b * a.H + h) * a.count;
-  if (n <= a.count) {
-    for (int i = tid; i < a.count; i += NT) out[i] = i < n ? i : -1;
-    return;
-  }
-  const int to = min(wave * part + part, n);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int part = rounds * 64, from = wave * part + lane, to = min(wave * part + part, n);
   // every number of this thread: place, number (places from `to` on: whatever lies there)
   auto each = [&](auto&& use) {
     if constexpr (HELD) {
@@ -444,7 +461,7 @@ __global__ __launch_bounds__(NT) void select_kernel(const SelectArgs a) {
       for (int r = 0; r < kHeld; ++r)
         if (r < rounds) use(from + 64 * r, held[r]);
     } else {
-      for (int r = 0; r < rounds && from - lane + 64 * r < n; ++r) use(from + 64 * r, keys[min(from + 64 * r, width - 1)]);
+      for (int r = 0; r < rounds && from - lane + 64 * r < n; ++r) use(from + 64 * r, load(from + 64 * r));
     }
   };
   // `known` bits from the top are those of the threshold; `need` of the numbers that have them are to be taken
@@ -518,6 +535,54 @@ __global__ __launch_bounds__(NT) void select_kernel(const SelectArgs a) {
   });
 }
 
+template <int NT, bool HELD>
+__global__ __launch_bounds__(NT) void select_kernel(const SelectArgs a) {
+  const int b = blockIdx.y, h = blockIdx.x, width = a.table.width;
+  const unsigned long long* keys = a.keys + ((long long)b * a.H + h) * width;
+  auto load = [&](int i) { return keys[min(i, width - 1)]; };
+  // parts of the table's width: a thread's numbers are on their way together with the length
+  const int rounds = (width + NT - 1) / NT, from = (threadIdx.x >> 6) * rounds * 64 + (threadIdx.x & 63);
+  unsigned long long held[kHeld];
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) held[r] = HELD && width > a.count ? load(from + 64 * r) : 0;  // (else there is no workspace)
+  const int n = row_pages(a, a.lengths[b]);
+  int* out = a.pages + ((long long)b * a.H + h) * a.count;
+  if (n <= a.count) take_all(a, out, n);
+  else choose<NT, HELD>(a, out, n, rounds, held, load);
+}
+
+// Scores and choice of a (row, head) of few pages, which need no second kernel and no workspace.
+template <class T, int D>
+__global__ __launch_bounds__(256) void few_kernel(const SelectArgs a) {
+  __shared__ unsigned long long s_keys[kFewPages];
+  const int b = blockIdx.y, h = blockIdx.x, wave = threadIdx.x >> 6;
+  Scores<T, D> scores(a, b, h, 1);
+  scores.load_queries();
+  int mine = scores.page_entry(wave * 64);
+  const int n = row_pages(a, a.lengths[b]);
+  int* out = a.pages + ((long long)b * a.H + h) * a.count;
+  if (n <= a.count) {
+    take_all(a, out, n);
+    return;
+  }
+  for (int p0 = wave * 64; p0 < n; p0 += 256) {
+    if (p0 >= 256) {
+      mine = scores.page_entry(p0);
+      scores.load_queries();
+    }
+    scores.have_queries();
+    const unsigned long long x = scores.number(mine, p0, n);
+    if (p0 + scores.in_wave() < n) s_keys[p0 + scores.in_wave()] = x;
+  }
+  __syncthreads();
+  const int rounds = (n + 255) / 256, from = wave * rounds * 64 + (threadIdx.x & 63);
+  auto load = [&](int i) { return s_keys[min(i, n - 1)]; };
+  unsigned long long held[kHeld];
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) held[r] = 64 * 4 * r < kFewPages ? load(from + 64 * r) : 0;
+  choose<256, true>(a, out, n, rounds, held, load);
+}
+
 template <class T>
 static void launch_score(const SelectArgs& args, hipStream_t stream) {
   SelectArgs a = args;
@@ -529,7 +594,18 @@ static void launch_score(const SelectArgs& args, hipStream_t stream) {
   void (*kernel)(SelectArgs) = a.D == 32 ? score_kernel<T, 32> : a.D == 64 ? score_kernel<T, 64> : a.D == 96 ? score_kernel<T, 96> : score_kernel<T, 128>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
 }
+template <class T>
+static void launch_few(const SelectArgs& a, hipStream_t stream) {
+  void (*kernel)(SelectArgs) = a.D == 32 ? few_kernel<T, 32> : a.D == 64 ? few_kernel<T, 64> : a.D == 96 ? few_kernel<T, 96> : few_kernel<T, 128>;
+  hipLaunchKernelGGL(kernel, dim3(a.H, a.B), dim3(256), 0, stream, a);
+}
+long long select_workspace(int width, long long rows) { return width <= kFewPages ? 0 : rows * width * (long long)sizeof(unsigned long long); }
 hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
+  if (a.table.width <= kFewPages) {
+    if (dtype == RA_DTYPE_F16) launch_few<F16>(a, stream);
+    else launch_few<BF16>(a, stream);
+    return hipGetLastError();
+  }
   if (a.table.width > a.count) {  // (else every row has few pages)
     if (dtype == RA_DTYPE_F16) launch_score<F16>(a, stream);
     else launch_score<BF16>(a, stream);

@@ -188,7 +188,7 @@ int ra_page_means(const ra_pool* k_pool, int32_t dtype, const ra_page_table* tab
 }
 
 int64_t ra_select_pages_workspace(const ra_page_table* table, int32_t B, int32_t H) {
-  return table && table->width > 0 && B > 0 && H > 0 ? (int64_t)B * H * table->width * (int64_t)sizeof(unsigned long long) : 0;
+  return table && table->width > 0 && B > 0 && H > 0 ? select_workspace(table->width, (int64_t)B * H) : 0;
 }
 int ra_select_pages(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* means, int64_t means_stride_page, int64_t means_stride_head,
                     int32_t dtype, const ra_page_table* table, const int32_t* lengths, int32_t B, int32_t H, int32_t group, int32_t D, int32_t count,
@@ -206,9 +206,9 @@ int ra_select_pages(const void* q, int64_t q_stride_b, int64_t q_stride_h, const
   if (int e = check_lengths(lengths, lengths)) return e;
   if (!pages) return fail(RA_ERR_NULL, "pages is NULL");
   if (misaligned(pages, 4)) return fail(RA_ERR_ALIGN, "pages must be aligned to its elements");
-  if (table->width > count) {
-    if (!workspace || workspace_bytes < ra_select_pages_workspace(table, B, H))
-      return fail(RA_ERR_NULL, "a workspace of %lld bytes is needed", (long long)ra_select_pages_workspace(table, B, H));
+  const int64_t need = ra_select_pages_workspace(table, B, H);
+  if (table->width > count && need > 0) {
+    if (!workspace || workspace_bytes < need) return fail(RA_ERR_NULL, "a workspace of %lld bytes is needed", (long long)need);
     if (misaligned(workspace, 16)) return fail(RA_ERR_ALIGN, "the workspace must be 16-byte aligned");
   }
   a.q = static_cast<const unsigned short*>(q);

@@ -356,7 +356,9 @@ def test_means_of_the_pages_that_change(dtype, heads, d, size):
 @pytest.mark.parametrize("count,first,last", [(2, 1, 1), (9, 1, 1), (64, 0, 0), (5, 2, 3), (200, 1, 1)])
 def test_chosen_pages(dtype, d, heads, group, count, first, last):
     size = 16
-    c = Cache([0, 1, 32, 33, 1000, 2500, 17 * 1024], heads, d, size, dtype, seed=11)
+    # (a table of up to 512 pages is one kernel's, one of up to 2048 and of 4096 others')
+    longest = {2: 500 * 16, 9: 17 * 1024, 64: 3000 * 16, 5: 512 * 16 - 40, 200: 5000 * 16}[count]
+    c = Cache([0, 1, 32, 33, 1000, 2500, longest], heads, d, size, dtype, seed=11)
     gen = c.gen
     means = torch.empty((c.k.shape[0], heads, d), dtype=dtype, device="cuda").normal_(generator=gen)
     q = c.queries(heads * group)
@@ -434,8 +436,8 @@ def test_refusals():
         attend(q=q.clone().requires_grad_())
     with torch.no_grad():
         attend(q=q.clone().requires_grad_())
-        with pytest.raises(RuntimeError, match="traced"):
-            torch.jit.trace(lambda x: ra.paged_attention(x, c.k, c.v, c.table, c.n), (q,))
+        with pytest.raises(RuntimeError, match="traced"), pytest.warns(DeprecationWarning):
+            torch.jit.trace(lambda x: ra.paged_attention(x, c.k, c.v, c.table, c.n, sm_scale=0.1), (q,))
     for call in (lambda: ra.write_pages(q[:, :2], q[:, 2:], c.k, c.v.float(), c.n.long()), lambda: ra.write_pages(q[:, :2], q[:1, 2:], c.k, c.v, c.n.long()),
                  lambda: ra.write_pages(q[:, :2], q[:, 2:].float(), c.k, c.v, c.n.long()), lambda: ra.write_pages(q[:, :2], q[:, 2:], c.k, c.v, c.n),
                  lambda: ra.write_pages(q[:, :2], q[:, 2:], c.k[:1].expand(3, -1, -1, -1), c.v[:1].expand(3, -1, -1, -1), c.n.long()),

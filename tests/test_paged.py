@@ -116,8 +116,10 @@ def test_slots_writes_means_and_selection_reject_bad_arguments(lib):
         return lib.ra_select_pages(q, 1024, 128, 0x8000, 512, 128, 0, C.byref(table), LENGTHS, 2, 4, group, 128, count, first, last, out, work, size, None)
 
     assert select(q=None) == -1 and select(count=0) == -2 and select(first=-1) == -2 and select(first=3, last=2) == -2 and select(group=0) == -2
-    assert select(work=None) == -1 and select(size=2 * 4 * 64 * 8 - 1) == -1 and select(work=WORK + 8) == -4 and select(out=None) == -1
-    assert lib.ra_select_pages_workspace(C.byref(t), 2, 4) == 2 * 4 * 64 * 8
+    assert select(out=None) == -1 and lib.ra_select_pages_workspace(C.byref(t), 2, 4) == 0  # (few pages)
+    wide = _lib.RaPageTable(TABLE, 600, 600, 1000, 16)
+    assert lib.ra_select_pages_workspace(C.byref(wide), 2, 4) == 2 * 4 * 600 * 8
+    assert select(work=None, table=wide) == -1 and select(size=2 * 4 * 600 * 8 - 1, table=wide) == -1 and select(work=WORK + 8, table=wide) == -4
 
 
 def test_tensors_on_the_host_are_refused():
