@@ -329,6 +329,15 @@ def test_writes_go_to_their_slots_and_nowhere_else(dtype, source, heads, d, layo
     assert torch.equal(c.k, want[0])
 
 
+def test_tokens_that_lie_in_the_pool_are_read_first():
+    """Tokens moved within the pool, each to the place of the next."""
+    c = Cache([320], 2, 64, 16, BF16, seed=17, spare=0)
+    k, v = (x.clone().flatten(0, 1) for x in (c.k, c.v))
+    at = torch.arange(320, device="cuda")
+    ra.write_pages(c.k.flatten(0, 1), c.v.flatten(0, 1), c.k, c.v, (at + 1) % 320)
+    assert torch.equal(c.k.flatten(0, 1), k.roll(1, 0)) and torch.equal(c.v.flatten(0, 1), v.roll(1, 0))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("heads,d,size", [(1, 32, 16), (3, 96, 32), (8, 128, 16), (2, 64, 128), (40, 128, 16)])
 def test_means_of_the_pages_that_change(dtype, heads, d, size):
