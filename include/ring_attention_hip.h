@@ -462,7 +462,8 @@ typedef struct ra_paged_params {
   ra_pool k, v;
   ra_page_table table;
   const int32_t* lengths;
-  const int32_t* pages;    /* numbers (within the sequence) of the pages that are read, each at most once, others left out; NULL: all are */
+  const int32_t* pages;    /* numbers (within the sequence) of the pages that are read, each at most once; of n_pages_read entries the first
+                            * ceil(lengths[b] / page_size) count, and those that are no pages are left out; NULL: all pages are read */
   const float* slopes;     /* ALiBi, [H * group]: -slope * distance added to the scores; NULL: none */
 } ra_paged_params;
 int64_t ra_paged_attention_workspace(const ra_paged_params* p);

@@ -82,7 +82,7 @@ def attention(q, k_pages, v_pages, table, lengths, scale: float, window: int = 0
     for b in range(B):
         n = int(lengths[b])
         for h in range(H):
-            numbers = range(n_pages(n, size)) if pages is None else [j for j in pages[b, h] if 0 <= j < table.shape[1]]
+            numbers = range(n_pages(n, size)) if pages is None else [j for j in pages[b, h, :n_pages(n, size)] if 0 <= j < table.shape[1]]
             ks, vs, at = [], [], []
             for j in numbers:
                 page, here = int(table[b, j]), min(size, n - int(j) * size)

@@ -628,11 +628,14 @@ hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
 // line's prefix sums for itself.  A stretch that holds a (row, head) whole stores its output; parts of one go to memory as (maximum, sum,
 // unnormalised output) in 32 bits and are joined by a second kernel.  Where no row is longer than kWholeKeys (by the table), a workgroup of
 // eight waves takes each (row, head) whole, and that is all.
-RA_DEV int first_key(const PagedArgs& a, int len) { return a.window > 0 ? max(len - a.window, 0) & ~31 : 0; }
+// (of chosen pages all are looked at)
+RA_DEV int first_key(const PagedArgs& a, int len) { return a.window > 0 && a.pages == nullptr ? max(len - a.window, 0) & ~31 : 0; }
 RA_DEV int row_length(const PagedArgs& a, int b) { return min(max(a.lengths[b], 0), a.table.width << a.table.shift); }
+// Pages of a row that are read, or looked at: no more than it has.
+RA_DEV int row_entries(const PagedArgs& a, int len) { return min(pages_of(len, a.table.shift), a.pages != nullptr ? a.count : a.table.width); }
 template <int STEP>
 RA_DEV int row_steps(const PagedArgs& a, int len) {
-  if (a.pages != nullptr) return ((a.count << a.table.shift) + STEP - 1) / STEP;
+  if (a.pages != nullptr) len = row_entries(a, len) << a.table.shift;
   return max((len - first_key(a, len) + STEP - 1) / STEP, 1);  // (one for an empty row: its output is stored too)
 }
 RA_DEV unsigned start_of(unsigned wg, unsigned whole, unsigned rest) { return wg * whole + min(wg, rest); }
@@ -741,7 +744,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
     const int h = a.tiles == 1 ? (int)unit : (int)unit / a.tiles, tile = (int)unit - h * a.tiles;
     const int heads = min(a.G - tile * 16, 16);  // query heads of this unit
     const long long head0 = (long long)b * a.H * a.G + h * a.G + tile * 16;
-    const int low = a.window > 0 ? max(len - a.window, 0) : 0, key0 = a.pages != nullptr ? 0 : first_key(a, len);
+    const int low = a.window > 0 ? max(len - a.window, 0) : 0, key0 = first_key(a, len);
     u32x4 q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -753,7 +756,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
 #pragma unroll
     for (int i = 0; i < DPL; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    const int n_entries = a.pages != nullptr ? a.count : pages_of(len, a.table.shift);
+    const int n_entries = row_entries(a, len);
     // kEntries pages at a time
     unsigned step = at - unit0;
     const unsigned step_end = upto - unit0;

@@ -106,8 +106,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, bias_fn: Optional
             of -inf.  Several tokens of one sequence are several rows with the same pages, each with its own length.
         bias_fn: ``sliding_window_bias(w)`` (pages outside of it are not read), ``alibi_bias(slopes)``, their sum, ``causal_bias()``.
         sm_scale: softmax scale, 1/sqrt(d) if unspecified.
-        pages: int32 ``[sequences, kv_heads, count]``, the pages of each sequence that are read (``select_pages``), each at most once;
-            other numbers are left out.
+        pages: int32 ``[sequences, kv_heads, count]``, the pages of each sequence that are read (``select_pages``), each at most once. Of a
+            sequence of n pages the first n entries count; numbers that are no pages are left out.
     Returns:
         ``[sequences, heads, d]`` of q's type.
     """
