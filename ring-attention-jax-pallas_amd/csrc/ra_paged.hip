@@ -626,8 +626,8 @@ hipError_t launch_select(const SelectArgs& a, int dtype, hipStream_t stream) {
 // The work of a call is one line of steps of 128 keys: row by row of the batch, head by head of the cache, along the sequence.  Every workgroup
 // takes an equal stretch of it, so that rows of any lengths load the chip evenly; lengths are on the device, and each workgroup makes the
 // line's prefix sums for itself.  A stretch that holds a (row, head) whole stores its output; parts of one go to memory as (maximum, sum,
-// unnormalised output) in 32 bits and are joined by a second kernel.  Where no row is longer than kWholeKeys (by the table), a workgroup of
-// eight waves takes each (row, head) whole, and that is all.
+// unnormalised output) in 32 bits and are joined by a second kernel.  Short rows (paged_shape): a workgroup of eight waves takes each (row, head)
+// whole, and that is all.
 // (of chosen pages all are looked at)
 RA_DEV int first_key(const PagedArgs& a, int len) { return a.window > 0 && a.pages == nullptr ? max(len - a.window, 0) & ~31 : 0; }
 RA_DEV int row_length(const PagedArgs& a, int b) { return min(max(a.lengths[b], 0), a.table.width << a.table.shift); }
@@ -968,7 +968,7 @@ static long long part_bytes(int n_wg, int D) { return 2ll * n_wg * kPartRows * D
 static long long stat_bytes(int n_wg) { return 2ll * n_wg * kPartRows * (long long)sizeof(float2); }
 PagedShape paged_shape(long long keys, long long units, int D) {
   const long long steps = (keys + kStepKeys - 1) / kStepKeys, most = steps * units;
-  if (keys <= kWholeKeys) return {(int)units, true, 0};
+  if (keys * D <= kWholeSize || (keys <= kWholeKeys && units >= kWholeUnits)) return {(int)units, true, 0};
   // (as the kernel has it, of the steps that there are at most)
   const long long wanted = most / kStepsEach > kFewWorkgroups ? most / kStepsEach : kFewWorkgroups, cap = most < kPagedWorkgroups ? most : kPagedWorkgroups;
   const int n_wg = (int)(wanted < cap ? wanted : cap);

@@ -83,7 +83,7 @@ def test_attention_rejects_bad_results_and_workspaces(lib):
                        ((0x6000, 0x7002, WORK, need), -4), ((0x6000, 0x7000, None, need), -1), ((0x6000, 0x7000, WORK, need - 1), -1),
                        ((0x6000, 0x7000, WORK + 4, need), -4)):
         assert lib.ra_paged_attention(C.byref(p), *args, None) == code
-    p.table.width = p.table.stride_b = 64  # 1024 tokens are not, and nothing is joined
+    p.table.width = p.table.stride_b = 32  # 512 tokens are not, and nothing is joined
     assert lib.ra_paged_attention_workspace(C.byref(p)) == 0
     assert lib.ra_paged_attention(None, 0x6000, 0x7000, None, 0, None) == -1
 
