@@ -881,30 +881,34 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
       const unsigned last = complete ? blockIdx.x : holder_of(unit0 + steps - 1, whole, rest);
       a.where[b * units + (int)unit] = make_int2((int)slot, (int)(last - blockIdx.x) + 1);
     }
-    for (int i = tid; i < heads * (D / 2); i += THREADS) {
-      const int r = i / (D / 2), d = 2 * (i % (D / 2));
-      const int e = (d % DPL) * 16 + d / DPL;
-      float top = RA_NEG_INF, sum = 0.f, x = 0.f, y = 0.f;
+    // a thread for D / 16 neighbouring elements of a query head
+    if (tid < heads * 16) {
+      const int r = tid / 16, c = tid % 16;
+      float top = RA_NEG_INF, sum = 0.f, x[DPL];
 #pragma unroll 4
       for (int w = 0; w < WAVES; ++w) top = fmaxf(top, s_m[w][r]);
       const float base = top == RA_NEG_INF ? 0.f : top;  // (a wave without a score has a maximum of -inf, and a weight of 0)
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) x[i] = 0.f;
 #pragma unroll 4
       for (int w = 0; w < WAVES; ++w) {
         const float part = __builtin_amdgcn_exp2f(s_m[w][r] - base);
         sum += s_l[w][r] * part;
-        x += s_o[w][r][e] * part;
-        y += s_o[w][r][e + 16] * part;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) x[i] += s_o[w][r][16 * i + c] * part;
       }
       if (WHOLE || complete) {
         // (a row without a key has a sum of 0; scores that are not numbers are in no maximum, but in the sum)
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        *(unsigned*)(a.out + (head0 + r) * D + d) = down2<T>(x * inv, y * inv);
-        if (d == 0) a.lse[head0 + r] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
+        unsigned* out = (unsigned*)(a.out + (head0 + r) * D + c * DPL);
+#pragma unroll
+        for (int i = 0; i < DPL; i += 2) out[i / 2] = down2<T>(x[i] * inv, x[i + 1] * inv);
+        if (c == 0) a.lse[head0 + r] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
       } else {
-        float* p = a.part + (slot * kPartRows + r) * D + d;
-        p[0] = x;
-        p[1] = y;
-        if (d == 0) a.stats[slot * kPartRows + r] = make_float2(top, sum);
+        float* p = a.part + (slot * kPartRows + r) * D + c * DPL;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) p[i] = x[i];
+        if (c == 0) a.stats[slot * kPartRows + r] = make_float2(top, sum);
       }
     }
     at = WHOLE ? end : upto;
