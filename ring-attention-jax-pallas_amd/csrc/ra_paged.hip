@@ -137,7 +137,8 @@ RA_DEV int row_of(const int* sums, int B, int i) {
 // Row b goes from before[b] to after[b] tokens.  Pages are taken from the head of the ring of free pages and given back behind its end, both in the
 // order of the rows, so every place follows from prefix sums over the rows: each workgroup makes those for itself, and no workgroup waits for
 // another.  What is read (the ring's free part, the rows that end) is never what is written (the part behind it, the rows
-// that grow).
+// that grow).  Latency bound: lengths, sums, a row's page, the slot.  A step of 8 sequences 2.8 us, of 512 with 40500 new tokens 6.1 (a thread each,
+// up to 512 workgroups: two tokens a thread one after another took 7.5); an empty kernel's time is 2.3.
 constexpr int kSlotThreads = 256;
 __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) {
   extern __shared__ int s_mem[];
@@ -214,7 +215,8 @@ hipError_t launch_slots(const SlotsArgs& a, hipStream_t stream) {
 // ---------------------------------------------------------------------------------------
 // writes
 // ---------------------------------------------------------------------------------------
-// Eight elements of a token's key and of its value per thread, neighbouring threads on neighbouring chunks.  HBM bound.
+// Eight elements of a token's key and of its value per thread, neighbouring threads on neighbouring chunks.  HBM bound: 30005 tokens of 8 x 96
+// from 32 bits to fp16, 277 MB, 49 us (5.7 TB/s); 64 tokens of 8 x 128 2.5.
 template <class S, class T>
 RA_DEV u32x4 load8(const void* base, long long at) {
   if constexpr (__is_same(S, float)) {
@@ -260,7 +262,8 @@ hipError_t launch_write(const WriteArgs& a, int src_dtype, int dtype, hipStream_
 // mean keys
 // ---------------------------------------------------------------------------------------
 // The mean over the tokens that a page holds, for each page whose tokens change between before[b] and after[b]: a workgroup per page and up to 64 chunks
-// of eight elements, its threads on neighbouring chunks and, beyond those, on different tokens.  HBM bound.
+// of eight elements, its threads on neighbouring chunks and, beyond those, on different tokens.  HBM bound for prompts (46 MB, 12.3 us), latency for a
+// step (64 pages of 8 x 128: 4.8 us of lengths, sums, a page, its keys, the sum over threads).
 constexpr int kMeanThreads = 256;
 template <class T>
 __global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) {
@@ -330,8 +333,9 @@ hipError_t launch_means(const MeansArgs& args, int dtype, hipStream_t stream) {
 // ---------------------------------------------------------------------------------------
 // Scores: (sum of the group's queries) . (mean key), in 64 bits: products of 16-bit floats are exact there, and so are their sums but for
 // extreme ranges, so that the order of pages does not depend on the order of a sum.  A score becomes a whole number of the same order.
-// Sixteen lanes (eight, four for narrow heads) read a page's mean in one go, a wave 64 pages; their partial sums are exchanged so that each
-// lane ends with the sums of its own pages.
+// Sixteen lanes (eight, four for narrow heads) read a page's mean in one go, a wave 64 of them; their partial sums are exchanged so that each
+// lane ends with the sums of its own.  A load takes several heads of a page beside each other, where there are several: 16 x 8 heads, 37 MB of means,
+// 12.3 us, with a head alone in a load 16.5.  In 32 bits it would be 3 us less, and the choice would depend on the order of the sums.
 constexpr int kScoreRows = 256;  // (page, head)s of a workgroup, 64 a wave
 constexpr unsigned long long kForced = ~0ull;
 RA_DEV unsigned long long ordered(double x) {
@@ -442,7 +446,8 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
 // The `count` largest of a row's numbers, ties from the lowest place, their places in order: the threshold by its digits of twelve bits (ten
 // for few numbers) from the top, until all that share the digits found so far are taken; then every wave places what it takes of its part of the
 // row.  Twelve bits: the first digit is a double's sign and exponent, and the second mostly settles it.  Bound by latency: some ten
-// barriers, and few numbers between them.  HELD: the row's numbers stay in registers, kHeld of a thread.
+// barriers, and few numbers between them: 128 of 4096 for 128 (row, head)s 6.3 us.  HELD: the row's numbers stay in registers, kHeld of a thread (read from the caches in every
+// pass: 12; from shared memory: 11.5).
 constexpr int kHeld = 8;
 RA_DEV void take_all(const SelectArgs& a, int* out, int n) {
   for (int i = threadIdx.x; i < a.count; i += blockDim.x) out[i] = i < n ? i : -1;
@@ -551,7 +556,8 @@ __global__ __launch_bounds__(NT) void select_kernel(const SelectArgs a) {
   else choose<NT, HELD>(a, out, n, rounds, held, load);
 }
 
-// Scores and choice of a (row, head) of few pages, which need no second kernel and no workspace.
+// Scores and choice of a (row, head) of few pages, which need no second kernel and no workspace.  In a graph, one kernel | two, us: 250 pages of 2 x 2 heads
+// 4.9 | 7.1, 512 of 8 heads 8.6 | 9.2, of 64 x 8 16.2 | 22.3: a compute unit reads the 128 KB of 512 pages' means about as fast as a second kernel starts.
 template <class T, int D>
 __global__ __launch_bounds__(256) void few_kernel(const SelectArgs a) {
   __shared__ unsigned long long s_keys[kFewPages];
@@ -652,7 +658,8 @@ RA_DEV float logsumexp_of(float top, float sum) {
 
 // A wave's 32 keys and values on their way.  Keys are the matrix instruction's first operand: lane l holds key l % 16 of each half, eight
 // elements from 8 (l / 16) of every 32.  Of values lane l holds, of D / 16 elements from (l % 16) D / 16, the eight keys whose weights it gets from the scores'
-// product: 4 (l / 16) + 0 .. 3 of each half; a row is read whole by sixteen lanes.
+// product: 4 (l / 16) + 0 .. 3 of each half; a row is read whole by sixteen lanes.  Both go from memory to the registers that the matrix unit reads: nothing
+// is shared between waves, and nothing goes through shared memory but the waves' ends.
 template <int D>
 struct KeyTile {
   u32x4 k[2][D / 32];
@@ -688,6 +695,9 @@ RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
 constexpr int kEntries = 1024, kNearRows = 1024;  // of a stretch's pages, of the rows' lengths in shared memory
 constexpr int kNowhere = 0x3fffffff;  // (a position behind every sequence)
 
+// HBM bound: the matrix unit multiplies sixteen rows however few there are, and is busy for a sixteenth of the time.  64 x 8 heads, 2.06 GB, 335 us (6.15 TB/s), 32 x
+// 131071 keys, 2.15 GB, 330 (6.5); 16 x 16 heads, 231 MB, 46, of which 4 pass before the first keys arrive.  A call on 1000 keys of 8 heads,
+// D=64, is 9.3 us of one workgroup per head: what a compute unit alone gets from memory.
 template <class T, int D, bool ALIBI, bool WHOLE>
 __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const PagedArgs a) {
   constexpr int WAVES = WHOLE ? 8 : 4, THREADS = 64 * WAVES, STEP = 32 * WAVES;
@@ -916,7 +926,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
 }
 
 // The parts of a (row, query head): a workgroup each, threads on neighbouring elements and on different parts.  Latency bound: a part's statistics and
-// its elements are on their way together, for 64 parts at a time.
+// its elements are on their way together, for 64 parts at a time: 2.6 us for 60 (row, head)s, 4.1 for 2048.
 template <class T, int D>
 __global__ __launch_bounds__(256) void join_kernel(const PagedArgs a) {
   constexpr int COLS = D / 4, GROUPS = 256 / COLS, MOST = (64 + GROUPS - 1) / GROUPS;

@@ -1,5 +1,5 @@
 // Calls on a paged key-value cache from Python: checks, results and workspace, and the library's one call each, without Python code on the
-// way.  Such calls are small: the slots of a step are 5 us of kernel.
+// way.  Such calls are small: the slots of a step are 3 us of kernel and 4 of host.
 #include "ra_host.h"
 
 #include <ATen/EmptyTensor.h>
