@@ -693,7 +693,7 @@ RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
 }
 
 constexpr int kEntries = 1024, kNearRows = 1024;  // of a stretch's pages, of the rows' lengths in shared memory
-constexpr int kNowhere = 0x3fffffff;  // (a position behind every sequence)
+constexpr int kNowhere = 0x7ff00000;  // (a position behind every sequence, of 2^30 tokens at most; a page and a tile on top of it fit 32 bits)
 
 // HBM bound: the matrix unit multiplies sixteen rows however few there are, and is busy for a sixteenth of the time.  64 x 8 heads, 2.06 GB, 335 us (6.15 TB/s), 32 x
 // 131071 keys, 2.15 GB, 330 (6.5); 16 x 16 heads, 231 MB, 46, of which 4 pass before the first keys arrive.  A call on 1000 keys of 8 heads,

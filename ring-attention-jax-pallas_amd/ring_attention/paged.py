@@ -38,7 +38,7 @@ def page_slots(block_table, lengths, new_lengths, free_pages, free_state, page_s
 
     Args:
         block_table: int32 ``[sequences, width]``, rows contiguous; entries of new pages are written, others left.
-        lengths, new_lengths: int32 ``[sequences]``.
+        lengths, new_lengths: int32 ``[sequences]``.  (A row that ends and takes a new sequence at once goes through 0 in a call of its own.)
         free_pages: int32 ``[pages]``, a ring: from place ``free_state[0]`` on, around its end, ``free_state[1]`` pages are free.  To
             begin with ``arange(pages)`` and ``(0, pages)``.  Pages given back are written behind the free ones.
         free_state: int32 ``[2]``.

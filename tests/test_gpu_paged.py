@@ -220,6 +220,18 @@ def test_stretches_of_more_pages_than_shared_memory_holds():
             assert abs(float(lse[b, h]) - float(torch.logsumexp(s, 0))) <= 2.0 ** -24 * 2 ** 13
 
 
+def test_the_longest_sequence():
+    """2^30 tokens, pages named again and again, and one that is not in the pool: the pool's first page, which must not stand in for it, holds NaN."""
+    k, v = torch.zeros((5, 64, 1, 32), dtype=BF16, device="cuda"), torch.ones((5, 64, 1, 32), dtype=BF16, device="cuda")
+    k[0], v[0] = math.nan, math.nan
+    table = torch.randint(1, 5, (1, 1 << 24), device="cuda", dtype=torch.int32)
+    table[0, -3] = -1
+    q = torch.ones((1, 1, 32), dtype=BF16, device="cuda")
+    out, lse = ra.paged_attention_with_lse(q, k, v, table, _ints([1 << 30]))
+    # equal weights: sums of whole numbers, of 2^30 in the end, in 32 bits
+    assert bool((out == 1).all()) and abs(float(lse) - math.log(2.0 ** 30 - 64)) <= 2.0 ** -22 * 21
+
+
 def test_small_weights_beside_a_large_one():
     """fp16: 60000 keys of 2^-20 of the largest weight each make up 5 percent of the output."""
     n, d = 60001, 64
