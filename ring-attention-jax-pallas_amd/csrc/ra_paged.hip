@@ -668,10 +668,22 @@ struct KeyTile {
 
 // STREAM: the caches are not to keep it, as they cannot keep what a large call reads once (64 x 8 heads, 2.06 GB: 341 us against 367); a small one's
 // keys may be there from the step before (1000 x 8 heads: 9.4 us either way from caches, 13.3 with the hint where they would have been in them).
-template <bool STREAM, class V>
-RA_DEV V load_row(const V* at) {
-  if constexpr (STREAM) return __builtin_nontemporal_load(at);
-  return *at;
+// (an overload for each width: a template's parameter would not keep that rows are aligned to four bytes only)
+template <bool STREAM>
+RA_DEV u32x4 load_row(const u32x4* at) {
+  return STREAM ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool STREAM>
+RA_DEV u32x3a load_row(const u32x3a* at) {
+  return STREAM ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool STREAM>
+RA_DEV u32x2a load_row(const u32x2a* at) {
+  return STREAM ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool STREAM>
+RA_DEV unsigned load_row(const unsigned* at) {
+  return STREAM ? __builtin_nontemporal_load(at) : *at;
 }
 template <int D, bool STREAM>
 RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
