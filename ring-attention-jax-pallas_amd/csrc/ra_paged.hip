@@ -656,15 +656,24 @@ RA_DEV float logsumexp_of(float top, float sum) {
   return ((top == RA_NEG_INF ? 0.f : top) - T::kLift + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// A wave's 32 keys and values on their way.  Keys are the matrix instruction's first operand: lane l holds key l % 16 of each half, eight
-// elements from 8 (l / 16) of every 32.  Of values lane l holds, of D / 16 elements from (l % 16) D / 16, the eight keys whose weights it gets from the scores'
-// product: 4 (l / 16) + 0 .. 3 of each half; a row is read whole by sixteen lanes.  Both go from memory to the registers that the matrix unit reads: nothing
-// is shared between waves, and nothing goes through shared memory but the waves' ends.
+// A wave's 32 keys and values on their way.  Both are loaded with neighbouring lanes on neighbouring 16 bytes of a row: a load whose lanes 0 .. 15 are on
+// rows of their own, as the matrix instruction wants keys, takes a cache lookup for each of them (a compute unit gets 38 GB/s so, and 148 from whole
+// rows).  Keys then pass through the wave's own piece of shared memory: instruction i of a half writes the 16-byte chunks 64 i .. 64 i + 63 of its
+// sixteen rows, and lane l reads chunks l / 16 + 4 s of key l % 16, the first operand.  Of values lane l holds, of D / 16 elements from (l % 16) D / 16,
+// the eight keys whose weights it gets from the scores' product: 4 (l / 16) + 0 .. 3 of each half.  Nothing is shared between waves but their ends.
 template <int D>
 struct KeyTile {
   u32x4 k[2][D / 32];
   unsigned v[8][D / 32];
 };
+// The place of a key row's chunk among the row's: sixteen rows' chunks of one number lie in different banks.
+template <int D>
+RA_DEV int chunk_place(int row, int chunk) {
+  if constexpr (D == 128) return chunk ^ row;
+  if constexpr (D == 96) return (chunk + row / 4) % 12;
+  if constexpr (D == 64) return chunk ^ row / 2;
+  return chunk ^ row / 4;
+}
 
 // STREAM: the caches are not to keep it, as they cannot keep what a large call reads once (64 x 8 heads, 2.06 GB: 341 us against 367); a small one's
 // keys may be there from the step before (1000 x 8 heads: 9.4 us either way from caches, 13.3 with the hint where they would have been in them).
@@ -715,14 +724,29 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
   constexpr int WAVES = WHOLE ? 8 : 4, THREADS = 64 * WAVES, STEP = 32 * WAVES;
   constexpr int KS = D / 32;  // matrix instructions of a score, words of a lane's value row
   constexpr int DPL = D / 16;  // elements of a lane's value row
+  constexpr int CHUNKS = D / 8;  // of 16 bytes in a row
   extern __shared__ int s_first[];
   __shared__ int red[WAVES][1];
   __shared__ int s_page[kEntries], s_pos[kEntries], s_len[WHOLE ? 1 : kNearRows];
   __shared__ float s_m[WAVES][16], s_l[WAVES][16];
-  __shared__ float s_o[WAVES][16][D + 4];  // elements in the order of the lanes' registers: 16 i + m is element m D / 16 + i
+  // the waves' keys, and when all are through their outputs, elements in the order of the lanes' registers: 16 i + m is element m D / 16 + i
+  __shared__ union {
+    u32x4 k[WAVES][2][16 * CHUNKS];
+    float o[WAVES][16][D + 4];
+  } s_tile;
+  auto& s_o = s_tile.o;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int units = a.H * a.tiles;  // of a row
+  // this lane's chunks of a half's rows: where they are in the pool, where they go, and where its operands are
+  int k_from[KS], k_to[KS], k_at[KS];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    const int row = (64 * i + lane) / CHUNKS, chunk = (64 * i + lane) % CHUNKS;
+    k_from[i] = row * a.k.st + chunk * 8;
+    k_to[i] = row * CHUNKS + chunk_place<D>(row, chunk);
+    k_at[i] = col * CHUNKS + chunk_place<D>(col, 4 * i + grp);
+  }
   unsigned whole = 0, rest = 0, begin = 0, end = 1;
   if constexpr (!WHOLE) {
     scan_rows<THREADS, 1>(
@@ -798,7 +822,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
         s_pos[i] = there ? logical << a.table.shift : kNowhere;
       }
       __syncthreads();
-      // A step's keys are replaced by the next one's as soon as the scores are made, its values after the product with the weights: one is
+      // A step's keys are replaced by the next one's as soon as they are in shared memory, its values after the product with the weights: one is
       // always on its way while the other is used, in the registers of a single step.
       KeyTile<D> x;
       int p[2];
@@ -815,7 +839,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           } else {
             const unsigned short* kp = a.k.ptr + page * a.k.sp + (off * a.k.st + h * a.k.sh);
 #pragma unroll
-            for (int i = 0; i < KS; ++i) x.k[t][i] = load_row<!WHOLE>((const u32x4*)(kp + (col * a.k.st + i * 32 + grp * 8)));
+            for (int i = 0; i < KS; ++i) x.k[t][i] = load_row<!WHOLE>((const u32x4*)(kp + k_from[i]));
           }
         }
       };
@@ -827,19 +851,26 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           const int kt = key0 + (int)step * STEP + wave * 32 + 16 * t;
           p[t] = __builtin_amdgcn_readfirstlane(s_pos[(kt >> a.table.shift) - entry0]) + (kt & (size - 1));
         }
+        // (a wave's accesses to shared memory are done in their order)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < KS; ++i) s_tile.k[wave][t][k_to[i]] = x.k[t][i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (step + 1 < chunk_end) load(step + 1, false);
         float w[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < KS; ++i) c = T::mfma(x.k[t][i], q[i], c);
+          for (int i = 0; i < KS; ++i) c = T::mfma(s_tile.k[wave][t][k_at[i]], q[i], c);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             w[4 * t + r] = c[r] * a.scale2;
             if constexpr (ALIBI) w[4 * t + r] -= slope * (float)(len - 1 - p[t] - 4 * grp - r);
           }
         }
-        if (step + 1 < chunk_end) load(step + 1, false);
         const bool inside = p[0] >= low && p[0] + 16 <= len && p[1] >= low && p[1] + 16 <= len;
         if (!inside) {
           // What is masked may hold anything: its score is replaced, and its value too (0 times infinity is not 0).
