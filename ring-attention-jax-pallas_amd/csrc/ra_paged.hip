@@ -5,12 +5,13 @@
 namespace ra {
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(2), aligned(4))) unsigned int u32x2a;
 typedef __attribute__((ext_vector_type(3), aligned(4))) unsigned int u32x3a;
 
 struct BF16 {
   static RA_DEV float up(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
-  static RA_DEV unsigned short down(float x) { return __builtin_bit_cast(unsigned short, (bf16_t)x); }
+  static RA_DEV unsigned down2(float lo, float hi) { return __builtin_bit_cast(unsigned, (bf16x2){(bf16_t)lo, (bf16_t)hi}); }
   static RA_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -18,7 +19,7 @@ struct BF16 {
 };
 struct F16 {
   static RA_DEV float up(unsigned short x) { return (float)__builtin_bit_cast(_Float16, x); }
-  static RA_DEV unsigned short down(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
+  static RA_DEV unsigned down2(float lo, float hi) { return __builtin_bit_cast(unsigned, (f16x2){(_Float16)lo, (_Float16)hi}); }
   static RA_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -26,10 +27,6 @@ struct F16 {
   // the output.
   static constexpr float kLift = 15.f;
 };
-template <class T>
-RA_DEV unsigned down2(float lo, float hi) {
-  return (unsigned)T::down(lo) | (unsigned)T::down(hi) << 16;
-}
 
 RA_DEV int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
 
@@ -221,13 +218,13 @@ template <class S, class T>
 RA_DEV u32x4 load8(const void* base, long long at) {
   if constexpr (__is_same(S, float)) {
     const f32x4 x = *(const f32x4*)((const float*)base + at), y = *(const f32x4*)((const float*)base + at + 4);
-    return (u32x4){down2<T>(x[0], x[1]), down2<T>(x[2], x[3]), down2<T>(y[0], y[1]), down2<T>(y[2], y[3])};
+    return (u32x4){T::down2(x[0], x[1]), T::down2(x[2], x[3]), T::down2(y[0], y[1]), T::down2(y[2], y[3])};
   } else {
     const u32x4 x = *(const u32x4*)((const unsigned short*)base + at);
     if constexpr (__is_same(S, T)) return x;
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = down2<T>(S::up((unsigned short)x[i]), S::up((unsigned short)(x[i] >> 16)));
+    for (int i = 0; i < 4; ++i) r[i] = T::down2(S::up((unsigned short)x[i]), S::up((unsigned short)(x[i] >> 16)));
     return r;
   }
 }
@@ -309,8 +306,8 @@ __global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) 
         for (int e = 0; e < 8; ++e) sum[e] += s_sum[tid + g * cols][e];
       const float count = (float)n;
       *(u32x4*)(a.means + page * a.means_sp + (h * a.means_sh + d)) =
-          (u32x4){down2<T>(sum[0] / count, sum[1] / count), down2<T>(sum[2] / count, sum[3] / count), down2<T>(sum[4] / count, sum[5] / count),
-                  down2<T>(sum[6] / count, sum[7] / count)};
+          (u32x4){T::down2(sum[0] / count, sum[1] / count), T::down2(sum[2] / count, sum[3] / count), T::down2(sum[4] / count, sum[5] / count),
+                  T::down2(sum[6] / count, sum[7] / count)};
     }
     __syncthreads();
   }
@@ -898,11 +895,11 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           w[j] = __builtin_amdgcn_exp2f(w[j] - base);
           l += w[j];
         }
-        const u32x4 wb = {down2<T>(w[0], w[1]), down2<T>(w[2], w[3]), down2<T>(w[4], w[5]), down2<T>(w[6], w[7])};
+        const u32x4 wb = {T::down2(w[0], w[1]), T::down2(w[2], w[3]), T::down2(w[4], w[5]), T::down2(w[6], w[7])};
         // What the rounded weights lack of theirs goes through the matrix unit as well, which has the time: the output is off by its own rounding.
         u32x4 wr;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wr[j] = down2<T>(w[2 * j] - T::up((unsigned short)wb[j]), w[2 * j + 1] - T::up((unsigned short)(wb[j] >> 16)));
+        for (int j = 0; j < 4; ++j) wr[j] = T::down2(w[2 * j] - T::up((unsigned short)wb[j]), w[2 * j + 1] - T::up((unsigned short)(wb[j] >> 16)));
 #pragma unroll
         for (int i = 0; i < DPL; ++i) {
           const unsigned pick = i & 1 ? 0x07060302u : 0x05040100u;
@@ -955,7 +952,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         unsigned* out = (unsigned*)(a.out + (head0 + r) * D + c * DPL);
 #pragma unroll
-        for (int i = 0; i < DPL; i += 2) out[i / 2] = down2<T>(x[i] * inv, x[i + 1] * inv);
+        for (int i = 0; i < DPL; i += 2) out[i / 2] = T::down2(x[i] * inv, x[i + 1] * inv);
         if (c == 0) a.lse[head0 + r] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
       } else {
         float* p = a.part + (slot * kPartRows + r) * D + c * DPL;
@@ -1015,7 +1012,7 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedArgs a) {
       y += s_sum[p][2 * tid];
       z += s_sum[p][2 * tid + 1];
     }
-    *(unsigned*)(a.out + at * D + 2 * tid) = down2<T>(y * inv, z * inv);
+    *(unsigned*)(a.out + at * D + 2 * tid) = T::down2(y * inv, z * inv);
   }
   if (tid == 0) a.lse[at] = sum == 0.f ? RA_NEG_INF : logsumexp_of<T>(top, sum);
 }
