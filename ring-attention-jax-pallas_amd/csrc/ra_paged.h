@@ -9,12 +9,14 @@ constexpr int kMaxRows = RA_MAX_PAGED_ROWS;  // sequences of one call: their pre
 constexpr int kStepKeys = 128;               // keys that a workgroup of the attention kernel takes at a time, 32 a wave
 // A (row, head) is one workgroup's where its keys and values by the table are at most 256 KB (keys x D up to kWholeSize), which a compute unit
 // reads in some 6 us, or up to kWholeKeys keys where there are kWholeUnits of them; else the call's keys are shared between workgroups and their parts
-// joined, for 4 us and a launch more.  Whole | shared, us: 512 keys, D=128, 8 (row, head)s 8.5 | 8.5, 128 of them 10.5 | 13.9; 1024 keys, D=128, 8: 13.1 |
-// 9.4, 128: 16.4 | 19.2, 256: 28.3 | 30.5, 1024: 101 | 99; 1000 keys, D=64, 8: 9.1 | 7.7 in a graph, 9.4 | 11.2 from the host, which launches once.
+// joined, for 4 us and a launch more.  Whole | shared in a graph, us: 512 keys, D=128, 8 (row, head)s 7.2 | 8.8, 128 of them 10.8 | 13.5, 1024 48.7 | 47.9;
+// 1024 keys, D=128, 8: 10.4 | 9.1, 32: 12.4 | 10.3, 128: 16.1 | 18.5, 256: 27.9 | 28.2, 1024: 99.6 | 92.2; 2048 keys, D=128, 8: 17.8 | 9.4, 128: 34.5 | 29.0;
+// 1000 keys, D=64, 8: 8.4 | 7.5 (from the host, which launches one kernel instead of two, 8.1 | 11), 128: 10.4 | 14.5, 1024: 45.3 | 61.3.
 constexpr int kWholeSize = 65536, kWholeKeys = 1024, kWholeUnits = 128;
-// Workgroups that share: kStepsEach steps for each (128 keys), and at least kFewWorkgroups, two on each compute unit as their registers allow; at most
-// kPagedWorkgroups, whose ends a large call does not feel.  2.15 GB: 512 workgroups 398 us, 1024 354, 2048 334, 4096 335; 231 MB: 2 steps each
-// 56, 4: 54, 8: 54.5; 256 workgroups at least instead of 512: 20 MB 15.3 instead of 13.8, 1024: 134 MB 62.0 instead of 59.6.
+// Workgroups that share: kStepsEach steps for each (128 keys), and at least kFewWorkgroups, two on each compute unit as their registers allow (three, with registers spilled: 391 us for 335); at most
+// kPagedWorkgroups, whose ends a large call does not feel.  2.15 GB: 1024 workgroups 354 us, 2048 335, 4096 329, but 2.06 GB of 64 rows 336
+// with 2048 and 344 with 4096; 231 MB: 2 steps each 49.2, 4: 48.5, 8: 50.6; at least 256 workgroups instead of 512: 20 MB 14.6 instead of 13.7, 768: 134 MB
+// 54.1 instead of 50.4.
 constexpr int kPagedWorkgroups = 2048, kFewWorkgroups = 512, kStepsEach = 4;
 constexpr int kPartRows = 16;                // query heads of a workgroup: the columns of a matrix instruction
 

@@ -672,8 +672,8 @@ RA_DEV int chunk_place(int row, int chunk) {
   return chunk ^ row / 4;
 }
 
-// STREAM: the caches are not to keep it, as they cannot keep what a large call reads once (64 x 8 heads, 2.06 GB: 341 us against 367); a small one's
-// keys may be there from the step before (1000 x 8 heads: 9.4 us either way from caches, 13.3 with the hint where they would have been in them).
+// STREAM: the caches are not to keep it, as they cannot keep what a large call reads once (64 x 8 heads, 2.06 GB: 336 us against 367; 231 MB 48.6 against 54.0); a small one's
+// keys may be there from the step before (1000 x 8 heads, whole: 4 us more with the hint where they would have been).
 // (an overload for each width: a template's parameter would not keep that rows are aligned to four bytes only)
 template <bool STREAM>
 RA_DEV u32x4 load_row(const u32x4* at) {
@@ -713,9 +713,9 @@ RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
 constexpr int kEntries = 1024, kNearRows = 1024;  // of a stretch's pages, of the rows' lengths in shared memory
 constexpr int kNowhere = 0x7ff00000;  // (a position behind every sequence, of 2^30 tokens at most; a page and a tile on top of it fit 32 bits)
 
-// HBM bound: the matrix unit multiplies sixteen rows however few there are, and is busy for a sixteenth of the time.  64 x 8 heads, 2.06 GB, 335 us (6.15 TB/s), 32 x
-// 131071 keys, 2.15 GB, 330 (6.5); 16 x 16 heads, 231 MB, 46, of which 4 pass before the first keys arrive.  A call on 1000 keys of 8 heads,
-// D=64, is 9.3 us of one workgroup per head: what a compute unit alone gets from memory.
+// HBM bound: the matrix unit multiplies sixteen rows however few there are, and is busy for a sixteenth of the time.  64 x 8 heads, 2.06 GB, 331 us (6.2 TB/s), 32 x
+// 131071 keys, 2.15 GB, 328 (6.5); 16 x 16 heads, 231 MB, 44, of which 4 pass before the first keys arrive.  A call on 1000 keys of 8 heads,
+// D=64, is 8.5 us of one workgroup per head: what a compute unit alone gets from memory.
 template <class T, int D, bool ALIBI, bool WHOLE>
 __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const PagedArgs a) {
   constexpr int WAVES = WHOLE ? 8 : 4, THREADS = 64 * WAVES, STEP = 32 * WAVES;
