@@ -83,7 +83,7 @@ int paged_args(const ra_paged_params* p, PagedArgs& a, PagedShape& shape) {
   if (int e = check_rows(p->B, p->H, p->D)) return e;
   if (p->group <= 0 || (int64_t)p->H * p->group > 65535) return fail(RA_ERR_SHAPE, "1 to 65535 query heads (got %d x %d)", p->H, p->group);
   if (p->window < 0) return fail(RA_ERR_BIAS, "window must be positive, or 0 for none (got %d)", p->window);
-  if (!isfinite(p->sm_scale)) return fail(RA_ERR_SHAPE, "sm_scale must be finite");
+  if (!isfinite(p->sm_scale * kLog2e)) return fail(RA_ERR_SHAPE, "sm_scale must be finite, times log2(e) too");
   if (int e = check_table(&p->table, p->B, a.table)) return e;
   if (int e = check_strides("q", p->q, p->q_stride_b, p->q_stride_h, p->H * p->group, p->D)) return e;
   if (int e = check_pool("k", &p->k, p->H, p->D, p->table.page_size, a.k)) return e;

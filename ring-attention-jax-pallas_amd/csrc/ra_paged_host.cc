@@ -328,6 +328,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     if (slopes.defined()) {
       c.here(slopes, "slopes");
+      c.no_grad(slopes, "slopes");
       TORCH_CHECK_VALUE(slopes.scalar_type() == at::kFloat && slopes.dim() == 1 && slopes.size(0) == x.size(1), "ALiBi slopes must be float32 [", x.size(1),
                         "], one for each query head, not ", slopes.scalar_type(), " ", slopes.sizes());
       heads_slopes = slopes.contiguous();

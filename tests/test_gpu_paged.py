@@ -464,6 +464,9 @@ def test_refusals():
             attend(**kw)
     with pytest.raises(RuntimeError, match="gradient"):
         attend(q=q.clone().requires_grad_())
+    for device in ("cuda", "cpu"):
+        with pytest.raises(RuntimeError, match="slopes requires a gradient"):
+            attend(bias=ra.alibi_bias(ra.alibi_slopes(4).to(device).requires_grad_()))
     with torch.no_grad():
         attend(q=q.clone().requires_grad_())
         with pytest.raises(RuntimeError, match="traced"), pytest.warns(DeprecationWarning):

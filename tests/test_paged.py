@@ -42,6 +42,7 @@ def test_struct_layout():
     (lambda p: setattr(p, "dtype", _lib.RA_DTYPE_F32), -7),
     (lambda p: setattr(p, "window", -1), -5),
     (lambda p: setattr(p, "sm_scale", float("inf")), -2),
+    (lambda p: setattr(p, "sm_scale", 3e38), -2),
     (lambda p: setattr(p, "q", None), -1),
     (lambda p: setattr(p, "q", 0x1008), -4),
     (lambda p: setattr(p, "q_stride_h", 129), -4),
