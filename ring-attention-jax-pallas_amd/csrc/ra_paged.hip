@@ -848,7 +848,9 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           const int kt = key0 + (int)step * STEP + wave * 32 + 16 * t;
           p[t] = __builtin_amdgcn_readfirstlane(s_pos[(kt >> a.table.shift) - entry0]) + (kt & (size - 1));
         }
-        // (a wave's accesses to shared memory are done in their order)
+        // (a wave's accesses to shared memory are done in their order: the fences keep the compiler to it, and cost nothing)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
