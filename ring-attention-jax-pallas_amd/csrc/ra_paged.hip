@@ -16,6 +16,7 @@ struct BF16 {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   static constexpr float kLift = 0.f;
+  static constexpr int kPieces = 3;  // of 8 bits each: all of a weight's 24
 };
 struct F16 {
   static RA_DEV float up(unsigned short x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -26,6 +27,7 @@ struct F16 {
   // Weights are rounded to fp16 as 2^15 times their value: 2^17 of them that are 2^-25 of the largest, each below fp16's least, make up 2^-8 of
   // the output.
   static constexpr float kLift = 15.f;
+  static constexpr int kPieces = 2;  // of 11 bits each
 };
 
 RA_DEV int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
@@ -897,18 +899,26 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           w[j] = __builtin_amdgcn_exp2f(w[j] - base);
           l += w[j];
         }
-        const u32x4 wb = {T::down2(w[0], w[1]), T::down2(w[2], w[3]), T::down2(w[4], w[5]), T::down2(w[6], w[7])};
-        // What the rounded weights lack of theirs goes through the matrix unit as well, which has the time: the output is off by its own rounding.
-        u32x4 wr;
+        // A weight goes in as pieces of the type's precision, what the ones before lack of it in the next, through the matrix unit, which has the time: the
+        // output is off by its own rounding and by sums in 32 bits.  (Two pieces of bf16 left 2^-17 of a weight: one output in 500 was the neighbour of the nearest number.)
+        u32x4 piece[T::kPieces];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wr[j] = T::down2(w[2 * j] - T::up((unsigned short)wb[j]), w[2 * j + 1] - T::up((unsigned short)(wb[j] >> 16)));
+        for (int n = 0; n < T::kPieces; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            piece[n][j] = T::down2(w[2 * j], w[2 * j + 1]);
+            w[2 * j] -= T::up((unsigned short)piece[n][j]);
+            w[2 * j + 1] -= T::up((unsigned short)(piece[n][j] >> 16));
+          }
+        }
 #pragma unroll
         for (int i = 0; i < DPL; ++i) {
           const unsigned pick = i & 1 ? 0x07060302u : 0x05040100u;
           u32x4 vt;
 #pragma unroll
           for (int j = 0; j < 4; ++j) vt[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i >> 1], x.v[2 * j][i >> 1], pick);
-          o[i] = T::mfma(vt, wr, T::mfma(vt, wb, o[i]));
+#pragma unroll
+          for (int n = 0; n < T::kPieces; ++n) o[i] = T::mfma(vt, piece[n], o[i]);
         }
         if (step + 1 < chunk_end) load(step + 1, true);
       }
