@@ -464,10 +464,13 @@ typedef struct ra_paged_params {
   const int32_t* lengths;
   const int32_t* pages;    /* numbers (within the sequence) of the pages that are read, each at most once; of n_pages_read entries the first
                             * ceil(lengths[b] / page_size) count, and those that are no pages are left out; NULL: all pages are read */
-  const float* slopes;     /* ALiBi, [H * group]: -slope * distance added to the scores; NULL: none */
+  const float* slopes;     /* ALiBi, [H * group] on the device: -slope * distance added to the scores; NULL: none */
 } ra_paged_params;
 int64_t ra_paged_attention_workspace(const ra_paged_params* p);
 int ra_paged_attention(const ra_paged_params* p, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+/* to[0 .. n) = values[0 .. n), which lie in host memory (ALiBi slopes that a program keeps there): they go along as arguments of a kernel, so that the call
+ * waits for nothing, values is free when it returns, and a captured call holds what values was then. */
+int ra_put_floats(const float* values, int32_t n, float* to, void* stream);
 
 /* Host-only, pure: 1 if every score of the (query shard, key/value shard) pair is masked
  * by the positional terms of `bias` (CAUSAL / WINDOW), so that the whole ring step is an

@@ -116,4 +116,7 @@ struct PagedShape {
 PagedShape paged_shape(long long keys, long long units, int D);
 hipError_t launch_paged(PagedArgs& a, int D, int dtype, const PagedShape& shape, void* workspace, hipStream_t stream);
 
+// n floats of host memory to the device in the order of the stream, as kernel arguments.
+hipError_t launch_put(const float* values, int n, float* to, hipStream_t stream);
+
 }  // namespace ra

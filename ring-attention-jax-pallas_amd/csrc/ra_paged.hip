@@ -1071,4 +1071,31 @@ hipError_t launch_paged(PagedArgs& a, int D, int dtype, const PagedShape& shape,
   return dtype == RA_DTYPE_F16 ? launch_paged_type<F16>(a, D, shape, workspace, stream) : launch_paged_type<BF16>(a, D, shape, workspace, stream);
 }
 
+// ---------------------------------------------------------------------------------------
+// a few numbers from the host
+// ---------------------------------------------------------------------------------------
+// A copy from pageable memory waits for the stream and cannot be captured; a kernel's arguments are copied by the launch itself.  Up to 4 KB of them; one
+// launch for 512 numbers, an empty kernel's time.
+constexpr int kPut = 512;
+struct PutArgs {
+  float* to;
+  int n;
+  float x[kPut];
+};
+__global__ __launch_bounds__(kPut) void put_kernel(const PutArgs a) {
+  if ((int)threadIdx.x < a.n) a.to[threadIdx.x] = a.x[threadIdx.x];
+}
+hipError_t launch_put(const float* values, int n, float* to, hipStream_t stream) {
+  PutArgs a;
+  for (int i = 0; i < n; i += kPut) {
+    a.to = to + i;
+    a.n = n - i < kPut ? n - i : kPut;
+    for (int j = 0; j < kPut; ++j) a.x[j] = j < a.n ? values[i + j] : 0.f;
+    hipLaunchKernelGGL(put_kernel, dim3(1), dim3(kPut), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 }  // namespace ra

@@ -27,16 +27,17 @@ struct Library {
   decltype(&ra_select_pages_workspace) select_workspace;
   decltype(&ra_paged_attention) attention;
   decltype(&ra_paged_attention_workspace) attention_workspace;
+  decltype(&ra_put_floats) put_floats;
 } g_lib;
 
 // init_paged(addresses of the entry points, in the order above)
 PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long p[7];
-  if (!PyArg_ParseTuple(args, "KKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6)) return nullptr;
+  unsigned long long p[8];
+  if (!PyArg_ParseTuple(args, "KKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7)) return nullptr;
   g_lib = {reinterpret_cast<decltype(&ra_page_slots)>(p[0]),         reinterpret_cast<decltype(&ra_write_pages)>(p[1]),
            reinterpret_cast<decltype(&ra_page_means)>(p[2]),         reinterpret_cast<decltype(&ra_select_pages)>(p[3]),
            reinterpret_cast<decltype(&ra_select_pages_workspace)>(p[4]), reinterpret_cast<decltype(&ra_paged_attention)>(p[5]),
-           reinterpret_cast<decltype(&ra_paged_attention_workspace)>(p[6])};
+           reinterpret_cast<decltype(&ra_paged_attention_workspace)>(p[6]), reinterpret_cast<decltype(&ra_put_floats)>(p[7])};
   Py_RETURN_NONE;
 }
 
@@ -327,11 +328,17 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       p.n_pages_read = int32_of(pages.size(2), "pages");
     }
     if (slopes.defined()) {
-      c.here(slopes, "slopes");
+      const bool on_host = slopes.is_cpu();
+      if (!on_host) c.here(slopes, "slopes");
       c.no_grad(slopes, "slopes");
       TORCH_CHECK_VALUE(slopes.scalar_type() == at::kFloat && slopes.dim() == 1 && slopes.size(0) == x.size(1), "ALiBi slopes must be float32 [", x.size(1),
                         "], one for each query head, not ", slopes.scalar_type(), " ", slopes.sizes());
       heads_slopes = slopes.contiguous();
+      if (on_host) {  // (without a copy that waits for the GPU)
+        const Tensor there = empty({slopes.size(0)}, at::kFloat);
+        check("ra_put_floats", g_lib.put_floats(heads_slopes.data_ptr<float>(), int32_of(slopes.size(0), "slopes"), there.data_ptr<float>(), stream(c.device)));
+        heads_slopes = there;
+      }
       p.slopes = heads_slopes.data_ptr<float>();
     }
     p.B = int32_of(B, "block_table");

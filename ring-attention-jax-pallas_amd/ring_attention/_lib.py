@@ -183,6 +183,7 @@ EXPORTS = {
                                   C.c_void_p]),
     "ra_paged_attention_workspace": (C.c_int64, [C.POINTER(RaPagedParams)]),
     "ra_paged_attention": (C.c_int, [C.POINTER(RaPagedParams), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "ra_put_floats": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "ra_step_is_skippable": (C.c_int, [C.POINTER(RaBias), C.c_int32, C.c_int32]),
     "ra_fwd_step_check": (C.c_int, [C.POINTER(RaFwdStepParams)]),
     "ra_bwd_step_check": (C.c_int, [C.POINTER(RaBwdStepParams)]),
@@ -236,7 +237,7 @@ def host():
                                                                        lib.ra_bwd_terms_workspace)))
         module.init_paged(*(C.cast(f, C.c_void_p).value for f in (lib.ra_page_slots, lib.ra_write_pages, lib.ra_page_means, lib.ra_select_pages,
                                                                        lib.ra_select_pages_workspace, lib.ra_paged_attention,
-                                                                       lib.ra_paged_attention_workspace)))
+                                                                       lib.ra_paged_attention_workspace, lib.ra_put_floats)))
         _host = module
     return _host
 

@@ -16,8 +16,8 @@ model keeps them for many sequences of different lengths, which come, grow by a 
     pages = select_pages(q, means, block_table, lengths, page_size, count)
     out = paged_attention(q, k_pages, v_pages, block_table, lengths, pages=pages)
 
-Lengths, tables and the pool's state live on the GPU, nothing here waits for it, and every call can be captured into a graph: what the arrays
-hold when it is replayed counts.  None of them has a gradient.  What is on the device is not trusted: lengths are cut to what a row of the
+Lengths, tables and the pool's state live on the GPU, nothing here waits for it, and every call can be captured into a graph: what the arrays on
+the device hold when it is replayed counts.  None of them has a gradient.  What is on the device is not trusted: lengths are cut to what a row of the
 table can name, and pages and slots that are not in the pool take no part.  ``page_size`` is a power of two from 16 on, ``d`` 32, 64,
 96 or 128, up to 4096 sequences take part in a call.  Everything runs through ``libringattn_hip.so``.
 """
@@ -88,7 +88,7 @@ def paged_attention_with_lse(q, k_pages, v_pages, block_table, lengths, bias_fn:
             raise ValueError("attention over a paged cache takes causal, sliding-window and ALiBi terms only (a ring_attention.BiasFn of them)")
         window, slopes = bias_fn.window or 0, bias_fn.alibi_slopes
         window = min(window, 1 << 30)  # (wider than any sequence)
-        if slopes is not None and slopes.device != q.device:
+        if slopes is not None and slopes.is_cuda and slopes.device != q.device:
             slopes = slopes.to(q.device)
     return _lib.host().paged_attention(q, k_pages, v_pages, block_table, lengths, pages, slopes, window,
                                        1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale)
@@ -104,7 +104,9 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, bias_fn: Optional
         k_pages, v_pages: ``[pages, page_size, kv_heads, d]``, bfloat16 or float16.
         block_table, lengths: int32 ``[sequences, width]`` and ``[sequences]``.  A row of length 0 has an output of zeros and a logsumexp
             of -inf.  Several tokens of one sequence are several rows with the same pages, each with its own length.
-        bias_fn: ``sliding_window_bias(w)`` (pages outside of it are not read), ``alibi_bias(slopes)``, their sum, ``causal_bias()``.
+        bias_fn: ``sliding_window_bias(w)`` (pages outside of it are not read), ``alibi_bias(slopes)``, their sum, ``causal_bias()``.  Slopes on the
+            host (``alibi_slopes``) go along with a small kernel of each call, without waiting, and are what they are when the call is made or
+            captured; slopes on the device save that kernel, and slopes on another device are copied, which cannot be captured.
         sm_scale: softmax scale, 1/sqrt(d) if unspecified.
         pages: int32 ``[sequences, kv_heads, count]``, the pages of each sequence that are read (``select_pages``), each at most once. Of a
             sequence of n pages the first n entries count; numbers that are no pages are left out.

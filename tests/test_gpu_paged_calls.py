@@ -1,0 +1,78 @@
+"""Calls on a paged cache that a program may make: arguments in other places and layouts, captures, the largest numbers."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import ring_attention as ra
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _ints(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+def _np(t):
+    return t.detach().float().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+def _normal(*shape, seed=0, dtype=BF16):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return torch.empty(shape, dtype=dtype, device="cuda").normal_(generator=gen)
+
+
+@pytest.mark.parametrize("heads,group", [(2, 3), (350, 2), (1025, 1)])
+@pytest.mark.parametrize("width", [2, 100])
+def test_slopes_on_the_host_are_those_on_the_device(heads, group, width):
+    """Up to more than two kernels' arguments of them."""
+    k, v, q = _normal(4, 16, heads, 32), _normal(4, 16, heads, 32, seed=1), _normal(2, heads * group, 32, seed=2)
+    table, n = torch.randint(0, 4, (2, width), dtype=torch.int32, device="cuda"), _ints([width * 16 - 3, 1])
+    slopes = ra.alibi_slopes(heads * group)
+    want = ra.paged_attention_with_lse(q, k, v, table, n, bias_fn=ra.alibi_bias(slopes.cuda()))
+    plain = ra.paged_attention_with_lse(q, k, v, table, n)
+    for host in (slopes, torch.stack((slopes, slopes), 1)[:, 0]):
+        got = ra.paged_attention_with_lse(q, k, v, table, n, bias_fn=ra.alibi_bias(host))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not torch.equal(got[1], plain[1])
+    with pytest.raises(ValueError, match="one for each query head"):
+        ra.paged_attention(q, k, v, table, n, bias_fn=ra.alibi_bias(slopes[:1]))
+
+
+def test_slopes_on_the_host_are_not_waited_for():
+    k, v, q = _normal(4, 16, 2, 64), _normal(4, 16, 2, 64, seed=1), _normal(1, 4, 64, seed=2)
+    table, n, bias = _ints([[0, 1, 2, 3]]), _ints([60]), ra.alibi_bias(ra.alibi_slopes(4))
+    x = _normal(8192, 8192)
+    ra.paged_attention(q, k, v, table, n, bias_fn=bias), torch.mm(x, x)
+    torch.cuda.synchronize()
+    for _ in range(60):  # (some 50 ms of work)
+        torch.mm(x, x)
+    busy = torch.cuda.Event()
+    busy.record()
+    ra.paged_attention(q, k, v, table, n, bias_fn=bias)
+    assert not busy.query()
+    torch.cuda.synchronize()
+
+
+def test_a_captured_step_with_slopes_on_the_host():
+    """Made inside of the capture, as a model does it; the lengths move on between replays, and the program works and waits."""
+    k, v, q = _normal(40, 16, 2, 64), _normal(40, 16, 2, 64, seed=1), _normal(2, 4, 64, seed=2)
+    table, n = torch.randperm(40, device="cuda").to(torch.int32).view(2, 20), _ints([17, 250])
+
+    def step(where="cpu"):
+        return ra.paged_attention_with_lse(q, k, v, table, n, bias_fn=ra.sliding_window_bias(100) + ra.alibi_bias(ra.alibi_slopes(4).to(where)))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(6):
+        n.add_(3)
+        want = step("cuda")
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
