@@ -422,7 +422,7 @@ typedef struct ra_page_table {
  * free_state[1] from place free_state[0] on are free, around its end) and are written into the table; pages beyond the new length go
  * behind its last one; both in the order of the sequences.  Pages given back by a call are given out by later ones.  Results:
  *  - slots [n_slots]: page * page_size + place of each new token, sequence by sequence; -1 for one without a page and beyond the last
- *  - starts [B + 1]: where a sequence's tokens begin in slots
+ *  - starts [B + 1]: where a sequence's tokens begin in slots (at most 2^31 - 1)
  *  - granted [B]: the new lengths, cut to what there were pages for: the lengths to go on with
  *  - free_state_out [2]: the ring's new state (none of the results may overlap an operand) */
 int ra_page_slots(const ra_page_table* table, const int32_t* lengths, const int32_t* new_lengths, int32_t B, int32_t* free_pages,

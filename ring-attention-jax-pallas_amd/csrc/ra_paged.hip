@@ -78,10 +78,24 @@ RA_DEV float sum_of_rows(float x) {
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// Exclusive prefix sums of N values of each row, sums[n][0 .. B] in shared memory, so that whatever walks the rows' items in one line finds an
-// item's row by halving; all NT threads, neighbouring rows in a thread.  `values(row, x)` is called twice where B > NT.
-template <int NT, int N, class F>
+// Sums of numbers >= 0 that stop at 2^31 - 1: the order of additions does not change what they are.
+RA_DEV int capped_sum(int x, int y) { return (int)min((unsigned)x + (unsigned)y, 0x7fffffffu); }
+RA_DEV int scan_capped(int x) {
+  x = capped_sum(x, lane_before<0x111>(0, x));
+  x = capped_sum(x, lane_before<0x112>(0, x));
+  x = capped_sum(x, lane_before<0x114>(0, x));
+  x = capped_sum(x, lane_before<0x118>(0, x));
+  x = capped_sum(x, lane_before<0x142, 0xa>(0, x));
+  x = capped_sum(x, lane_before<0x143, 0xc>(0, x));
+  return x;
+}
+
+// Exclusive prefix sums of N values >= 0 of each row, sums[n][0 .. B] in shared memory, so that whatever walks the rows' items in one line finds an
+// item's row by halving; all NT threads, neighbouring rows in a thread.  `values(row, x)` is called twice where B > NT.  CAPPED: the first
+// value's sums may pass 2^31 - 1, and stop there.
+template <int NT, int N, bool CAPPED = false, class F>
 RA_DEV void scan_rows(int B, F values, int* const (&sums)[N], int (&red)[NT / 64][N]) {
+  auto plus = [](int n, int x, int y) { return CAPPED && n == 0 ? capped_sum(x, y) : x + y; };
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int per = (B + NT - 1) / NT, from = threadIdx.x * per, to = min(from + per, B);
   int x[N], mine[N], s[N];
@@ -90,22 +104,25 @@ RA_DEV void scan_rows(int B, F values, int* const (&sums)[N], int (&red)[NT / 64
   for (int i = from; i < to; ++i) {
     values(i, x);
 #pragma unroll
-    for (int n = 0; n < N; ++n) mine[n] += x[n];
+    for (int n = 0; n < N; ++n) mine[n] = plus(n, mine[n], x[n]);
   }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    s[n] = scan_sum(mine[n]);
-    if (lane == 63) red[wave][n] = s[n];
+    // (a sum that has stopped does not say what it was without this lane's value: that of the lane before does)
+    const bool capped = CAPPED && n == 0;
+    const int upto = capped ? scan_capped(mine[n]) : scan_sum(mine[n]);
+    if (lane == 63) red[wave][n] = upto;
+    s[n] = capped ? __shfl_up(upto, 1, 64) : upto - mine[n];
+    if (capped && lane == 0) s[n] = 0;
   }
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     int all = 0;
-    s[n] -= mine[n];
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) {
-      s[n] += w < wave ? red[w][n] : 0;
-      all += red[w][n];
+      s[n] = plus(n, s[n], w < wave ? red[w][n] : 0);
+      all = plus(n, all, red[w][n]);
     }
     if (threadIdx.x == 0) sums[n][B] = all;
   }
@@ -115,7 +132,7 @@ RA_DEV void scan_rows(int B, F values, int* const (&sums)[N], int (&red)[NT / 64
     if (per == 1) break;
     values(i, x);
 #pragma unroll
-    for (int n = 0; n < N; ++n) s[n] += x[n];
+    for (int n = 0; n < N; ++n) s[n] = plus(n, s[n], x[n]);
   }
   __syncthreads();
 }
@@ -151,12 +168,13 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
   auto old_of = [&](int b) { return min(max(a.before[b], 0), cap); };
   auto had_of = [&](int b) { return pages_of(old_of(b), a.shift); };
   auto wants_of = [&](int b) { return pages_of(min(max(a.after[b], 0), cap), a.shift); };
-  scan_rows<kSlotThreads, 3>(
+  // (pages fit 31 bits in all, as the table's entries do; tokens that are asked for need not)
+  scan_rows<kSlotThreads, 3, true>(
       a.B,
       [&](int b, int (&x)[3]) {
         const int n = a.before[b], m = a.after[b];
         const int pages = pages_of(min(max(m, 0), cap), a.shift) - pages_of(min(max(n, 0), cap), a.shift);
-        x[0] = max(m - max(n, 0), 0);
+        x[0] = max(max(m, 0) - max(n, 0), 0);
         x[1] = max(pages, 0);
         x[2] = max(-pages, 0);
       },
@@ -184,7 +202,7 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
   for (int t = me; t < a.n_slots; t += stride) {
     long long slot = -1;
     if (t < s_new[a.B]) {
-      const int b = row_of(s_new, a.B, t), n = old_of(b), position = n + t - s_new[b];
+      const int b = row_of(s_new, a.B, t), n = old_of(b), position = n + (t - s_new[b]);
       if (position >= n && position < granted_of(b)) {
         const int j = position >> a.shift, had = pages_of(n, a.shift);
         const int page = j < had ? a.table[b * a.table_sb + j] : a.ring[ring_at(s_take[b] + j - had)];

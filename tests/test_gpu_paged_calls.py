@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import ring_attention as ra
+from oracle import paged_oracle as R
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -76,3 +77,33 @@ def test_a_captured_step_with_slopes_on_the_host():
         if i % 2:
             torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+
+
+@pytest.mark.parametrize("B,nonsense", [(4, {1: 1 << 30, 2: 1 << 30, 3: 1 << 30}), (6, {1: 1 << 30, 2: (1 << 31) - 1, 3: 1 << 30, 4: 1 << 30}), (5, {0: -(1 << 31), 3: 1 << 30}),
+                                        (1000, {500: 1 << 30, 501: 1 << 30, 502: (1 << 31) - 1, 700: -(1 << 31), 998: 1 << 30}),
+                                        (4096, {i: (1 << 31) - 1 for i in range(2000, 4096)})])
+def test_lengths_that_no_caller_should_ask_for_leave_the_rows_before_them_alone(B, nonsense):
+    """Sums of the new tokens pass 31 and 32 bits.  The oracle is asked for lengths beyond what the table and the slots hold, but within reason: the same but for
+    where the rows behind begin, which is at most 2^31 - 1."""
+    size, width, tokens = 16, 4, 3 * B + 200
+    rng = np.random.default_rng(B)
+    P = 3 * B
+    lengths = rng.integers(0, 30, B).astype(np.int32)
+    table, at = np.full((B, width), -1, np.int32), 0
+    order = rng.permutation(P).astype(np.int32)
+    for b in range(B):
+        held = R.n_pages(int(lengths[b]), size)
+        table[b, :held] = order[at:at + held]
+        at += held
+    ring, state = np.roll(order, -at), np.array([0, P - at], np.int32)
+    new = (lengths + rng.integers(0, 4, B)).astype(np.int64)
+    for b, n in nonsense.items():
+        new[b] = n
+    t, r = _ints(table), _ints(ring)
+    got = ra.page_slots(t, _ints(lengths), _ints(new), r, _ints(state), size, tokens)
+    want = R.page_slots(table, lengths, np.clip(new, 0, tokens + 100), ring, state, size, tokens)
+    starts = np.minimum(np.concatenate(([0], np.maximum(np.maximum(new, 0) - lengths, 0).cumsum())), (1 << 31) - 1)
+    for x, y, name in zip((t, r, *got), want, ("table", "ring", "slots", "starts", "lengths", "state")):
+        if name == "lengths":
+            y = np.minimum(y, width * size)
+        assert np.array_equal(_np(x), starts if name == "starts" else y), name
