@@ -187,8 +187,9 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
     const int got = min(s_take[b + 1] - s_take[b], max(count - s_take[b], 0));
     return min(m, (pages_of(n, a.shift) + got) << a.shift);
   };
-  const int stride = gridDim.x * kSlotThreads, me = blockIdx.x * kSlotThreads + tid;
-  for (int b = me; b < a.B; b += stride) {
+  // (unsigned: a step behind the last of 2^31 - 1 is one, too)
+  const unsigned stride = gridDim.x * kSlotThreads, me = blockIdx.x * kSlotThreads + tid;
+  for (int b = (int)me; b < a.B; b += (int)stride) {
     a.granted[b] = granted_of(b);
     a.starts[b] = s_new[b];
   }
@@ -196,13 +197,13 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
     const int used = min(take, count);
     a.starts[a.B] = s_new[a.B];
     a.state_out[0] = (int)(((unsigned)first + (unsigned)used) % (unsigned)P);
-    a.state_out[1] = min(count - used + give, P);
+    a.state_out[1] = (int)min((unsigned)(count - used) + (unsigned)give, (unsigned)P);
   }
   auto ring_at = [&](int r) { return (int)(((unsigned)first + (unsigned)r) % (unsigned)P); };
-  for (int t = me; t < a.n_slots; t += stride) {
+  for (unsigned t = me; t < (unsigned)a.n_slots; t += stride) {
     long long slot = -1;
-    if (t < s_new[a.B]) {
-      const int b = row_of(s_new, a.B, t), n = old_of(b), position = n + (t - s_new[b]);
+    if ((int)t < s_new[a.B]) {
+      const int b = row_of(s_new, a.B, (int)t), n = old_of(b), position = n + ((int)t - s_new[b]);
       if (position >= n && position < granted_of(b)) {
         const int j = position >> a.shift, had = pages_of(n, a.shift);
         const int page = j < had ? a.table[b * a.table_sb + j] : a.ring[ring_at(s_take[b] + j - had)];
@@ -212,19 +213,20 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(const SlotsArgs a) 
     a.slots[t] = slot;
   }
   // (the rest from other workgroups on: the first one has had the rows)
-  auto from = [&](int third) { return (int)((blockIdx.x + gridDim.x * third / 3) % gridDim.x) * kSlotThreads + tid; };
-  for (int i = from(1); i < min(take, count); i += stride) {
-    const int b = row_of(s_take, a.B, i);
-    a.table[b * a.table_sb + had_of(b) + i - s_take[b]] = a.ring[ring_at(i)];
+  auto from = [&](unsigned third) { return (blockIdx.x + gridDim.x * third / 3) % gridDim.x * kSlotThreads + tid; };
+  for (unsigned i = from(1); i < (unsigned)min(take, count); i += stride) {
+    const int b = row_of(s_take, a.B, (int)i);
+    a.table[b * a.table_sb + had_of(b) + ((int)i - s_take[b])] = a.ring[ring_at((int)i)];
   }
-  for (int i = from(2); i < give; i += stride) {
-    const int b = row_of(s_give, a.B, i);
-    a.ring[(int)(((unsigned)ring_at(count) + (unsigned)i) % (unsigned)P)] = a.table[b * a.table_sb + wants_of(b) + i - s_give[b]];
+  for (unsigned i = from(2); i < (unsigned)give; i += stride) {
+    const int b = row_of(s_give, a.B, (int)i);
+    a.ring[(int)(((unsigned)ring_at(count) + i) % (unsigned)P)] = a.table[b * a.table_sb + wants_of(b) + ((int)i - s_give[b])];
   }
 }
 
 hipError_t launch_slots(const SlotsArgs& a, hipStream_t stream) {
-  const int items = a.n_slots > a.B ? a.n_slots : a.B, wgs = (items + kSlotThreads - 1) / kSlotThreads;
+  // (items: up to 2^31 - 1)
+  const int items = a.n_slots > a.B ? a.n_slots : a.B, wgs = (items - 1) / kSlotThreads + 1;
   hipLaunchKernelGGL(slots_kernel, dim3(wgs < 512 ? wgs : 512), dim3(kSlotThreads), 3 * (a.B + 1) * sizeof(int), stream, a);
   return hipGetLastError();
 }
@@ -299,8 +301,8 @@ __global__ __launch_bounds__(kMeanThreads) void means_kernel(const MeansArgs a) 
   const int cpr = a.D / 8, line = cpr * a.H, cols = a.cols;
   const int chunk = blockIdx.y * cols + tid % cols, step = kMeanThreads / cols, r0 = tid / cols;
   const int h = chunk / cpr, d = 8 * (chunk % cpr);
-  for (int i = blockIdx.x; i < total; i += gridDim.x) {
-    const int b = row_of(s_first, a.B, i), j = low(b) + i - s_first[b];
+  for (unsigned next = blockIdx.x; next < (unsigned)total; next += gridDim.x) {  // (of up to 2^31 - 1: a step behind them is no int)
+    const int i = (int)next, b = row_of(s_first, a.B, i), j = low(b) + (i - s_first[b]);
     const int n = min(size, min(max(a.after[b], 0), cap) - (j << a.table.shift));
     const int page = a.table.at[b * a.table.sb + j];
     const bool there = page >= 0 && page < a.table.n_pages;

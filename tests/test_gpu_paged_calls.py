@@ -107,3 +107,15 @@ def test_lengths_that_no_caller_should_ask_for_leave_the_rows_before_them_alone(
         if name == "lengths":
             y = np.minimum(y, width * size)
         assert np.array_equal(_np(x), starts if name == "starts" else y), name
+
+
+def test_the_most_slots():
+    """2^31 - 1 of them, 17 GB: the last step of a thread's walk over them passes what an int holds."""
+    table, ring = torch.full((2, 4), -1, dtype=torch.int32, device="cuda"), torch.arange(9, dtype=torch.int32, device="cuda")
+    most = (1 << 31) - 1
+    slots, starts, lengths, state = ra.page_slots(table, _ints([0, 0]), _ints([20, 40]), ring, _ints([0, 9]), 16, most)
+    assert slots.shape == (most,) and starts.tolist() == [0, 20, 60] and lengths.tolist() == [20, 40] and state.tolist() == [5, 4]
+    assert slots[:60].tolist() == [*range(20), *range(32, 72)] and table.tolist() == [[0, 1, -1, -1], [2, 3, 4, -1]]
+    assert int(slots[60:].max()) == int(slots[60:].min()) == -1
+    with pytest.raises(ValueError, match="num_tokens"):
+        ra.page_slots(table, _ints([0, 0]), _ints([20, 40]), ring, _ints([0, 9]), 16, most + 1)
