@@ -468,7 +468,7 @@ typedef struct ra_paged_params {
 } ra_paged_params;
 int64_t ra_paged_attention_workspace(const ra_paged_params* p);
 int ra_paged_attention(const ra_paged_params* p, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
-/* to[0 .. n) = values[0 .. n), which lie in host memory (ALiBi slopes that a program keeps there): they go along as arguments of a kernel, so that the call
+/* to[0 .. n) = values[0 .. n), n up to 65535, which lie in host memory (ALiBi slopes that a program keeps there): they go along as arguments of a kernel, so that the call
  * waits for nothing, values is free when it returns, and a captured call holds what values was then. */
 int ra_put_floats(const float* values, int32_t n, float* to, void* stream);
 

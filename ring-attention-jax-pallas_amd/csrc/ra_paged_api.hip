@@ -250,7 +250,7 @@ int ra_paged_attention(const ra_paged_params* p, void* out, float* lse, void* wo
   return done(launch_paged(a, p->D, p->dtype, shape, workspace, static_cast<hipStream_t>(stream)), "ra_paged_attention");
 }
 int ra_put_floats(const float* values, int32_t n, float* to, void* stream) {
-  if (n < 0) return fail(RA_ERR_SHAPE, "n must not be negative (got %d)", n);
+  if (n < 0 || n > 65535) return fail(RA_ERR_SHAPE, "0 to 65535 numbers, as many as there are query heads (got %d)", n);
   if (n == 0) return RA_OK;
   if (!values || !to) return fail(RA_ERR_NULL, "an array is NULL");
   if (misaligned(values, 4) || misaligned(to, 4)) return fail(RA_ERR_ALIGN, "arrays must be aligned to their elements");

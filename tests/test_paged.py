@@ -161,3 +161,9 @@ def test_numbers_from_the_host_reject_bad_arguments(lib):
     assert lib.ra_put_floats(0x1000, 0, 0x2000, None) == 0 and lib.ra_put_floats(None, 0, None, None) == 0  # nothing to do, nothing launched
     assert lib.ra_put_floats(0x1000, -1, 0x2000, None) == -2 and lib.ra_put_floats(None, 1, 0x2000, None) == -1
     assert lib.ra_put_floats(0x1000, 1, None, None) == -1 and lib.ra_put_floats(0x1002, 1, 0x2000, None) == -4 and lib.ra_put_floats(0x1000, 1, 0x2001, None) == -4
+
+
+def test_numbers_from_the_host_are_as_many_as_there_are_heads(lib):
+    """More would pass 31 bits in the loop over them."""
+    assert lib.ra_put_floats(None, (1 << 31) - 1, None, None) == -2 and lib.ra_put_floats(None, 65536, None, None) == -2
+    assert lib.ra_put_floats(None, 65535, None, None) == -1
