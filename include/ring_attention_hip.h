@@ -442,7 +442,7 @@ int ra_page_means(const ra_pool* k_pool, int32_t dtype, const ra_page_table* tab
 
 /* For each sequence and head of the cache the numbers (within the sequence) of the `count` pages with the largest score, in order:
  * (sum of the queries of the `group` heads that share it) . (the page's mean key), in 64 bits, ties from the lowest number.  The first `first`
- * and the last `last` pages are always among them.  A sequence of no more pages than `count` has all of them, and -1 behind.
+ * and the last `last` pages are always among them.  Pages that are not in the pool come behind all others, those included.  A sequence of no more pages than `count` has all of them, and -1 behind.
  * q: [B, H * group, D].  pages: [B, H, count] contiguous.  workspace: ra_select_pages_workspace() bytes, 16-byte aligned. */
 int64_t ra_select_pages_workspace(const ra_page_table* table, int32_t B, int32_t H);
 int ra_select_pages(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* means, int64_t means_stride_page, int64_t means_stride_head,

@@ -62,12 +62,13 @@ def select_pages(q, means, table, lengths, size: int, count: int, first: int = 1
             together = q[b].reshape(H, heads // H, d)[h].astype(np.float64).sum(0)
             page = table[b, :n]
             ok = (page >= 0) & (page < len(means))
-            score = np.where(ok, np.matmul(means[np.where(ok, page, 0), h].astype(np.float64), together), 0.0)
-            always = [i for i in range(n) if i < first or i >= n - last]
-            rest = [i for i in range(n) if not (i < first or i >= n - last)]
+            score = np.matmul(means[np.where(ok, page, 0), h].astype(np.float64), together)
+            always = [i for i in range(n) if ok[i] and (i < first or i >= n - last)]
+            rest = [i for i in range(n) if ok[i] and not (i < first or i >= n - last)]
             # not a number first, then the largest, the lowest number among equals
             rest.sort(key=lambda i: (not np.isnan(score[i]), -score[i] if not np.isnan(score[i]) else 0.0, i))
-            pick = sorted((always + rest)[:count]) if n > count else list(range(n))
+            missing = [i for i in range(n) if not ok[i]]  # pages that are not in the pool, where there are no others
+            pick = sorted((always + rest + missing)[:count]) if n > count else list(range(n))
             out[b, h, :len(pick)] = pick
     return out
 

@@ -356,7 +356,7 @@ hipError_t launch_means(const MeansArgs& args, int dtype, hipStream_t stream) {
 // lane ends with the sums of its own.  A load takes several heads of a page beside each other, where there are several: 16 x 8 heads, 37 MB of means,
 // 12.3 us, with a head alone in a load 16.5.  In 32 bits it would be 3 us less, and the choice would depend on the order of the sums.
 constexpr int kScoreRows = 256;  // (page, head)s of a workgroup, 64 a wave
-constexpr unsigned long long kForced = ~0ull;
+constexpr unsigned long long kForced = ~0ull, kNotThere = 0;  // (before and behind all numbers: that of -inf is larger than 0)
 RA_DEV unsigned long long ordered(double x) {
   if (x != x) return kForced - 1;  // (not a number: before every number, as sorting has it)
   const unsigned long long u = __builtin_bit_cast(unsigned long long, x + 0.0);  // (-0 and 0 are equal)
@@ -441,7 +441,7 @@ struct Scores {
     }
     exchange<LPR / 2>(s, c);  // (lane c of a row's lanes: the rows of load c)
     const int p = p0 + in_wave(), page = __shfl(mine, in_wave(), 64);
-    if (page < 0 || page >= a.table.n_pages) s[0] = 0.0;
+    if (page < 0 || page >= a.table.n_pages) return kNotThere;
     return p < a.first || p >= n - a.last ? kForced : ordered(s[0]);
   }
 };

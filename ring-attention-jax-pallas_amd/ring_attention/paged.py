@@ -72,7 +72,8 @@ def select_pages(q, means, block_table, lengths, page_size: int, count: int, fir
 
     The query heads that share a head of the cache share its pages too: a page's score is the sum of their queries times the page's
     mean key, in 64 bits.  Of each sequence the ``first`` and the ``last`` pages and, of the others, those with the largest scores are chosen
-    (of equal ones the lowest), ``count`` in all.  A mean that is not a number ranks before all numbers.
+    (of equal ones the lowest), ``count`` in all.  A mean that is not a number ranks before all numbers, and a page that is not in
+    the pool behind all pages that are.
 
     Returns int32 ``[sequences, kv_heads, count]``, numbers of pages within their sequence, in order; a sequence of fewer pages has all
     of them, and -1 behind."""

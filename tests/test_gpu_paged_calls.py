@@ -119,3 +119,27 @@ def test_the_most_slots():
     assert int(slots[60:].max()) == int(slots[60:].min()) == -1
     with pytest.raises(ValueError, match="num_tokens"):
         ra.page_slots(table, _ints([0, 0]), _ints([20, 40]), ring, _ints([0, 9]), 16, most + 1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("width", [40, 500, 1500, 9000])
+def test_pages_that_are_not_in_the_pool_take_no_place_of_others(dtype, width):
+    """Every score is negative, some are -inf; a third of the entries name no page, the first and the last of a sequence among them."""
+    P, H, d = 30, 2, 64
+    means = _normal(P, H, d, seed=3, dtype=dtype).abs()
+    means[7, 0, 0] = math.inf
+    q = -_normal(3, 2 * H, d, seed=4, dtype=dtype).abs() - 0.01
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(width)
+    table = torch.randint(-P // 2, P, (3, width), generator=gen, device="cuda", dtype=torch.int32)
+    table[:, 5], table[0, 0], table[1, width - 1] = P, -1, 1 << 30
+    table[2] = -1
+    table[2, 3:6] = torch.tensor([4, 2, 7], dtype=torch.int32)  # (fewer than are chosen)
+    n = _ints([width * 16, width * 16 - 3, width * 16])
+    inside = ((table >= 0) & (table < P)).sum(1)
+    for count, first, last in ((2, 1, 1), (12, 0, 0), (int(inside[0]) - 1, 1, 1), (width - 2, 3, 4)):
+        got = ra.select_pages(q, means, table, n, 16, count, first, last)
+        assert np.array_equal(_np(got), R.select_pages(_np(q), _np(means), _np(table), _np(n), 16, count, first, last))
+        there = torch.stack([table[b][got[b].long()] for b in range(3)])
+        there = ((there >= 0) & (there < P)).sum(2)
+        assert bool((there == inside.clamp(max=count)[:, None]).all())
