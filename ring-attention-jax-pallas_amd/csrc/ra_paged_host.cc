@@ -6,6 +6,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -92,6 +93,8 @@ struct Call {
   }
   void no_grad(const Tensor& t, const char* name) const {
     TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), name, " requires a gradient, and calls on a paged cache have none: use torch.no_grad()");
+    TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), name,
+                " has a tangent of forward-mode differentiation, and calls on a paged cache have no gradient");
   }
 };
 

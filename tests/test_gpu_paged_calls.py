@@ -143,3 +143,29 @@ def test_pages_that_are_not_in_the_pool_take_no_place_of_others(dtype, width):
         there = torch.stack([table[b][got[b].long()] for b in range(3)])
         there = ((there >= 0) & (there < P)).sum(2)
         assert bool((there == inside.clamp(max=count)[:, None]).all())
+
+
+def test_tangents_are_refused():
+    """Operands of forward-mode differentiation ask for no gradient; without a refusal the output has no tangent."""
+    fwd = torch.autograd.forward_ad
+    k, v, q = _normal(4, 16, 2, 64), _normal(4, 16, 2, 64, seed=1), _normal(1, 4, 64, seed=2)
+    table, n, means, slots = _ints([[0, 1, 2, 3]]), _ints([60]), k.mean(1), torch.zeros(1, dtype=torch.int64, device="cuda")
+    before = [x.clone() for x in (k, v, means)]
+    slopes = ra.alibi_slopes(4)
+    with fwd.dual_level():
+        def dual(x):
+            return fwd.make_dual(x, torch.ones_like(x))
+
+        for call in (lambda: ra.paged_attention(dual(q), k, v, table, n), lambda: ra.paged_attention(q, dual(k), v, table, n),
+                     lambda: ra.paged_attention(q, k, dual(v), table, n), lambda: ra.paged_attention(q, k, v, table, n, bias_fn=ra.alibi_bias(dual(slopes))),
+                     lambda: ra.paged_attention(q, k, v, table, n, bias_fn=ra.alibi_bias(dual(slopes.cuda()))),
+                     lambda: ra.select_pages(dual(q), means, table, n, 16, 2), lambda: ra.select_pages(q, dual(means), table, n, 16, 2),
+                     lambda: ra.write_pages(dual(q[:, :2]), q[:, 2:], k, v, slots), lambda: ra.write_pages(q[:, :2], dual(q[:, 2:]), k, v, slots),
+                     lambda: ra.write_pages(q[:, :2], q[:, 2:], dual(k), v, slots), lambda: ra.page_means(dual(k), table, n - 1, n, means),
+                     lambda: ra.page_means(k, table, n - 1, n, dual(means))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):  # (which leaves forward mode on)
+                call()
+        ra.paged_attention(q, k, v, table, n)
+    assert all(torch.equal(x, y) for x, y in zip(before, (k, v, means)))
