@@ -211,7 +211,7 @@ PyObject* write_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       slots.scalar_type(), " ", slots.sizes());
     if (k.size(0)) {
       // (a source that lies in a pool itself is read before anything is written)
-      auto apart = [&](const Tensor& t) { return t.is_alias_of(k_pages) || t.is_alias_of(v_pages) ? t.clone() : rows(t); };
+      auto apart = [&](const Tensor& t) { return t.is_alias_of(k_pages) || t.is_alias_of(v_pages) ? t.clone(at::MemoryFormat::Contiguous) : rows(t); };
       const Tensor x = apart(k), y = apart(v), s = slots.contiguous();
       check("ra_write_pages", g_lib.write_pages(x.data_ptr(), stride_of(x, 0), stride_of(x, 1), y.data_ptr(), stride_of(y, 0), stride_of(y, 1),
                                                 row_dtype(x.scalar_type()), int32_of(x.size(0), "k"), (int32_t)x.size(1), (int32_t)x.size(2), &kp, &vp,

@@ -169,3 +169,17 @@ def test_tangents_are_refused():
                 call()
         ra.paged_attention(q, k, v, table, n)
     assert all(torch.equal(x, y) for x, y in zip(before, (k, v, means)))
+
+
+def test_tokens_that_lie_in_the_pool_in_another_order():
+    """Heads and dimensions of the pool exchanged (as many of both): a copy that keeps the order of dense strides would not do."""
+    k, v = _normal(3, 16, 32, 32), _normal(3, 16, 32, 32, seed=1)
+    want = [x.flatten(0, 1).transpose(1, 2).contiguous().view_as(x) for x in (k, v)]
+    ra.write_pages(k.flatten(0, 1).transpose(1, 2), v.flatten(0, 1).transpose(1, 2), k, v, torch.arange(48, device="cuda"))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    # every second token to the place behind it
+    want = [x.clone() for x in (k, v)]
+    for x in want:
+        x.view(48, 32, 32)[1::2] = x.view(48, 32, 32)[::2]
+    ra.write_pages(k.flatten(0, 1)[::2], v.flatten(0, 1)[::2], k, v, torch.arange(1, 48, 2, device="cuda"))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
