@@ -144,11 +144,12 @@ void check_pair(const Tensor& k, const Tensor& v) {
                     v.scalar_type(), " must be of one shape and type");
 }
 
-// [n, heads, d], as the kernels take it: itself or a copy.
+// [n, heads, d], as the kernels take it: itself or a copy (one that is contiguous, too, where it does not begin on 16 bytes).
+Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
 Tensor rows(const Tensor& t) {
   const bool ok = t.stride(2) == 1 && aligned(t) && !((stride_of(t, 0) | stride_of(t, 1)) & 7) && stride_of(t, 0) >= 0 && stride_of(t, 1) >= 0 &&
                   t.size(1) * stride_of(t, 1) <= INT32_MAX;
-  return ok ? t : t.contiguous();
+  return ok ? t : copy_of(t);
 }
 
 int32_t int32_of(int64_t n, const char* name) {
@@ -211,7 +212,7 @@ PyObject* write_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       slots.scalar_type(), " ", slots.sizes());
     if (k.size(0)) {
       // (a source that lies in a pool itself is read before anything is written)
-      auto apart = [&](const Tensor& t) { return t.is_alias_of(k_pages) || t.is_alias_of(v_pages) ? t.clone(at::MemoryFormat::Contiguous) : rows(t); };
+      auto apart = [&](const Tensor& t) { return t.is_alias_of(k_pages) || t.is_alias_of(v_pages) ? copy_of(t) : rows(t); };
       const Tensor x = apart(k), y = apart(v), s = slots.contiguous();
       check("ra_write_pages", g_lib.write_pages(x.data_ptr(), stride_of(x, 0), stride_of(x, 1), y.data_ptr(), stride_of(y, 0), stride_of(y, 1),
                                                 row_dtype(x.scalar_type()), int32_of(x.size(0), "k"), (int32_t)x.size(1), (int32_t)x.size(2), &kp, &vp,

@@ -183,3 +183,26 @@ def test_tokens_that_lie_in_the_pool_in_another_order():
         x.view(48, 32, 32)[1::2] = x.view(48, 32, 32)[::2]
     ra.write_pages(k.flatten(0, 1)[::2], v.flatten(0, 1)[::2], k, v, torch.arange(1, 48, 2, device="cuda"))
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+@pytest.mark.parametrize("by", [1, 4, 8])
+def test_rows_that_begin_anywhere(by):
+    """Contiguous, but not on 16 bytes, as a piece of a larger buffer lies; by 8 it is taken as it is."""
+    k, v = _normal(4, 16, 2, 64), _normal(4, 16, 2, 64, seed=1)
+    table, n, means = _ints([[0, 1, 2, 3]] * 3), _ints([60, 30, 5]), k.float().mean(1).to(BF16)
+
+    def moved(x):
+        at = torch.empty(x.numel() + by, dtype=x.dtype, device="cuda")[by:].view_as(x)
+        assert at.copy_(x).is_contiguous()
+        return at
+
+    q, pools = _normal(3, 4, 64, seed=2), [(k.clone(), v.clone()) for _ in range(2)]
+    slots = torch.tensor([3, 17, 40], device="cuda")
+    for kind in (BF16, F32):
+        new = [_normal(3, 2, 64, seed=s, dtype=kind) for s in (5, 6)]
+        ra.write_pages(*new, *pools[0], slots)
+        ra.write_pages(*(moved(x) for x in new), *pools[1], slots)
+        assert torch.equal(pools[0][0], pools[1][0]) and torch.equal(pools[0][1], pools[1][1]) and not torch.equal(pools[0][0], k)
+    for x, y in zip(ra.paged_attention_with_lse(q, k, v, table, n), ra.paged_attention_with_lse(moved(q), k, v, table, n)):
+        assert torch.equal(x, y)
+    assert torch.equal(ra.select_pages(q, means, table, n, 16, 2), ra.select_pages(moved(q), means, table, n, 16, 2))
