@@ -206,3 +206,29 @@ def test_rows_that_begin_anywhere(by):
     for x, y in zip(ra.paged_attention_with_lse(q, k, v, table, n), ra.paged_attention_with_lse(moved(q), k, v, table, n)):
         assert torch.equal(x, y)
     assert torch.equal(ra.select_pages(q, means, table, n, 16, 2), ra.select_pages(moved(q), means, table, n, 16, 2))
+
+
+def test_a_step_in_inference_mode():
+    """The tensors of such a program have no versions; its results are of the same kind."""
+    def step(s):
+        slots, _, n, state = ra.page_slots(s["table"], s["n"], s["n"] + 3, s["ring"], s["state"], 16, 6)
+        ra.write_pages(s["new"], s["new"] * 2, s["k"], s["v"], slots)
+        ra.page_means(s["k"], s["table"], s["n"], n, s["means"])
+        pages = ra.select_pages(s["q"], s["means"], s["table"], n, 16, 2)
+        return (n, state, pages, *ra.paged_attention_with_lse(s["q"], s["k"], s["v"], s["table"], n, pages=pages, bias_fn=ra.alibi_bias(ra.alibi_slopes(4))))
+
+    def made():
+        k = _normal(9, 16, 2, 64)
+        return dict(table=_ints([[0, 1, 2, -1], [3, 4, 5, -1]]), n=_ints([40, 47]), ring=_ints([6, 7, 8, 0, 0, 0, 0, 0, 0]), state=_ints([0, 3]), k=k, v=k * 3,
+                    means=k.mean(1), new=_normal(6, 2, 64, seed=1), q=_normal(2, 4, 64, seed=2))
+
+    want = made()
+    out = step(want)
+    with torch.inference_mode():
+        for s in (made(), want | {x: want[x].clone() for x in ("k", "v", "means", "table", "ring")}):
+            got = step(s)
+            assert all(x.is_inference() for x in got) and all(torch.equal(x, y) for x, y in zip(got[3:], out[3:]))
+    held = made()
+    with torch.inference_mode():
+        got = step(held)
+    assert all(torch.equal(x, y) for x, y in zip(got, out)) and all(torch.equal(held[x], want[x]) for x in want)
