@@ -5,7 +5,6 @@
 
 namespace ra {
 
-constexpr int kMaxRows = RA_MAX_PAGED_ROWS;  // sequences of one call: their prefix sums lie in shared memory
 constexpr int kStepKeys = 128;               // keys that a workgroup of the attention kernel takes at a time, 32 a wave
 // A (row, head) is one workgroup's where its keys and values by the table are at most 256 KB (keys x D up to kWholeSize), which a compute unit
 // reads in some 6 us, or up to kWholeKeys keys where there are kWholeUnits of them; else the call's keys are shared between workgroups and their parts

@@ -105,8 +105,7 @@ void changed(const Tensor& t) {
 // An int32 array [B] that is read.
 Tensor ints(const Call& c, const Tensor& t, const char* name, int64_t B) {
   c.here(t, name);
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 1 && (B < 0 || t.size(0) == B), name, " must be int32 [", B < 0 ? "n" : std::to_string(B), "], not ",
-                    t.scalar_type(), " ", t.sizes());
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == B, name, " must be int32 [", B, "], not ", t.scalar_type(), " ", t.sizes());
   return t.contiguous();
 }
 

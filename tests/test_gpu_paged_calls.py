@@ -225,9 +225,8 @@ def test_a_step_in_inference_mode():
     want = made()
     out = step(want)
     with torch.inference_mode():
-        for s in (made(), want | {x: want[x].clone() for x in ("k", "v", "means", "table", "ring")}):
-            got = step(s)
-            assert all(x.is_inference() for x in got) and all(torch.equal(x, y) for x, y in zip(got[3:], out[3:]))
+        got = step(made())
+        assert all(x.is_inference() for x in got) and all(torch.equal(x, y) for x, y in zip(got, out))
     held = made()
     with torch.inference_mode():
         got = step(held)
