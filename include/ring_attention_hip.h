@@ -420,7 +420,8 @@ typedef struct ra_page_table {
 
 /* Sequences go from lengths[b] to new_lengths[b] tokens.  Pages come from the head of the ring of free ones (free_pages [n_pages], of which
  * free_state[1] from place free_state[0] on are free, around its end) and are written into the table; pages beyond the new length go
- * behind its last one; both in the order of the sequences.  Pages given back by a call are given out by later ones.  Results:
+ * behind its last one; both in the order of the sequences.  Pages given back by a call are given out by later ones.  A page that
+ * several rows name would be given back by each of them that ends: one at most may.  Results:
  *  - slots [n_slots]: page * page_size + place of each new token, sequence by sequence; -1 for one without a page and beyond the last
  *  - starts [B + 1]: where a sequence's tokens begin in slots (at most 2^31 - 1)
  *  - granted [B]: the new lengths, cut to what there were pages for: the lengths to go on with

@@ -37,7 +37,8 @@ def page_slots(block_table, lengths, new_lengths, free_pages, free_state, page_s
     says where the new tokens go.
 
     Args:
-        block_table: int32 ``[sequences, width]``, rows contiguous; entries of new pages are written, others left.
+        block_table: int32 ``[sequences, width]``, rows contiguous; entries of new pages are written, others left.  A page belongs to one row here:
+            of rows that name the same page (which attention allows) one at most may end or shrink below it, or it is given back twice.
         lengths, new_lengths: int32 ``[sequences]``.  (A row that ends and takes a new sequence at once goes through 0 in a call of its own.)
         free_pages: int32 ``[pages]``, a ring: from place ``free_state[0]`` on, around its end, ``free_state[1]`` pages are free.  To
             begin with ``arange(pages)`` and ``(0, pages)``.  Pages given back are written behind the free ones.
