@@ -12,7 +12,7 @@ constexpr int kStepKeys = 128;               // keys that a workgroup of the att
 // 1024 keys, D=128, 8: 10.4 | 9.1, 32: 12.4 | 10.3, 128: 16.1 | 18.5, 256: 27.9 | 28.2, 1024: 99.6 | 92.2; 2048 keys, D=128, 8: 17.8 | 9.4, 128: 34.5 | 29.0;
 // 1000 keys, D=64, 8: 8.4 | 7.5 (from the host, which launches one kernel instead of two, 8.1 | 11), 128: 10.4 | 14.5, 1024: 45.3 | 61.3.
 // (The crossing goes by the number of keys more than by their bytes: 1000 keys of D=64 are taken whole for the host's sake, and lose 0.9 us in a graph.)  Lengths are not known
-// here: short rows in a table made for longer ones are shared.  1000 keys of 8 heads, D=64, by a table of 63 pages | of 1024 to 8192: in a graph 8.6 | 7.7, from the host 8.9 | 11.0.
+// here: short rows in a table made for longer ones are shared.  1000 keys of 8 heads, D=64, by a table of 63 pages | of 1024 to 8192: in a graph 8.7 | 7.7, from the host 9.0 | 10.5.
 constexpr int kWholeSize = 65536, kWholeKeys = 1024, kWholeUnits = 128;
 // Workgroups that share: kStepsEach steps for each (128 keys), and at least kFewWorkgroups, two on each compute unit as their registers allow at D = 128 (three, with registers spilled: 391 us for 335; at D = 96, 64 and 32 three, four and five fit, which
 // the rule does not use: its figures are D = 128's); at most

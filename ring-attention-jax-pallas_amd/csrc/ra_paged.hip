@@ -16,7 +16,8 @@ struct BF16 {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   static constexpr float kLift = 0.f;
-  static constexpr int kPieces = 3;  // of 8 bits each: all of a weight's 24
+  static RA_DEV unsigned cut2(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+  static RA_DEV float rest(float w, float lack) { return __builtin_fmaf(w, 0x1p-31f, lack); }
 };
 struct F16 {
   static RA_DEV float up(unsigned short x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -24,10 +25,11 @@ struct F16 {
   static RA_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
-  // Weights are rounded to fp16 as 2^15 times their value: 2^17 of them that are 2^-25 of the largest, each below fp16's least, make up 2^-8 of
+  // Weights go into the matrix unit as 2^15 times their value: 2^17 of them that are 2^-25 of the largest, each below fp16's least, make up 2^-8 of
   // the output.
   static constexpr float kLift = 15.f;
-  static constexpr int kPieces = 2;  // of 11 bits each
+  static RA_DEV unsigned cut2(float lo, float hi) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(lo, hi)); }
+  static RA_DEV float rest(float, float lack) { return fmaxf(lack, 0x1p-24f); }
 };
 
 RA_DEV int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
@@ -732,6 +734,7 @@ RA_DEV void load_values(unsigned (&v)[D / 32], const unsigned short* at) {
   }
 }
 
+constexpr int kPieces = 3;  // of a weight
 constexpr int kEntries = 1024, kNearRows = 1024;  // of a stretch's pages, of the rows' lengths in shared memory
 constexpr int kNowhere = 0x7ff00000;  // (a position behind every sequence, of 2^30 tokens at most; a page and a tile on top of it fit 32 bits)
 
@@ -919,17 +922,20 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
           w[j] = __builtin_amdgcn_exp2f(w[j] - base);
           l += w[j];
         }
-        // A weight goes in as pieces of the type's precision, what the ones before lack of it in the next, through the matrix unit, which has the time: the
-        // output is off by its own rounding and by sums in 32 bits.  (Two pieces of bf16 left 2^-17 of a weight: one output in 500 was the neighbour of the nearest number.)
-        u32x4 piece[T::kPieces];
+        // A weight goes in as three pieces, each of what the ones before lack of it, through the matrix unit, which has the time: all its 24 bits, so that the output
+        // is off by its own rounding and by sums in 32 bits.  (Two pieces of bf16 left 2^-17 of a weight: one output in 500 was the neighbour of the nearest number.)
+        // The first two are cut off, not rounded, and what is left is made no less than 2^-31 of the weight (fp16: than 2^-24, its least, 2^-39 of the largest weight): pieces
+        // of 0 or below it would make NaN of an infinite value.
+        u32x4 piece[kPieces];
+        float left[8];
 #pragma unroll
-        for (int n = 0; n < T::kPieces; ++n) {
+        for (int j = 0; j < 8; ++j) left[j] = w[j];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            piece[n][j] = T::down2(w[2 * j], w[2 * j + 1]);
-            w[2 * j] -= T::up((unsigned short)piece[n][j]);
-            w[2 * j + 1] -= T::up((unsigned short)(piece[n][j] >> 16));
-          }
+        for (int n = 0; n < kPieces; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) piece[n][j] = n + 1 < kPieces ? T::cut2(left[2 * j], left[2 * j + 1]) : T::down2(left[2 * j], left[2 * j + 1]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) left[j] = T::rest(w[j], left[j] - T::up((unsigned short)(piece[n][j / 2] >> (j & 1 ? 16 : 0))));
         }
 #pragma unroll
         for (int i = 0; i < DPL; ++i) {
@@ -938,7 +944,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, 2) void paged_kernel(const Paged
 #pragma unroll
           for (int j = 0; j < 4; ++j) vt[j] = __builtin_amdgcn_perm(x.v[2 * j + 1][i >> 1], x.v[2 * j][i >> 1], pick);
 #pragma unroll
-          for (int n = 0; n < T::kPieces; ++n) o[i] = T::mfma(vt, piece[n], o[i]);
+          for (int n = 0; n < kPieces; ++n) o[i] = T::mfma(vt, piece[n], o[i]);
         }
         if (step + 1 < chunk_end) load(step + 1, true);
       }

@@ -193,3 +193,29 @@ def test_means_of_the_most_heads():
     ra.page_means(k, _ints([[1, 0]]), _ints([0]), _ints([20]), means)
     for page, n in ((1, 16), (0, 4)):
         assert torch.equal(means[page], (k[page, :n].float().sum(0) / n).to(BF16))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("width", [13, 90])
+def test_values_that_are_not_finite(dtype, d, width):
+    """An infinite value that counts makes its own element of the output infinite, two of different signs or one that is no number make it none, and all other elements are
+    as they are without."""
+    c = Switches(20, 16, 2, d, dtype, 0.5, seed=d)
+    table = torch.arange(13, dtype=torch.int32, device="cuda").repeat(2, 1)
+    table = torch.nn.functional.pad(table, (0, width - 13), value=-1)
+    lengths, q = [200, 77], c.queries(2, 3)
+    want, want_lse = ra.paged_attention_with_lse(q, c.k, c.v, table, _ints(lengths))
+    v = c.v.clone()
+    v[1, 0, 0, 3], v[2, 0, 1, 5], v[4, 0, 1, d - 1], v[3, 0, 0, 8], v[4, 0, 0, 8], v[2, 0, 0, 0] = math.inf, -math.inf, math.inf, math.inf, -math.inf, math.nan
+    v[4, 13, 0, 4] = v[12, 8, 1, 4] = math.inf  # behind the second row's end and the first one's
+    want = want.view(2, 2, 3, d)
+    want[:, 0, :, 3], want[:, 1, :, 5], want[:, 1, :, d - 1], want[:, 0, :, 8], want[:, 0, :, 0] = math.inf, -math.inf, math.inf, math.nan, math.nan
+    seen = c.bits[:, 4, 13, 0]  # (within the first row, by the query heads for which it is on)
+    for g in range(3):
+        if seen[g % 2]:
+            want[0, 0, g, 4] = math.inf
+        else:
+            want[0, 0, g, 4] = math.nan  # (a weight of 0 times infinity)
+    got, lse = ra.paged_attention_with_lse(q, c.k, v, table, _ints(lengths))
+    assert torch.equal(lse, want_lse) and torch.allclose(got.view_as(want), want, rtol=0, atol=0, equal_nan=True)
